@@ -77,6 +77,23 @@ PROTOTYPES = {
     "gtm_debug_last_fit_kernel": [C.c_void_p, C.c_void_p],
     "gtm_debug_fit_phase_cycles": [C.c_void_p, C.c_void_p],
     "gtm_debug_logic_op_rate": [C.c_void_p, C.POINTER(C.c_double)],
+    "gtm_embed_workspace": [C.c_int64, C.c_int64, C.c_int, C.POINTER(C.c_uint64)],
+    "gtm_embed": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int,
+                  C.c_int64, C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_uint64],
+    "gtm_embed_gradient_workspace": [C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_uint64)],
+    "gtm_embed_gradient": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int,
+                           C.c_int64, C.c_float, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_uint64],
+    "gtm_softmax_workspace": [C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.POINTER(C.c_uint64)],
+    "gtm_softmax_loss": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int,
+                         C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64],
+    "gtm_softmax_loss_gradient": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,
+                                  C.c_int, C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
+                                  C.c_uint64],
+    "gtm_softmax_predict": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_float, C.c_void_p,
+                            C.c_void_p, C.c_void_p, C.c_uint64],
+    "gtm_softmax_failed": [C.c_int, C.POINTER(C.c_int)],
+    "gtm_adamw_step": [C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p,
+                       C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, C.c_uint32],
     "gtm_dataset_create_scored": [C.c_void_p, C.POINTER(GraphsView), C.c_int, C.c_void_p, C.POINTER(C.c_void_p)],
 }
 

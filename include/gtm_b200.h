@@ -238,6 +238,63 @@ int gtm_transform(gtm_model *model, gtm_dataset *dataset, int number_of_node_typ
 int gtm_transform_nodewise(gtm_model *model, gtm_dataset *dataset, int number_of_node_types, int64_t first, int64_t count,
                            int node_stride, int32_t *node_outputs_out, int32_t *class_sums_out);
 
+/* Readout operators.  NO COUNTERPART IN THE REFERENCE, whose `transform` (tm.py:814-851) hands clause outputs to learners of
+ * other libraries.  They work on DEVICE arrays without a model: row-major matrices whose rows lie `..._stride` elements apart,
+ * element types gtm_type, indices int32 or int64 (`..._64` = 1).  Work is queued on `cuda_stream` of `device` (the caller's
+ * current device is left as it is) and the call returns without synchronising; nothing is allocated, so that calls can be captured
+ * into a CUDA graph.  The caller's workspace (device memory, 256-byte aligned, contents arbitrary) belongs to one call at a time;
+ * its size comes from the ..._workspace function for the same arrays and sizes.  Sums are held in 32 bits. */
+typedef enum gtm_type { GTM_F32 = 0, GTM_BF16 = 1, GTM_F16 = 2 } gtm_type;
+
+/* Embedding lookup: out[b] = scale * sum of table[ids[i]] over offsets[b] <= i < offsets[b+1]; with offsets NULL one row per id
+ * (number_of_bags is ignored).  offsets must not decrease; they are kept within 0..number_of_ids.  A negative id is padding and adds
+ * nothing; the result of an id that the table does not have is NaN.  Bags may be empty: zeros. */
+int gtm_embed_workspace(int64_t number_of_ids, int64_t columns, int bags, uint64_t *bytes_out);
+int gtm_embed(int device, void *cuda_stream, int type, const void *table, int64_t rows, int64_t columns, int64_t row_stride, const void *ids, int ids_64,
+              int64_t number_of_ids, const void *offsets, int offsets_64, int64_t number_of_bags, float scale, void *out, int64_t out_stride, void *workspace,
+              uint64_t workspace_bytes);
+/* Its gradient: table_gradient[r] = scale * sum over the positions with ids[i] = r of gradient[bag of i].  Every row is written.  Ids
+ * that the table does not have add nothing.  The sum's order is that of the positions: results do not change from run to run. */
+int gtm_embed_gradient_workspace(int64_t number_of_ids, int64_t rows, int64_t columns, uint64_t *bytes_out);
+int gtm_embed_gradient(int device, void *cuda_stream, int type, const void *gradient, int64_t columns, int64_t gradient_stride, const void *ids, int ids_64,
+                       int64_t number_of_ids, const void *offsets, int offsets_64, int64_t number_of_bags, float scale, void *table_gradient, int64_t rows,
+                       int64_t row_stride, void *workspace, uint64_t workspace_bytes);
+
+/* Softmax cross entropy without keeping the logits l[n][v] = scale * features[n] . weights[v], scale > 0: normalisers[n] =
+ * log sum_v exp l[n][v], losses[n] = normalisers[n] - l[n][labels[n]].  Examples whose label is ignore_label have loss zero; the
+ * loss of a label that there is not is NaN.
+ * The gradient takes gradients[n * gradients_step] = dL/dlosses[n] (step 0: one value for all) and the normalisers of the forward
+ * call.  Ignored examples have gradient zero, whatever their features hold.
+ * gtm_softmax_predict gives the most probable label, the lowest of equal ones, and its log probability; -1 and NaN where the logits are
+ * not numbers. */
+int gtm_softmax_workspace(int type, const void *features, int64_t examples, int64_t features_stride, const void *weights, int64_t labels,
+                          int64_t weights_stride, int64_t columns, int gradient, uint64_t *bytes_out);
+int gtm_softmax_loss(int device, void *cuda_stream, int type, const void *features, int64_t examples, int64_t features_stride, const void *weights,
+                     int64_t number_of_labels, int64_t weights_stride, int64_t columns, const void *labels, int labels_64, int64_t ignore_label, float scale,
+                     float *losses, float *normalisers, void *workspace, uint64_t workspace_bytes);
+int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type, const void *features, int64_t examples, int64_t features_stride, const void *weights,
+                              int64_t number_of_labels, int64_t weights_stride, int64_t columns, const void *labels, int labels_64, int64_t ignore_label,
+                              float scale, const float *normalisers, const float *gradients, int64_t gradients_step, void *features_gradient,
+                              int64_t features_gradient_stride, void *weights_gradient, int64_t weights_gradient_stride, void *workspace,
+                              uint64_t workspace_bytes);
+int gtm_softmax_predict(int device, void *cuda_stream, int type, const void *features, int64_t examples, int64_t features_stride, const void *weights,
+                        int64_t number_of_labels, int64_t weights_stride, int64_t columns, float scale, int64_t *labels_out, float *log_probabilities_out,
+                        void *workspace, uint64_t workspace_bytes);
+/* Waits for the device and tells whether a wait inside a softmax kernel ran out since the last call (*failed_out = 0 or 1, then cleared).  Such
+ * waits are bounded at two seconds; results of a call in which one ran out are not to be used. */
+int gtm_softmax_failed(int device, int *failed_out);
+
+/* One AdamW step over a list of tensors, in place: with t = *steps + 1 (*steps, int64 in device memory, is then counted up), g = gradient *
+ * gradient_scale: m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2; p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m /
+ * (sqrt(v) / sqrt(1 - beta2^t) + eps).  The states of all tensors lie in two flat arrays in which every tensor starts at a multiple of 256
+ * elements (16-byte aligned).  state_bits 32: m and v, float.  state_bits 8: e4m3 codes of m and of sqrt(v) in units of one float scale per 256
+ * elements, rounded to one of their two neighbours by a hash of (seed, t, element).  copies (may be NULL) receive the parameters
+ * once more, as GTM_BF16 or GTM_F16.  No tensor, state or copy may overlap another. */
+int gtm_adamw_step(int device, void *cuda_stream, int64_t number_of_tensors, const int64_t *counts, int param_type, const void *const *params,
+                   int gradient_type, const void *const *gradients, int copy_type, const void *const *copies, int state_bits, void *first, void *second,
+                   float *first_scales, float *second_scales, int64_t *steps, double lr, double beta1, double beta2, double eps, double weight_decay,
+                   double gradient_scale, uint32_t seed);
+
 /* Differential-test taps (no counterpart call in the reference; they expose the buffers its kernels leave in
  * device memory between launches of tm.py:563-747).
  *  gtm_debug_evaluate: inference on one graph through the scoring kernel (path 0) or through the learning
