@@ -79,7 +79,7 @@ PROTOTYPES = {
     "gtm_debug_logic_op_rate": [C.c_void_p, C.POINTER(C.c_double)],
     "gtm_embed_workspace": [C.c_int64, C.c_int64, C.c_int, C.POINTER(C.c_uint64)],
     "gtm_embed": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int,
-                  C.c_int64, C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_uint64],
+                  C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_uint64],
     "gtm_embed_gradient_workspace": [C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_uint64)],
     "gtm_embed_gradient": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int,
                            C.c_int64, C.c_float, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_uint64],

@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kBlock = 256;                   // elements of a warp's turn, and of one 8-bit scale
 constexpr int kTensors = 512;                 // tensors of one launch: their table travels with the launch's arguments
-constexpr float kLargest = 448.f, kLeastScale = 1.1754943508222875e-38f, kLeastCode = 0.001953125f;
+constexpr float kLeastScale = 1.1754943508222875e-38f, kLeastCode = 0.001953125f;
 
 struct AdamTensor {
     void *param;
@@ -50,28 +50,39 @@ __device__ __forceinline__ unsigned mix(unsigned x)
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
-// e4m3 bits of x / scale, rounded with 16 random bits.  What is not finite is held as NaN.
-__device__ __forceinline__ unsigned encode(float x, float inverse, unsigned random, bool root)
+__device__ __forceinline__ float root_fast(float v)
 {
-    const float r = __fmul_rn(fabsf(x), inverse);
-    float q;
-    if (r >= 0.015625f) q = __uint_as_float((__float_as_uint(r) + (random << 4)) & ~0xfffffu);
-    else q = floorf(__fadd_rn(__fmul_rn(r, 512.f), (float)random * 1.52587890625e-5f)) * kLeastCode;
-    q = fminf(q, kLargest);
-    if (root && x > 0.f) q = fmaxf(q, kLeastCode);
-    // q is an e4m3 value: normal ones have their top three fraction bits at 20..22, the exponent's bias moves from 127 to 7
-    const unsigned bits = __float_as_uint(q);
-    unsigned code = q >= 0.015625f ? (bits >> 20) - (120u << 3) : (unsigned)(q * 512.f);
-    if (!finite(x)) code = 0x7f;
-    return code | (x < 0.f ? 0x80u : 0u);
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
 
-__device__ __forceinline__ float decode(unsigned code)
+// Values of four codes.
+__device__ __forceinline__ void decode4(unsigned codes, float (&v)[4])
 {
-    const unsigned c = code & 0x7f;
-    float v = c >= 8 ? __uint_as_float((c + (120u << 3)) << 20) : (float)c * kLeastCode;
-    if (c == 0x7f) v = __int_as_float(0x7fffffff);
-    return code & 0x80 ? -v : v;
+    unsigned low, high;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(low) : "h"((unsigned short)codes));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(high) : "h"((unsigned short)(codes >> 16)));
+    const float2 a = __half22float2(reinterpret_cast<const __half2 &>(low)), b = __half22float2(reinterpret_cast<const __half2 &>(high));
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+
+// Codes of four values that are codes' values already (NaN stays NaN).
+__device__ __forceinline__ unsigned encode4(const float (&v)[4])
+{
+    unsigned short low, high;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(low) : "f"(v[1]), "f"(v[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(high) : "f"(v[3]), "f"(v[2]));
+    return low | (unsigned)high << 16;
+}
+
+// The code's value that a magnitude in units of the scale is rounded to, with 16 random bits.  Normal values (2^-6 and above) have four
+// bits of fraction: random bits are added below and what is below is cut off.  Smaller ones are multiples of 2^-9.
+__device__ __forceinline__ float round_normal(float r, unsigned random) { return __uint_as_float((__float_as_uint(r) + (random << 4)) & ~0xfffffu); }
+__device__ __forceinline__ float round_small(float r, unsigned random)
+{
+    const float below_one = __uint_as_float(0x3f800000u | random << 7) - 1.f;      // random / 2^16
+    return floorf(__fadd_rn(__fmul_rn(r, 512.f), below_one)) * kLeastCode;
 }
 
 template <class T>
@@ -127,21 +138,17 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
         const long long n = t.count;
         const bool wide_p = (uintptr_t)t.param % (4 * sizeof(P)) == 0, wide_g = (uintptr_t)t.gradient % (4 * sizeof(G)) == 0;
         float p[2][4], g[2][4], m[2][4], u[2][4];
+        unsigned codes_m[2], codes_u[2];
         float scale_m = 0.f, scale_u = 0.f;
+        if (kNarrow) scale_m = a.first_scales[block], scale_u = a.second_scales[block];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             const long long i = i0 + j * 128 + lane * 4, flat = block * kBlock + j * 128 + lane * 4;
             load4((const P *)t.param, i, n, wide_p, p[j]);
             load4((const G *)t.gradient, i, n, wide_g, g[j]);
             if (kNarrow) {
-                const unsigned cm = *(const unsigned *)((const unsigned char *)a.first + flat), cu = *(const unsigned *)((const unsigned char *)a.second + flat);
-                if (j == 0) scale_m = a.first_scales[block], scale_u = a.second_scales[block];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    m[j][k] = __fmul_rn(decode(cm >> (8 * k)), scale_m);
-                    u[j][k] = __fmul_rn(decode(cu >> (8 * k)), scale_u);
-                    u[j][k] = __fmul_rn(u[j][k], u[j][k]);
-                }
+                codes_m[j] = *(const unsigned *)((const unsigned char *)a.first + flat);
+                codes_u[j] = *(const unsigned *)((const unsigned char *)a.second + flat);
             } else {
                 load4((const float *)a.first, flat, flat + 4, true, m[j]);
                 load4((const float *)a.second, flat, flat + 4, true, u[j]);
@@ -150,32 +157,84 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
         float largest_m = 0.f, largest_u = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
+            if (kNarrow) decode4(codes_m[j], m[j]), decode4(codes_u[j], u[j]);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const float gr = __fmul_rn(g[j][k], a.gradient_scale);
+                if (kNarrow) {
+                    m[j][k] = __fmul_rn(m[j][k], scale_m);
+                    u[j][k] = __fmul_rn(u[j][k], scale_u);
+                    u[j][k] = __fmul_rn(u[j][k], u[j][k]);
+                }
                 m[j][k] = __fadd_rn(__fmul_rn(m[j][k], a.b1), __fmul_rn(gr, a.other1));
                 u[j][k] = __fadd_rn(__fmul_rn(u[j][k], a.b2), __fmul_rn(__fmul_rn(gr, gr), a.other2));
-                const float root = __fsqrt_rn(u[j][k]);
-                const float moved = __fdiv_rn(m[j][k], __fadd_rn(__fmul_rn(root, root_correction), a.eps));
+                // next to 8-bit states the hardware's root (2^-23) and quotient (2^-22) are exact enough, and a third of the instructions
+                const float root = kNarrow ? root_fast(u[j][k]) : __fsqrt_rn(u[j][k]);
+                const float below = __fadd_rn(__fmul_rn(root, root_correction), a.eps);
+                const float moved = kNarrow ? __fdividef(m[j][k], below) : __fdiv_rn(m[j][k], below);
                 p[j][k] = __fsub_rn(__fmul_rn(p[j][k], a.decay), __fmul_rn(step_size, moved));
                 if (kNarrow) {
                     u[j][k] = root;
-                    if (finite(m[j][k])) largest_m = fmaxf(largest_m, fabsf(m[j][k]));
-                    if (finite(root)) largest_u = fmaxf(largest_u, root);
+                    largest_m = fmaxf(largest_m, fabsf(m[j][k]));           // NaN is passed over
+                    largest_u = fmaxf(largest_u, root);
                 }
             }
         }
-        float inverse_m = 0.f, inverse_u = 0.f;
         if (kNarrow) {
 #pragma unroll
             for (int o = 16; o; o /= 2) {
                 largest_m = fmaxf(largest_m, __shfl_xor_sync(~0u, largest_m, o));
                 largest_u = fmaxf(largest_u, __shfl_xor_sync(~0u, largest_u, o));
             }
+            if (!finite(largest_m) || !finite(largest_u)) {
+                // infinities are held as NaN and have no part in the scale
+                largest_m = largest_u = 0.f;
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if (finite(m[j][k])) largest_m = fmaxf(largest_m, fabsf(m[j][k]));
+                        else m[j][k] = __int_as_float(0x7fffffff);
+                        if (finite(u[j][k])) largest_u = fmaxf(largest_u, u[j][k]);
+                        else u[j][k] = __int_as_float(0x7fffffff);
+                    }
+#pragma unroll
+                for (int o = 16; o; o /= 2) {
+                    largest_m = fmaxf(largest_m, __shfl_xor_sync(~0u, largest_m, o));
+                    largest_u = fmaxf(largest_u, __shfl_xor_sync(~0u, largest_u, o));
+                }
+            }
             scale_m = fmaxf(__fmul_rn(largest_m, (float)(1.0 / 448.0)), kLeastScale);
             scale_u = fmaxf(__fmul_rn(largest_u, (float)(1.0 / 448.0)), kLeastScale);
-            inverse_m = __fdiv_rn(1.f, scale_m), inverse_u = __fdiv_rn(1.f, scale_u);
+            const float inverse_m = __fdiv_rn(1.f, scale_m), inverse_u = __fdiv_rn(1.f, scale_u);
             if (lane == 0) a.first_scales[block] = scale_m, a.second_scales[block] = scale_u;
+            const unsigned flat = (unsigned)(block * kBlock) + lane * 4;
+            bool small = false;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                unsigned random[4];
+                float qm[4], qu[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    random[k] = mix((flat + j * 128 + k) * 0x9e3779b1u + key);
+                    qm[k] = __fmul_rn(fabsf(m[j][k]), inverse_m), qu[k] = __fmul_rn(u[j][k], inverse_u);
+                    small |= !(qm[k] >= 0.015625f) | !(qu[k] >= 0.015625f);
+                }
+                if (!__any_sync(~0u, small)) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) qm[k] = round_normal(qm[k], random[k] >> 16), qu[k] = round_normal(qu[k], random[k] & 0xffff);
+                } else {                                             // zeros, NaN, and one in thousands of usual values
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        qm[k] = qm[k] >= 0.015625f ? round_normal(qm[k], random[k] >> 16) : round_small(qm[k], random[k] >> 16);
+                        qu[k] = qu[k] >= 0.015625f ? round_normal(qu[k], random[k] & 0xffff) : round_small(qu[k], random[k] & 0xffff);
+                        if (u[j][k] > 0.f) qu[k] = fmaxf(qu[k], kLeastCode);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) qm[k] = copysignf(qm[k], m[j][k]);
+                codes_m[j] = encode4(qm), codes_u[j] = encode4(qu);
+            }
         }
 #pragma unroll
         for (int j = 0; j < 2; j++) {
@@ -190,15 +249,8 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
                 else store4((__half *)t.copy, i, n, wide_c, p[j]);
             }
             if (kNarrow) {
-                unsigned cm = 0, cu = 0;
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const unsigned random = mix((unsigned)(flat + k) * 0x9e3779b1u + key);
-                    cm |= encode(m[j][k], inverse_m, random >> 16, false) << (8 * k);
-                    cu |= encode(u[j][k], inverse_u, random & 0xffff, true) << (8 * k);
-                }
-                *(unsigned *)((unsigned char *)a.first + flat) = cm;
-                *(unsigned *)((unsigned char *)a.second + flat) = cu;
+                *(unsigned *)((unsigned char *)a.first + flat) = codes_m[j];
+                *(unsigned *)((unsigned char *)a.second + flat) = codes_u[j];
             } else {
                 store4((float *)a.first, flat, flat + 4, true, m[j]);
                 store4((float *)a.second, flat, flat + 4, true, u[j]);

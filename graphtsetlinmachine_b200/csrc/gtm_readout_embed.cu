@@ -9,12 +9,15 @@
 // pieces of kPiece: there are no atomics and results do not change from run to run.
 #include "gtm_readout.cuh"
 
+#include <type_traits>
+#include <utility>
+
 namespace gtm_readout {
 namespace {
 
 // A warp adds up to kPiece rows.  Longer segments leave their first kPiece rows in `head` and the rest in `part`, one slot
 // per kPiece positions of the list: at most one such segment begins in a span of kPiece positions, and at most one goes on
-// through it, so that a slot has one owner.
+// through it, so that a slot has one owner.  `ends[span]` is the long segment that ends in a span, -1: none does.
 constexpr int kPiece = 128;
 
 struct GatherArgs {
@@ -22,261 +25,474 @@ struct GatherArgs {
     long long src_stride, rows;      // elements, rows of src
     const void *list;                // row of src per position
     int list_wide;
-    const void *offsets;             // segments [offsets[s], offsets[s + 1]) of the list; null: one position each
+    const void *offsets;             // segments [offsets[s], offsets[s + 1]) of the list
     int offsets_wide;
     long long positions, segments;
     int columns;
     float scale;
     void *out;
     long long out_stride;
-    float *head, *part;              // [spans][columns]
+    float *head, *part;              // [spans][partial_stride]
+    int partial_stride;
+    int *ends;
 };
 
-__device__ __forceinline__ long long clamp_offset(const GatherArgs &a, long long s)
+__device__ __forceinline__ long long clamp_offset(const void *offsets, int wide, long long positions, long long s)
 {
-    const long long o = index_at(a.offsets, a.offsets_wide, s);
-    return o < 0 ? 0 : o > a.positions ? a.positions : o;
+    const long long o = index_at(offsets, wide, s);
+    return o < 0 ? 0 : o > positions ? positions : o;
 }
 
-// Last segment that begins at or before `position`; -1: none does.
-__device__ long long segment_at(const GatherArgs &a, long long position)
+__device__ __forceinline__ long long clamp_offset(const GatherArgs &a, long long s) { return clamp_offset(a.offsets, a.offsets_wide, a.positions, s); }
+
+// Last segment that begins at or before `position`; -1: none does.  A warp asks together, 32 segments at a time.
+__device__ long long segment_at(const void *offsets, int wide, long long positions, long long segments, long long position)
 {
-    long long low = -1, high = a.segments;        // offsets[low] <= position < offsets[high]
+    const int lane = threadIdx.x & 31;
+    long long low = -1, high = segments;          // offsets[low] <= position < offsets[high]
     while (high - low > 1) {
-        const long long mid = (low + high) / 2;
-        if (clamp_offset(a, mid) <= position) low = mid;
-        else high = mid;
+        const long long step = (high - low - 1 + 31) / 32, at = low + 1 + lane * step;
+        const unsigned before = __ballot_sync(~0u, at < high && clamp_offset(offsets, wide, positions, at) <= position);
+        const int n = __popc(before);             // offsets do not decrease: the first n lanes
+        if (n < 32) high = min(high, low + 1 + n * step);
+        if (n > 0) low = low + 1 + (n - 1) * step;
     }
     return low;
 }
 
-// Columns of a lane: U runs of V next to each other, 32 lanes of V apart.
-template <class T, int V, int U>
-__device__ __forceinline__ void add_rows(const GatherArgs &a, long long begin, long long end, int column0, float (&acc)[U][V])
+__device__ __forceinline__ void add2(float2 &a, float x, float y)
 {
-    const int lane = threadIdx.x & 31;
-    const T *src = (const T *)a.src;
-    for (long long base = begin; base < end; base += 32) {
-        const int n = (int)min(32ll, end - base);
-        long long mine = -1;
-        if (lane < n) mine = index_at(a.list, a.list_wide, base + lane);
-        constexpr int kAhead = V * U * sizeof(T) >= 32 ? 4 : 8;
-        for (int i = 0; i < n; i += kAhead) {
-            Pack<T, V> got[kAhead][U];
-            long long row[kAhead];
+    unsigned long long &s = reinterpret_cast<unsigned long long &>(a);
+    const float2 b = make_float2(x, y);
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(reinterpret_cast<const unsigned long long &>(b)));
+}
+
+// Values of a pack as floats, two at a time.
+template <class T, int V>
+__device__ __forceinline__ void accumulate(float2 (&acc)[(V + 1) / 2], const Pack<T, V> &p)
+{
+    if constexpr (V == 1) acc[0].x += to_float(p.v[0]);
+    else
 #pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                row[k] = __shfl_sync(~0u, mine, (i + k) & 31);
-                if (i + k >= n) row[k] = -1;
+        for (int v = 0; v < V; v += 2) add2(acc[v / 2], to_float(p.v[v]), to_float(p.v[v + 1]));
+}
+
+// kLanes lanes have a row's columns, U runs of V next to each other, kLanes * V apart; the 32 / kLanes groups of a warp take rows in turn.
+template <class T, int V, int U, int kLanes>
+struct Gather {
+    static constexpr int kGroups = 32 / kLanes, kAhead = U == 1 ? 8 : 4, kColumns = kLanes * V * U;
+    float2 acc[U][(V + 1) / 2];
+    bool bad = false;                // an id beyond the table
+
+    __device__ __forceinline__ void add(const GatherArgs &a, long long begin, long long end, int column0, int *compact)
+    {
+        const int lane = threadIdx.x & 31, group = lane / kLanes;
+        const T *column[U];
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int c = column0 + (u * 32 + lane) * V;
-                    if (row[k] >= 0 && row[k] < a.rows && c < a.columns)
-                        got[k][u] = *(const Pack<T, V> *)(src + row[k] * a.src_stride + c);
-                    else
+        for (int u = 0; u < U; u++) {
+            // lanes behind the last column read the first one, and drop it
+            const int c = column0 + (u * kLanes + lane % kLanes) * V;
+            column[u] = (const T *)a.src + (c < a.columns ? c : 0);
 #pragma unroll
-                        for (int v = 0; v < V; v++) got[k][u].v[v] = from_float<T>(0.f);
-                }
+            for (int v = 0; v < (V + 1) / 2; v++) acc[u][v] = make_float2(0.f, 0.f);
+        }
+        for (long long base = begin; base < end; base += 32) {
+            int n = (int)min(32ll, end - base), mine = -1;
+            if (lane < n) {
+                const long long id = index_at(a.list, a.list_wide, base + lane);
+                mine = id >= a.rows ? -2 : id < 0 ? -1 : (int)id;
             }
+            const unsigned real = __ballot_sync(~0u, mine >= 0);
+            if (__popc(real) < n) {              // padding: the others move up
+                bad |= __any_sync(~0u, mine == -2);
+                n = __popc(real);
+                if (mine >= 0) compact[__popc(real & ((1u << lane) - 1))] = mine;
+                __syncwarp();
+                if (lane < n) mine = compact[lane];
+                __syncwarp();
+            }
+            int i = 0;
+            for (; i + kAhead * kGroups <= n; i += kAhead * kGroups) {
+                Pack<T, V> got[kAhead][U];
 #pragma unroll
-            for (int k = 0; k < kAhead; k++)
+                for (int k = 0; k < kAhead; k++) {
+                    const long long at = (long long)__shfl_sync(~0u, mine, i + k * kGroups + group) * a.src_stride;
+#pragma unroll
+                    for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + at);
+                }
+#pragma unroll
+                for (int k = 0; k < kAhead; k++)
+#pragma unroll
+                    for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
+            }
+            for (; i < n; i += 4 * kGroups) {
+                Pack<T, V> got[4][U];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int r = i + k * kGroups + group;
+                    const long long at = (long long)__shfl_sync(~0u, mine, r & 31) * a.src_stride;
+                    if (r < n)
+#pragma unroll
+                        for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + at);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (i + k * kGroups + group < n)
+#pragma unroll
+                        for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
+            }
+        }
+        if constexpr (kGroups > 1)
+#pragma unroll
+            for (int o = kLanes; o < 32; o *= 2)
 #pragma unroll
                 for (int u = 0; u < U; u++)
 #pragma unroll
-                    for (int v = 0; v < V; v++)
-                        acc[u][v] += row[k] >= a.rows ? __int_as_float(0x7fffffff) : to_float(got[k][u].v[v]);
-        }
+                    for (int v = 0; v < (V + 1) / 2; v++) {
+                        acc[u][v].x += __shfl_xor_sync(~0u, acc[u][v].x, o);
+                        if (V > 1) acc[u][v].y += __shfl_xor_sync(~0u, acc[u][v].y, o);
+                    }
     }
-}
 
-template <class T, int V, int U>
-__global__ void __launch_bounds__(256) gather_sum_kernel(const GatherArgs a)
+    __device__ __forceinline__ float value(int u, int v) const
+    {
+        return bad ? __int_as_float(0x7fffffff) : v % 2 ? acc[u][v / 2].y : acc[u][v / 2].x;
+    }
+};
+
+template <class T, int V, int U, int kLanes>
+__global__ void __launch_bounds__(256, 3) gather_sum_kernel(const GatherArgs a)
 {
+    __shared__ int compact[8][32];
+    using G = Gather<T, V, U, kLanes>;
     const long long unit = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-    const int lane = threadIdx.x & 31, column0 = blockIdx.y * (32 * V * U);
-    const long long spans = a.offsets ? (a.positions + kPiece - 1) / kPiece : 0;
+    const int lane = threadIdx.x & 31, column0 = blockIdx.y * G::kColumns;
     long long begin, end;
     float *to = nullptr;
     if (unit < a.segments) {
-        begin = a.offsets ? clamp_offset(a, unit) : unit;
-        end = a.offsets ? clamp_offset(a, unit + 1) : unit + 1;
+        begin = clamp_offset(a, unit), end = clamp_offset(a, unit + 1);
         if (end - begin > kPiece) {
-            to = a.head + begin / kPiece * a.columns;
+            to = a.head + begin / kPiece * a.partial_stride;
             end = begin + kPiece;
         }
     } else {
-        if (a.positions <= kPiece || unit >= a.segments + spans) return;
-        const long long span = unit - a.segments, s = segment_at(a, span * kPiece);
-        if (s < 0) return;
-        begin = max(span * kPiece, clamp_offset(a, s) + kPiece);
-        end = min((span + 1) * kPiece, clamp_offset(a, s + 1));
+        const long long span = unit - a.segments;
+        if (a.positions <= kPiece || span * kPiece >= a.positions) return;
+        const long long s = segment_at(a.offsets, a.offsets_wide, a.positions, a.segments, span * kPiece);
+        begin = end = 0;
+        long long last = 0;
+        if (s >= 0) {
+            last = clamp_offset(a, s + 1);
+            begin = max(span * kPiece, clamp_offset(a, s) + kPiece);
+            end = min((span + 1) * kPiece, last);
+        }
+        if (blockIdx.y == 0 && lane == 0) a.ends[span] = begin < end && end == last ? (int)s : -1;
         if (begin >= end) return;
-        to = a.part + span * a.columns;
+        to = a.part + span * a.partial_stride;
     }
-    float acc[U][V];
-#pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-        for (int v = 0; v < V; v++) acc[u][v] = 0.f;
-    add_rows<T, V, U>(a, begin, end, column0, acc);
+    G g;
+    g.add(a, begin, end, column0, compact[threadIdx.x / 32]);
+    if (lane >= kLanes) return;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const int c = column0 + (u * 32 + lane) * V;
+        const int c = column0 + (u * kLanes + lane) * V;
         if (c >= a.columns) continue;
         if (to) {
 #pragma unroll
-            for (int v = 0; v < V; v++) to[c + v] = acc[u][v];
+            for (int v = 0; v < V; v++) to[c + v] = g.value(u, v);
         } else {
             Pack<T, V> p;
 #pragma unroll
-            for (int v = 0; v < V; v++) p.v[v] = from_float<T>(acc[u][v] * a.scale);
+            for (int v = 0; v < V; v++) p.v[v] = from_float<T>(g.value(u, v) * a.scale);
             *(Pack<T, V> *)((T *)a.out + unit * a.out_stride + c) = p;
         }
     }
 }
 
-// Segments longer than kPiece: head and parts, added in the order of the list.  A block has the segment that begins in one span
-// (if one does) and 32 columns; its eight warps take every eighth part and are added in order.
+// Segments longer than kPiece: head and parts, added in the order of the list.  A warp has the segment that ends in its span (if one
+// does) and 128 columns; where a segment has more than kAlone parts, the block's eight warps take every eighth.
 template <class T>
 __global__ void __launch_bounds__(256) gather_join_kernel(const GatherArgs a)
 {
-    __shared__ float sums[8][32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, c = blockIdx.y * 32 + lane;
-    const long long span = blockIdx.x, last = min((span + 1) * kPiece, a.positions) - 1;
-    const long long s = segment_at(a, last);
-    if (s < 0) return;
-    const long long begin = clamp_offset(a, s), end = clamp_offset(a, s + 1);
-    if (begin < span * kPiece || end - begin <= kPiece) return;
-    const long long first = (begin + kPiece) / kPiece, n = (end - 1) / kPiece - first + 1;
-    float sum = 0.f;
-    if (c < a.columns)
+    constexpr int kAlone = 64;
+    __shared__ float4 sums[8][32];
+    __shared__ long long longest[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, c = blockIdx.y * 128 + lane * 4;
+    const long long span = (long long)blockIdx.x * 8 + warp;
+    const bool inside = c < a.partial_stride;
+    const auto sum_of = [&](long long first, long long n, int step) {
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (inside)
 #pragma unroll 8
-        for (long long i = warp; i < n; i += 8) sum += a.part[(first + i) * a.columns + c];
-    sums[warp][lane] = sum;
-    __syncthreads();
-    if (warp || c >= a.columns) return;
-    sum = a.head[span * a.columns + c];
+            for (long long i = 0; i < n; i += step) {
+                const float4 v = *(const float4 *)(a.part + (first + i) * a.partial_stride + c);
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+        return sum;
+    };
+    const auto write = [&](long long s, float4 sum) {
+        const float4 head = inside ? *(const float4 *)(a.head + clamp_offset(a, s) / kPiece * a.partial_stride + c) : sum;
+        const float v[4] = {head.x + sum.x, head.y + sum.y, head.z + sum.z, head.w + sum.w};
 #pragma unroll
-    for (int w = 0; w < 8; w++) sum += sums[w][lane];
-    ((T *)a.out)[s * a.out_stride + c] = from_float<T>(sum * a.scale);
+        for (int k = 0; k < 4; k++)
+            if (c + k < a.columns) ((T *)a.out)[s * a.out_stride + c + k] = from_float<T>(v[k] * a.scale);
+    };
+    const long long s = span * kPiece < a.positions ? a.ends[span] : -1;
+    long long first = 0, n = 0;
+    if (s >= 0) {
+        first = clamp_offset(a, s) / kPiece + 1;
+        n = span - first + 1;
+    }
+    if (n > 0 && n <= kAlone) write(s, sum_of(first, n, 1));
+    if (lane == 0) longest[warp] = n > kAlone ? s : -1;
+    __syncthreads();
+    for (int w = 0; w < 8; w++) {
+        const long long one = longest[w];
+        if (one < 0) continue;                  // the block together
+        const long long begin = clamp_offset(a, one) / kPiece + 1, parts = (long long)blockIdx.x * 8 + w - begin + 1;
+        sums[warp][lane] = sum_of(begin + warp, parts - warp, 8);
+        __syncthreads();
+        if (warp == 0) {
+            float4 sum = sums[0][lane];
+            for (int k = 1; k < 8; k++) sum.x += sums[k][lane].x, sum.y += sums[k][lane].y, sum.z += sums[k][lane].z, sum.w += sums[k][lane].w;
+            write(one, sum);
+        }
+        __syncthreads();
+    }
 }
 
-template <class T, int V, int U>
+template <class T, int V, int U, int kLanes>
 int launch_gather(const GatherArgs &a, cudaStream_t stream)
 {
-    const bool long_ones = a.offsets && a.positions > kPiece;
-    const long long spans = long_ones ? (a.positions + kPiece - 1) / kPiece : 0, units = a.segments + spans;
-    const int wide = 32 * V * U;
+    const long long spans = a.positions > kPiece ? (a.positions + kPiece - 1) / kPiece : 0, units = a.segments + spans;
+    const int wide = Gather<T, V, U, kLanes>::kColumns;
     const dim3 grid((unsigned)((units + 7) / 8), (unsigned)((a.columns + wide - 1) / wide));
-    gather_sum_kernel<T, V, U><<<grid, 256, 0, stream>>>(a);
+    gather_sum_kernel<T, V, U, kLanes><<<grid, 256, 0, stream>>>(a);
     GTM_CU(cudaGetLastError());
-    if (long_ones) {
-        gather_join_kernel<T><<<dim3((unsigned)spans, (unsigned)((a.columns + 31) / 32)), 256, 0, stream>>>(a);
+    if (spans) {
+        gather_join_kernel<T><<<dim3((unsigned)((spans + 7) / 8), (unsigned)((a.columns + 127) / 128)), 256, 0, stream>>>(a);
         GTM_CU(cudaGetLastError());
     }
     return GTM_OK;
 }
 
+// As few lanes as have a row's columns, so that a warp has several narrow rows.  A lane has 16 bytes of a row whatever the loads, and with
+// that sums have the same order for every alignment.
+template <class T, int V>
+int launch_lanes(const GatherArgs &a, cudaStream_t stream)
+{
+    constexpr int kWide = 16 / sizeof(T), U = kWide / V;
+    return a.columns <= 4 * kWide ? launch_gather<T, V, U, 4>(a, stream) : a.columns <= 8 * kWide ? launch_gather<T, V, U, 8>(a, stream)
+         : a.columns <= 16 * kWide ? launch_gather<T, V, U, 16>(a, stream) : launch_gather<T, V, U, 32>(a, stream);
+}
+
 // The widest loads that rows of both arrays start at a boundary of.
+template <class T>
+int launch_gather(const GatherArgs &a, cudaStream_t stream)
+{
+    const auto fits = [&](unsigned bytes) {
+        return aligned(a.src, a.src_stride * sizeof(T), bytes) && aligned(a.out, a.out_stride * sizeof(T), bytes) && a.columns * sizeof(T) % bytes == 0;
+    };
+    if (fits(16)) return launch_lanes<T, 16 / sizeof(T)>(a, stream);
+    if (sizeof(T) == 2 && fits(4)) return launch_lanes<T, 4 / sizeof(T)>(a, stream);
+    return launch_lanes<T, 1>(a, stream);
+}
+
 int launch_gather(const GatherArgs &a, int type, cudaStream_t stream)
 {
-    const int64_t size = (int64_t)type_bytes(type);
-    const auto fits = [&](unsigned bytes) {
-        return aligned(a.src, a.src_stride * size, bytes) && aligned(a.out, a.out_stride * size, bytes) && a.columns * size % bytes == 0;
-    };
-    if (type == GTM_F32) return fits(16) ? launch_gather<float, 4, 1>(a, stream) : launch_gather<float, 1, 4>(a, stream);
-    if (type == GTM_BF16)
-        return fits(16) ? launch_gather<__nv_bfloat16, 8, 1>(a, stream)
-             : fits(4)  ? launch_gather<__nv_bfloat16, 2, 4>(a, stream) : launch_gather<__nv_bfloat16, 1, 8>(a, stream);
-    return fits(16) ? launch_gather<__half, 8, 1>(a, stream)
-         : fits(4)  ? launch_gather<__half, 2, 4>(a, stream) : launch_gather<__half, 1, 8>(a, stream);
+    return type == GTM_F32 ? launch_gather<float>(a, stream) : type == GTM_BF16 ? launch_gather<__nv_bfloat16>(a, stream) : launch_gather<__half>(a, stream);
+}
+
+// Rows by id, without bags.  A thread makes 16 bytes of the result at a time, kEach of them at once: one load where the rows lie at
+// 16-byte boundaries, single elements (of two rows, or of several short ones) where they do not.  kNarrow: the result has fewer than 2^32 elements.
+template <class T, bool kWhole, bool kNarrow>
+__global__ void __launch_bounds__(256) embed_rows_kernel(const T *table, long long stride, long long rows, const void *ids, int ids_wide, long long count, int columns, float scale, T *out)
+{
+    constexpr int V = 16 / sizeof(T), kEach = kWhole ? 4 : 2;
+    const long long all = count * columns, step = (long long)gridDim.x * 256 * V;
+    for (long long first = ((long long)blockIdx.x * 256 + threadIdx.x) * V; first < all; first += step * kEach) {
+        Pack<T, V> p[kEach];
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            const long long at = first + e * step;
+            if (at >= all) continue;
+            long long row = kNarrow ? (long long)((unsigned)at / (unsigned)columns) : at / columns;
+            int c = (int)(at - row * columns);
+            long long id = index_at(ids, ids_wide, row);
+            if constexpr (kWhole) {
+                if (id >= 0 && id < rows) p[e] = *(const Pack<T, V> *)(table + id * stride + c);
+                else
+#pragma unroll
+                    for (int v = 0; v < V; v++) p[e].v[v] = from_float<T>(id < 0 ? 0.f : __int_as_float(0x7fffffff));
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    p[e].v[v] = from_float<T>(id < 0 ? 0.f : __int_as_float(0x7fffffff));
+                    if (at + v < all) {
+                        if (id >= 0 && id < rows) p[e].v[v] = table[id * stride + c];
+                        if (++c == columns && at + v + 1 < all) c = 0, id = index_at(ids, ids_wide, ++row);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; e++) {
+            const long long at = first + e * step;
+            if (at >= all) continue;
+#pragma unroll
+            for (int v = 0; v < V; v++) p[e].v[v] = from_float<T>(to_float(p[e].v[v]) * scale);
+            if (at + V <= all) *(Pack<T, V> *)(out + at) = p[e];
+            else
+#pragma unroll
+                for (int v = 0; v < V; v++)
+                    if (at + v < all) out[at + v] = p[e].v[v];
+        }
+    }
+}
+
+template <class T>
+int launch_rows(const void *table, int64_t stride, int64_t rows, const void *ids, int ids_wide, int64_t count, int64_t columns, float scale, void *out, cudaStream_t stream)
+{
+    constexpr int64_t V = 16 / sizeof(T);
+    const bool whole = aligned(table, stride * sizeof(T), 16) && columns % V == 0, narrow = count * columns < (int64_t)1 << 32;
+    const int64_t chunks = (count * columns + V - 1) / V, blocks = (chunks + 255) / 256;
+    const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
+#define GTM_ROWS(W, N) embed_rows_kernel<T, W, N><<<grid, 256, 0, stream>>>((const T *)table, stride, rows, ids, ids_wide, count, (int)columns, scale, (T *)out)
+    if (whole) { if (narrow) GTM_ROWS(true, true); else GTM_ROWS(true, false); }
+    else if (narrow) GTM_ROWS(false, true);
+    else GTM_ROWS(false, false);
+#undef GTM_ROWS
+    GTM_CU(cudaGetLastError());
+    return GTM_OK;
 }
 
 // ------------------------------------------------------------------------------------ ids sorted, for the gradient
 // Radix sort by digits of kDigit bits, the lowest first, of (id, bag) pairs; every pass keeps the order of equal digits.
 // Ids that the table does not have (padding, too large ones, positions outside every bag) sort behind its last row.
-constexpr int kDigit = 8, kDigits = 1 << kDigit, kSortThreads = 256, kPerThread = 16, kTile = kSortThreads * kPerThread;
+constexpr int kDigit = 8, kDigits = 1 << kDigit, kSortThreads = 256, kSortWarps = kSortThreads / 32;
 
-__global__ void __launch_bounds__(256) sort_keys_kernel(const void *ids, int ids_wide, long long n, const void *offsets, int offsets_wide,
-                                                        long long bags, unsigned rows, uint2 *pairs)
+// A warp has kEach * 32 pairs in a row, 32 at a time.
+template <int kEach> __device__ __forceinline__ long long sort_first() { return (long long)blockIdx.x * (kSortThreads * kEach) + threadIdx.x / 32 * (kEach * 32) + (threadIdx.x & 31); }
+
+__device__ __forceinline__ void sort_count(unsigned *hist, unsigned *counts)
 {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const long long id = index_at(ids, ids_wide, i);
-    unsigned key = id < 0 || id >= (long long)rows ? rows : (unsigned)id, bag = (unsigned)i;
-    if (offsets) {
-        GatherArgs a;
-        a.offsets = offsets, a.offsets_wide = offsets_wide, a.positions = n, a.segments = bags;
-        const long long s = segment_at(a, i);
-        if (s < 0 || i >= clamp_offset(a, s + 1)) key = rows;
-        bag = s < 0 ? 0 : (unsigned)s;
-    }
-    pairs[i] = make_uint2(key, bag);
+    __syncthreads();
+    counts[(long long)blockIdx.x * kDigits + threadIdx.x] = hist[threadIdx.x];
 }
 
+template <int kEach>
+__global__ void __launch_bounds__(kSortThreads) sort_keys_kernel(const void *ids, int ids_wide, long long n, const void *offsets, int offsets_wide, long long bags, unsigned rows,
+                                                                uint2 *pairs, unsigned *counts)
+{
+    __shared__ unsigned hist[kDigits];
+    hist[threadIdx.x] = 0;
+    __syncthreads();
+    const long long first = sort_first<kEach>(), lane = threadIdx.x & 31;
+    long long bag = -1;
+    if (offsets && first - lane < n) bag = segment_at(offsets, offsets_wide, n, bags, first - lane);
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+        const long long i = first + k * 32;
+        if (i >= n) break;
+        const long long id = index_at(ids, ids_wide, i);
+        unsigned key = id < 0 || id >= (long long)rows ? rows : (unsigned)id;
+        if (offsets) {
+            // the bag of a later position is the same or one of the next; behind many empty ones, by halves
+            for (int tries = 0; tries < 8 && bag + 1 < bags && clamp_offset(offsets, offsets_wide, n, bag + 1) <= i; tries++) bag++;
+            long long high = bags;
+            if (bag + 1 < bags && clamp_offset(offsets, offsets_wide, n, bag + 1) <= i)
+                while (high - bag > 1) {
+                    const long long mid = (bag + high) / 2;
+                    if (clamp_offset(offsets, offsets_wide, n, mid) <= i) bag = mid;
+                    else high = mid;
+                }
+            if (bag < 0 || i >= clamp_offset(offsets, offsets_wide, n, bag + 1)) key = rows;
+        } else {
+            bag = i;
+        }
+        pairs[i] = make_uint2(key, bag < 0 ? 0 : (unsigned)bag);
+        atomicAdd(&hist[key & (kDigits - 1)], 1u);
+    }
+    sort_count(hist, counts);
+}
+
+template <int kEach>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const uint2 *pairs, long long n, int shift, unsigned *counts)
 {
     __shared__ unsigned hist[kDigits];
-    for (int d = threadIdx.x; d < kDigits; d += kSortThreads) hist[d] = 0;
+    hist[threadIdx.x] = 0;
     __syncthreads();
-    const long long first = (long long)blockIdx.x * kTile;
-    for (int k = 0; k < kPerThread; k++) {
-        const long long i = first + k * kSortThreads + threadIdx.x;
-        if (i < n) atomicAdd(&hist[(pairs[i].x >> shift) & (kDigits - 1)], 1u);
-    }
-    __syncthreads();
-    for (int d = threadIdx.x; d < kDigits; d += kSortThreads) counts[(long long)d * gridDim.x + blockIdx.x] = hist[d];
+    const long long first = sort_first<kEach>();
+    unsigned key[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; k++)
+        if (first + k * 32 < n) key[k] = pairs[first + k * 32].x;
+#pragma unroll
+    for (int k = 0; k < kEach; k++)
+        if (first + k * 32 < n) atomicAdd(&hist[(key[k] >> shift) & (kDigits - 1)], 1u);
+    sort_count(hist, counts);
 }
 
-// Exclusive running sums of all counts, digit by digit, block by block.  One block.
-__global__ void __launch_bounds__(1024) sort_scan_kernel(unsigned *counts, long long n)
+// Counts [block][digit] become where each block's pairs of a digit go: running sums digit by digit, block by block.  One block;
+// a thread has a digit and every fourth part of the blocks.
+__global__ void __launch_bounds__(1024) sort_scan_kernel(unsigned *counts, int blocks)
 {
-    __shared__ unsigned warp_sums[32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    const long long per = (n + 1023) / 1024, first = per * threadIdx.x, last = min(n, first + per);
+    __shared__ unsigned sums[4][kDigits], warp_sums[8];
+    const int digit = threadIdx.x & (kDigits - 1), part = threadIdx.x / kDigits, lane = threadIdx.x & 31;
+    const int per = (blocks + 3) / 4, first = min(blocks, part * per), last = min(blocks, first + per);
     unsigned sum = 0;
-    for (long long i = first; i < last; i++) sum += counts[i];
-    unsigned run = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        const unsigned v = __shfl_up_sync(~0u, run, o);
-        if (lane >= o) run += v;
-    }
-    if (lane == 31) warp_sums[warp] = run;
+#pragma unroll 8
+    for (int b = first; b < last; b++) sum += counts[(long long)b * kDigits + digit];
+    sums[part][digit] = sum;
     __syncthreads();
-    if (warp == 0) {
-        unsigned w = warp_sums[lane];
+    unsigned all = 0, run = 0;
+    if (part == 0) {
+        all = sums[0][digit] + sums[1][digit] + sums[2][digit] + sums[3][digit];
+        run = all;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
-            const unsigned v = __shfl_up_sync(~0u, w, o);
-            if (lane >= o) w += v;
+            const unsigned v = __shfl_up_sync(~0u, run, o);
+            if (lane >= o) run += v;
         }
-        warp_sums[lane] = w;
+        if (lane == 31) warp_sums[digit / 32] = run;
     }
     __syncthreads();
-    run += (warp ? warp_sums[warp - 1] : 0u) - sum;
-    for (long long i = first; i < last; i++) {
-        const unsigned c = counts[i];
-        counts[i] = run;
+    if (part == 0) {
+        for (int w = 0; w < digit / 32; w++) run += warp_sums[w];
+        run -= all;
+        for (int q = 0; q < 4; q++) {
+            const unsigned c = sums[q][digit];
+            sums[q][digit] = run;
+            run += c;
+        }
+    }
+    __syncthreads();
+    run = sums[part][digit];
+#pragma unroll 8
+    for (int b = first; b < last; b++) {
+        const unsigned c = counts[(long long)b * kDigits + digit];
+        counts[(long long)b * kDigits + digit] = run;
         run += c;
     }
 }
 
+template <int kEach>
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const uint2 *pairs, long long n, int shift, const unsigned *counts, uint2 *sorted)
 {
-    __shared__ unsigned warp_hist[kSortThreads / 32][kDigits];
+    __shared__ unsigned warp_hist[kSortWarps][kDigits];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    for (int d = threadIdx.x; d < kSortThreads / 32 * kDigits; d += kSortThreads) (&warp_hist[0][0])[d] = 0;
-    __syncthreads();
-    // a warp has kPerThread * 32 pairs in a row, 32 at a time: equal digits keep their order
-    const long long first = (long long)blockIdx.x * kTile + warp * (kPerThread * 32) + lane;
-    uint2 pair[kPerThread];
-    unsigned rank[kPerThread];
 #pragma unroll
-    for (int k = 0; k < kPerThread; k++)
+    for (int w = 0; w < kSortWarps; w++) warp_hist[w][threadIdx.x] = 0;
+    const long long first = sort_first<kEach>();
+    uint2 pair[kEach];
+    unsigned rank[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; k++)
         if (first + k * 32 < n) pair[k] = pairs[first + k * 32];
+    unsigned run = counts[(long long)blockIdx.x * kDigits + threadIdx.x];
+    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kPerThread; k++) {
+    for (int k = 0; k < kEach; k++) {
         const bool real = first + k * 32 < n;
         const unsigned digit = real ? (pair[k].x >> shift) & (kDigits - 1) : kDigits;
         const unsigned peers = __match_any_sync(~0u, digit);
@@ -287,55 +503,69 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const uint2 *p
         __syncwarp();
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < kDigits; d += kSortThreads) {
-        unsigned run = counts[(long long)d * gridDim.x + blockIdx.x];
-        for (int w = 0; w < kSortThreads / 32; w++) {
-            const unsigned c = warp_hist[w][d];
-            warp_hist[w][d] = run;
-            run += c;
-        }
+#pragma unroll
+    for (int w = 0; w < kSortWarps; w++) {
+        const unsigned c = warp_hist[w][threadIdx.x];
+        warp_hist[w][threadIdx.x] = run;
+        run += c;
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kPerThread; k++)
+    for (int k = 0; k < kEach; k++)
         if (first + k * 32 < n) sorted[warp_hist[warp][(pair[k].x >> shift) & (kDigits - 1)] + rank[k]] = pair[k];
 }
 
-// Where each row's positions begin in the sorted list (offsets[rows]: where ids that are no row begin), and the list of bags.
+// Where each row's positions begin in the sorted list (offsets[rows]: where ids that are no row begin), and the list of bags.  The
+// pair at a position writes the offsets of the rows behind the pair before it; of many such rows, its warp does.
 __global__ void __launch_bounds__(256) sort_rows_kernel(const uint2 *sorted, long long n, long long rows, int *offsets, int *bags)
 {
     const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (t <= rows) {
-        long long low = 0, high = n;
-        while (low < high) {
-            const long long mid = (low + high) / 2;
-            if (sorted[mid].x < t) low = mid + 1;
-            else high = mid;
-        }
-        offsets[t] = (int)low;
+    const int lane = threadIdx.x & 31;
+    long long low = 0, high = 0;                   // offsets [low, high) are t
+    if (t <= n) {
+        const uint2 pair = t < n ? sorted[t] : make_uint2((unsigned)rows, 0u);
+        low = t == 0 ? 0 : (long long)sorted[t - 1].x + 1;
+        high = t == n ? rows + 1 : (long long)pair.x + 1;
+        if (t < n) bags[t] = (int)pair.y;
     }
-    if (t < n) bags[t] = (int)sorted[t].y;
+    if (high - low <= 8) {
+        for (long long r = low; r < high; r++) offsets[r] = (int)t;
+        high = low;
+    }
+    for (unsigned many = __ballot_sync(~0u, high > low); many; many &= many - 1) {
+        const int from = __ffs(many) - 1;
+        const long long first = __shfl_sync(~0u, low, from), last = __shfl_sync(~0u, high, from);
+        const int value = (int)__shfl_sync(~0u, t, from);
+        for (long long r = first + lane; r < last; r += 32) offsets[r] = value;
+    }
 }
 
 struct GradientSpace {
-    uint64_t pairs[2], counts, offsets, bags, head, part, total;
+    uint64_t pairs[2], counts, offsets, bags, head, part, ends, total;
     long long tiles, spans;
+    int each;
 };
+
+int64_t partial_stride(int64_t columns) { return (int64_t)round_up(columns, 4); }
 
 GradientSpace gradient_space(long long ids, long long rows, long long columns)
 {
     GradientSpace s;
     uint64_t at = 0;
     const auto take = [&](uint64_t bytes) { const uint64_t here = at; at += round_up(bytes, 256); return here; };
-    s.tiles = (ids + kTile - 1) / kTile;
+    // small blocks of pairs as long as they do not fill the GPU, large ones (fewer counts) then
+    s.each = ids > 148 * 4 * kSortThreads * 4 ? 16 : 4;
+    s.tiles = (ids + kSortThreads * s.each - 1) / (kSortThreads * s.each);
     s.spans = (ids + kPiece - 1) / kPiece;
     s.pairs[0] = take(ids * 8);
     s.pairs[1] = take(ids * 8);
     s.counts = take(s.tiles * kDigits * 4);
     s.offsets = take((rows + 1) * 4);
     s.bags = take(ids * 4);
-    s.head = take(ids > kPiece ? s.spans * columns * 4 : 0);
-    s.part = take(ids > kPiece ? s.spans * columns * 4 : 0);
+    const bool pieces = ids > kPiece;
+    s.head = take(pieces ? s.spans * partial_stride(columns) * 4 : 0);
+    s.part = take(pieces ? s.spans * partial_stride(columns) * 4 : 0);
+    s.ends = take(pieces ? s.spans * 4 : 0);
     s.total = at;
     return s;
 }
@@ -359,33 +589,41 @@ extern "C" int gtm_embed_workspace(int64_t ids, int64_t columns, int bags, uint6
 {
     if (!bytes_out) return fail(GTM_ERR_ARG, "gtm_embed_workspace: null output");
     GTM_TRY(check_sizes("gtm_embed_workspace", GTM_F32, 1, columns, ids, 0));
-    const uint64_t slots = bags && ids > kPiece ? (uint64_t)((ids + kPiece - 1) / kPiece) : 0;
-    *bytes_out = 2 * round_up(slots * columns * 4, 256);
+    const uint64_t spans = bags && ids > kPiece ? (uint64_t)((ids + kPiece - 1) / kPiece) : 0;
+    *bytes_out = 2 * round_up(spans * partial_stride(columns) * 4, 256) + round_up(spans * 4, 256);
     return GTM_OK;
 }
 
 extern "C" int gtm_embed(int device, void *cuda_stream, int type, const void *table, int64_t rows, int64_t columns, int64_t row_stride, const void *ids,
                          int ids_64, int64_t number_of_ids, const void *offsets, int offsets_64, int64_t number_of_bags, float scale, void *out,
-                         int64_t out_stride, void *workspace, uint64_t workspace_bytes)
+                         void *workspace, uint64_t workspace_bytes)
 {
     GTM_TRY(check_sizes("gtm_embed", type, rows, columns, number_of_ids, number_of_bags));
     const int64_t segments = offsets ? number_of_bags : number_of_ids;
     if (segments == 0) return GTM_OK;
     if (!table || !out || (!ids && number_of_ids)) return fail(GTM_ERR_ARG, "gtm_embed: null array");
-    if (row_stride < 0 || out_stride < columns) return fail(GTM_ERR_ARG, "gtm_embed: row stride %lld of the table, %lld of the result", (long long)row_stride, (long long)out_stride);
+    if (row_stride < 0) return fail(GTM_ERR_ARG, "gtm_embed: row stride %lld of the table", (long long)row_stride);
+    if ((uintptr_t)out % 16) return fail(GTM_ERR_ARG, "gtm_embed: the result does not start at a 16-byte boundary");
     uint64_t need = 0;
     GTM_TRY(gtm_embed_workspace(number_of_ids, columns, offsets != nullptr, &need));
     if (workspace_bytes < need || (need && ((uintptr_t)workspace % 16 || !workspace)))
         return fail(GTM_ERR_ARG, "gtm_embed: workspace of %llu bytes, %llu needed (16-byte aligned)", (unsigned long long)workspace_bytes, (unsigned long long)need);
     DeviceGuard guard(device);
     GTM_TRY(guard.status);
+    cudaStream_t stream = (cudaStream_t)cuda_stream;
+    if (!offsets)
+        return type == GTM_F32    ? launch_rows<float>(table, row_stride, rows, ids, ids_64, number_of_ids, columns, scale, out, stream)
+               : type == GTM_BF16 ? launch_rows<__nv_bfloat16>(table, row_stride, rows, ids, ids_64, number_of_ids, columns, scale, out, stream)
+                                  : launch_rows<__half>(table, row_stride, rows, ids, ids_64, number_of_ids, columns, scale, out, stream);
     GatherArgs a;
     a.src = table, a.src_stride = row_stride, a.rows = rows;
     a.list = ids, a.list_wide = ids_64, a.positions = number_of_ids;
     a.offsets = offsets, a.offsets_wide = offsets_64, a.segments = segments;
-    a.columns = (int)columns, a.scale = scale, a.out = out, a.out_stride = out_stride;
-    a.head = (float *)workspace, a.part = (float *)((char *)workspace + need / 2);
-    return launch_gather(a, type, (cudaStream_t)cuda_stream);
+    a.columns = (int)columns, a.scale = scale, a.out = out, a.out_stride = columns;
+    const uint64_t spans = (uint64_t)((number_of_ids + kPiece - 1) / kPiece), half = round_up(spans * partial_stride(columns) * 4, 256);
+    a.head = (float *)workspace, a.part = (float *)((char *)workspace + half), a.ends = (int *)((char *)workspace + 2 * half);
+    a.partial_stride = (int)partial_stride(columns);
+    return launch_gather(a, type, stream);
 }
 
 extern "C" int gtm_embed_gradient_workspace(int64_t ids, int64_t rows, int64_t columns, uint64_t *bytes_out)
@@ -415,26 +653,32 @@ extern "C" int gtm_embed_gradient(int device, void *cuda_stream, int type, const
     unsigned *counts = (unsigned *)(w + space.counts);
     const long long n = number_of_ids;
     if (n) {
-        sort_keys_kernel<<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(ids, ids_64, n, offsets, offsets_64, number_of_bags, (unsigned)rows, from);
-        GTM_CU(cudaGetLastError());
-        for (int shift = 0; shift < 32 && ((uint64_t)rows >> shift) != 0; shift += kDigit) {
-            sort_count_kernel<<<(unsigned)space.tiles, kSortThreads, 0, stream>>>(from, n, shift, counts);
+        const unsigned tiles = (unsigned)space.tiles;
+        const auto sort = [&](auto each) -> int {
+            constexpr int kEach = decltype(each)::value;
+            sort_keys_kernel<kEach><<<tiles, kSortThreads, 0, stream>>>(ids, ids_64, n, offsets, offsets_64, number_of_bags, (unsigned)rows, from, counts);
             GTM_CU(cudaGetLastError());
-            sort_scan_kernel<<<1, 1024, 0, stream>>>(counts, space.tiles * kDigits);
-            GTM_CU(cudaGetLastError());
-            sort_place_kernel<<<(unsigned)space.tiles, kSortThreads, 0, stream>>>(from, n, shift, counts, to);
-            GTM_CU(cudaGetLastError());
-            std::swap(from, to);
-        }
+            for (int shift = 0; shift < 32 && ((uint64_t)rows >> shift) != 0; shift += kDigit) {
+                if (shift) sort_count_kernel<kEach><<<tiles, kSortThreads, 0, stream>>>(from, n, shift, counts);
+                GTM_CU(cudaGetLastError());
+                sort_scan_kernel<<<1, 1024, 0, stream>>>(counts, (int)tiles);
+                GTM_CU(cudaGetLastError());
+                sort_place_kernel<kEach><<<tiles, kSortThreads, 0, stream>>>(from, n, shift, counts, to);
+                GTM_CU(cudaGetLastError());
+                std::swap(from, to);
+            }
+            return GTM_OK;
+        };
+        GTM_TRY(space.each == 4 ? sort(std::integral_constant<int, 4>()) : sort(std::integral_constant<int, 16>()));
     }
-    const long long threads = rows + 1 > n ? rows + 1 : n;
-    sort_rows_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, stream>>>(from, n, rows, (int *)(w + space.offsets), (int *)(w + space.bags));
+    sort_rows_kernel<<<(unsigned)((n + 256) / 256), 256, 0, stream>>>(from, n, rows, (int *)(w + space.offsets), (int *)(w + space.bags));
     GTM_CU(cudaGetLastError());
     GatherArgs a;
     a.src = gradient, a.src_stride = gradient_stride, a.rows = offsets ? number_of_bags : n;
     a.list = w + space.bags, a.list_wide = 0, a.positions = n;
     a.offsets = w + space.offsets, a.offsets_wide = 0, a.segments = rows;
     a.columns = (int)columns, a.scale = scale, a.out = table_gradient, a.out_stride = row_stride;
-    a.head = (float *)(w + space.head), a.part = (float *)(w + space.part);
+    a.head = (float *)(w + space.head), a.part = (float *)(w + space.part), a.ends = (int *)(w + space.ends);
+    a.partial_stride = (int)partial_stride(columns);
     return launch_gather(a, type, stream);
 }

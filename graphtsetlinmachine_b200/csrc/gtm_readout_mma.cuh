@@ -45,7 +45,7 @@ __device__ __forceinline__ void barrier_arrive_leader(unsigned barrier_in_leader
 __device__ __forceinline__ bool barrier_try(unsigned barrier, unsigned parity)
 {
     unsigned done;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(barrier), "r"(parity) : "memory");
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(barrier), "r"(parity) : "memory");
     return done;
 }
 

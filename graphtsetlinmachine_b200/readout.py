@@ -111,7 +111,7 @@ def embed(table, ids, offsets=None, scale=1.0):
         if size:
             workspace = _workspace(size, device)
     _lib.check(lib.gtm_embed(device.index, _stream(device), _TYPES[table.dtype], table.data_ptr(), rows, columns, stride, ids.data_ptr(), wide, ids.numel(),
-                             None if offsets is None else offsets.data_ptr(), wide_offsets, count, scale, out.data_ptr(), columns,
+                             None if offsets is None else offsets.data_ptr(), wide_offsets, count, scale, out.data_ptr(),
                              None if workspace is None else workspace.data_ptr(), size))
     return out
 

@@ -251,7 +251,7 @@ typedef enum gtm_type { GTM_F32 = 0, GTM_BF16 = 1, GTM_F16 = 2 } gtm_type;
  * nothing; the result of an id that the table does not have is NaN.  Bags may be empty: zeros. */
 int gtm_embed_workspace(int64_t number_of_ids, int64_t columns, int bags, uint64_t *bytes_out);
 int gtm_embed(int device, void *cuda_stream, int type, const void *table, int64_t rows, int64_t columns, int64_t row_stride, const void *ids, int ids_64,
-              int64_t number_of_ids, const void *offsets, int offsets_64, int64_t number_of_bags, float scale, void *out, int64_t out_stride, void *workspace,
+              int64_t number_of_ids, const void *offsets, int offsets_64, int64_t number_of_bags, float scale, void *out, void *workspace,
               uint64_t workspace_bytes);
 /* Its gradient: table_gradient[r] = scale * sum over the positions with ids[i] = r of gradient[bag of i].  Every row is written.  Ids
  * that the table does not have add nothing.  The sum's order is that of the positions: results do not change from run to run. */

@@ -25,7 +25,7 @@ POINTER = C.c_void_p(4096)      # never followed: the calls below are refused fi
 
 def _embed(lib, **kw):
     a = dict(device=0, stream=None, type=0, table=POINTER, rows=4, columns=8, stride=8, ids=POINTER, wide=1, n=3, offsets=None, wide_offsets=0, bags=0, scale=1.0,
-             out=POINTER, out_stride=8, workspace=None, bytes=0)
+             out=POINTER, workspace=None, bytes=0)
     a.update(kw)
     return lib.gtm_embed(*a.values())
 
@@ -53,7 +53,7 @@ def _predict(lib, **kw):
 
 @pytest.mark.parametrize("call,bad", [
     (_embed, dict(type=3)), (_embed, dict(rows=0)), (_embed, dict(columns=0)), (_embed, dict(n=-1)), (_embed, dict(n=1 << 31)), (_embed, dict(table=None)),
-    (_embed, dict(ids=None)), (_embed, dict(out=None)), (_embed, dict(stride=-8)), (_embed, dict(out_stride=7)), (_embed, dict(offsets=POINTER, bags=-1)),
+    (_embed, dict(ids=None)), (_embed, dict(out=None)), (_embed, dict(stride=-8)), (_embed, dict(out=C.c_void_p(4100))), (_embed, dict(offsets=POINTER, bags=-1)),
     (_embed, dict(offsets=POINTER, bags=2, n=1000)), (_embed_gradient, dict(rows=0)), (_embed_gradient, dict(rows=1 << 31)), (_embed_gradient, dict(bytes=16)),
     (_embed_gradient, dict(workspace=None)), (_embed_gradient, dict(workspace=C.c_void_p(4097))), (_embed_gradient, dict(gradient=None)), (_embed_gradient, dict(out=None)),
     (_loss, dict(type=-1)), (_loss, dict(n=-1)), (_loss, dict(n=1 << 23)), (_loss, dict(v=0)), (_loss, dict(v=1 << 29)), (_loss, dict(columns=0)), (_loss, dict(scale=0.0)),
