@@ -3,7 +3,7 @@
 //   g = gradient * gradient_scale      m = b1 m + (1 - b1) g      v = b2 v + (1 - b2) g g      u = sqrt(v)
 //   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (u / sqrt(1 - b2^t) + eps)
 //
-// in 32 bits, every operation rounded by itself, p rounded once to its type.  The moments of all tensors lie in two flat
+// in 32 bits, p rounded once to its type.  The moments of all tensors lie in two flat
 // arrays in which every tensor starts at a multiple of kBlock elements.
 //
 // 8-bit states: of kBlock elements, m and u are held as e4m3 codes times one 32-bit scale (largest magnitude / 448).  u and not
@@ -53,12 +53,19 @@ __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466
 __device__ __forceinline__ float root_fast(float v)
 {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+__device__ __forceinline__ float reciprocal_fast(float v)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
 
 // Values of four codes.
-__device__ __forceinline__ void decode4(unsigned codes, float (&v)[4])
+__device__ __forceinline__ void decode4(unsigned codes, float *v)
 {
     unsigned low, high;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(low) : "h"((unsigned short)codes));
@@ -68,7 +75,7 @@ __device__ __forceinline__ void decode4(unsigned codes, float (&v)[4])
 }
 
 // Codes of four values that are codes' values already (NaN stays NaN).
-__device__ __forceinline__ unsigned encode4(const float (&v)[4])
+__device__ __forceinline__ unsigned encode4(const float *v)
 {
     unsigned short low, high;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(low) : "f"(v[1]), "f"(v[0]));
@@ -85,177 +92,201 @@ __device__ __forceinline__ float round_small(float r, unsigned random)
     return floorf(__fadd_rn(__fmul_rn(r, 512.f), below_one)) * kLeastCode;
 }
 
-template <class T>
-__device__ __forceinline__ void load4(const T *p, long long i, long long n, bool wide, float (&v)[4])
+// A lane's elements in a row: all of them, at a boundary of the load (or store), or element by element as far as the tensor goes (zeros behind it).
+template <class T, int N>
+__device__ __forceinline__ void load_some(const T *p, long long i, long long n, Pack<T, N> &v)
 {
-    if (wide && i + 4 <= n) {
-        const Pack<T, 4> q = *(const Pack<T, 4> *)(p + i);
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = to_float(q.v[k]);
+    for (int k = 0; k < N; k++) v.v[k] = i + k < n ? p[i + k] : from_float<T>(0.f);
+}
+
+template <class T, int N>
+__device__ __forceinline__ void load_all(const T *p, long long i, Pack<T, N> &v)
+{
+    constexpr int kWide = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+#pragma unroll
+    for (int k = 0; k < N; k += kWide) reinterpret_cast<Pack<T, kWide> &>(v.v[k]) = *(const Pack<T, kWide> *)(p + i + k);
+}
+
+template <class T, int N>
+__device__ __forceinline__ void store(T *p, long long i, long long n, bool whole, const float (&v)[N])
+{
+    constexpr int kWide = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+    Pack<T, N> q;
+#pragma unroll
+    for (int k = 0; k < N; k++) q.v[k] = from_float<T>(v[k]);
+    if (whole) {
+#pragma unroll
+        for (int k = 0; k < N; k += kWide) *(Pack<T, kWide> *)(p + i + k) = reinterpret_cast<const Pack<T, kWide> &>(q.v[k]);
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = i + k < n ? to_float(p[i + k]) : 0.f;
+        for (int k = 0; k < N; k++)
+            if (i + k < n) p[i + k] = q.v[k];
     }
 }
 
-template <class T>
-__device__ __forceinline__ void store4(T *p, long long i, long long n, bool wide, const float (&v)[4])
-{
-    if (wide && i + 4 <= n) {
-        Pack<T, 4> q;
-#pragma unroll
-        for (int k = 0; k < 4; k++) q.v[k] = from_float<T>(v[k]);
-        *(Pack<T, 4> *)(p + i) = q;
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (i + k < n) p[i + k] = from_float<T>(v[k]);
-    }
-}
+// What hangs on the number of the step, once per block.
+struct StepConstants {
+    float step_size, root_correction;
+    unsigned key;
+};
 
-template <class P, class G, bool kNarrow>
-__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamArgs a)
+__device__ __forceinline__ StepConstants step_constants(const AdamArgs &a)
 {
-    __shared__ float constants[2];
-    __shared__ unsigned key_shared;
-    const int lane = threadIdx.x & 31;
+    __shared__ StepConstants c;
     if (threadIdx.x == 0) {
         const long long step = *a.steps + 1;
         const double t = (double)step;
-        constants[0] = (float)(a.lr / (1.0 - pow(a.beta1, t)));
-        constants[1] = (float)(1.0 / sqrt(1.0 - pow(a.beta2, t)));
-        key_shared = mix(mix(a.seed) + (unsigned)step);
+        c.step_size = (float)(a.lr / (1.0 - pow(a.beta1, t)));
+        c.root_correction = (float)(1.0 / sqrt(1.0 - pow(a.beta2, t)));
+        c.key = mix(mix(a.seed) + (unsigned)step);
     }
     __syncthreads();
-    const float step_size = constants[0], root_correction = constants[1];
-    const unsigned key = key_shared;
+    return c;
+}
+
+// Whether a block of a tensor is there as a whole, at boundaries of 16 bytes.
+template <class P, class G>
+__device__ __forceinline__ bool is_whole(const AdamTensor &t, long long i)
+{
+    return (((uintptr_t)t.param | (uintptr_t)t.gradient | (uintptr_t)t.copy) & 15) == 0 && i / kBlock * kBlock + kBlock <= t.count;
+}
+
+// The parameter as it is held, and its copy.
+template <class P, int N>
+__device__ __forceinline__ void store_param(const AdamArgs &a, const AdamTensor &t, long long i, bool whole, float (&p)[N])
+{
+    store((P *)t.param, i, t.count, whole, p);
+    if (!t.copy) return;
+#pragma unroll
+    for (int k = 0; k < N; k++) p[k] = to_float(from_float<P>(p[k]));
+    if (a.copy_type == GTM_BF16) store((__nv_bfloat16 *)t.copy, i, t.count, whole, p);
+    else store((__half *)t.copy, i, t.count, whole, p);
+}
+
+template <class P, class G>
+__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamArgs a)
+{
+    const int lane = threadIdx.x & 31;
+    const StepConstants c = step_constants(a);
     int at = 0;
     for (long long b = (long long)blockIdx.x * 8 + threadIdx.x / 32; b < a.blocks; b += (long long)gridDim.x * 8) {
         const long long block = a.t[0].block + b;
         while (at + 1 < a.tensors && a.t[at + 1].block <= block) at++;
         const AdamTensor &t = a.t[at];
-        const long long i0 = (block - t.block) * kBlock;           // of the tensor
-        const long long n = t.count;
-        const bool wide_p = (uintptr_t)t.param % (4 * sizeof(P)) == 0, wide_g = (uintptr_t)t.gradient % (4 * sizeof(G)) == 0;
-        float p[2][4], g[2][4], m[2][4], u[2][4];
-        unsigned codes_m[2], codes_u[2];
-        float scale_m = 0.f, scale_u = 0.f;
-        if (kNarrow) scale_m = a.first_scales[block], scale_u = a.second_scales[block];
+        // four elements, and four 128 further: 16 bytes of 32-bit arrays, one next to the other over the warp
+        const long long flat = block * kBlock + lane * 4, i = flat - t.block * kBlock;
+        const bool whole = is_whole<P, G>(t, i);
+        Pack<P, 4> p4[2];
+        Pack<G, 4> g4[2];
+        Pack<float, 4> m[2], v[2];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const long long i = i0 + j * 128 + lane * 4, flat = block * kBlock + j * 128 + lane * 4;
-            load4((const P *)t.param, i, n, wide_p, p[j]);
-            load4((const G *)t.gradient, i, n, wide_g, g[j]);
-            if (kNarrow) {
-                codes_m[j] = *(const unsigned *)((const unsigned char *)a.first + flat);
-                codes_u[j] = *(const unsigned *)((const unsigned char *)a.second + flat);
-            } else {
-                load4((const float *)a.first, flat, flat + 4, true, m[j]);
-                load4((const float *)a.second, flat, flat + 4, true, u[j]);
-            }
+        for (int j = 0; j < 2; j++) m[j] = *(const Pack<float, 4> *)((const float *)a.first + flat + j * 128), v[j] = *(const Pack<float, 4> *)((const float *)a.second + flat + j * 128);
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) p4[j] = *(const Pack<P, 4> *)((const P *)t.param + i + j * 128), g4[j] = *(const Pack<G, 4> *)((const G *)t.gradient + i + j * 128);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 2; j++) load_some((const P *)t.param, i + j * 128, t.count, p4[j]), load_some((const G *)t.gradient, i + j * 128, t.count, g4[j]);
         }
-        float largest_m = 0.f, largest_u = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            if (kNarrow) decode4(codes_m[j], m[j]), decode4(codes_u[j], u[j]);
+            float p[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const float gr = __fmul_rn(g[j][k], a.gradient_scale);
-                if (kNarrow) {
-                    m[j][k] = __fmul_rn(m[j][k], scale_m);
-                    u[j][k] = __fmul_rn(u[j][k], scale_u);
-                    u[j][k] = __fmul_rn(u[j][k], u[j][k]);
-                }
-                m[j][k] = __fadd_rn(__fmul_rn(m[j][k], a.b1), __fmul_rn(gr, a.other1));
-                u[j][k] = __fadd_rn(__fmul_rn(u[j][k], a.b2), __fmul_rn(__fmul_rn(gr, gr), a.other2));
-                // next to 8-bit states the hardware's root (2^-23) and quotient (2^-22) are exact enough, and a third of the instructions
-                const float root = kNarrow ? root_fast(u[j][k]) : __fsqrt_rn(u[j][k]);
-                const float below = __fadd_rn(__fmul_rn(root, root_correction), a.eps);
-                const float moved = kNarrow ? __fdividef(m[j][k], below) : __fdiv_rn(m[j][k], below);
-                p[j][k] = __fsub_rn(__fmul_rn(p[j][k], a.decay), __fmul_rn(step_size, moved));
-                if (kNarrow) {
-                    u[j][k] = root;
-                    largest_m = fmaxf(largest_m, fabsf(m[j][k]));           // NaN is passed over
-                    largest_u = fmaxf(largest_u, root);
-                }
+                const float g = __fmul_rn(to_float(g4[j].v[k]), a.gradient_scale);
+                m[j].v[k] = __fadd_rn(__fmul_rn(m[j].v[k], a.b1), __fmul_rn(g, a.other1));
+                v[j].v[k] = __fadd_rn(__fmul_rn(v[j].v[k], a.b2), __fmul_rn(__fmul_rn(g, g), a.other2));
+                const float moved = __fdiv_rn(m[j].v[k], __fadd_rn(__fmul_rn(__fsqrt_rn(v[j].v[k]), c.root_correction), a.eps));
+                p[k] = __fsub_rn(__fmul_rn(to_float(p4[j].v[k]), a.decay), __fmul_rn(c.step_size, moved));
+            }
+            *(Pack<float, 4> *)((float *)a.first + flat + j * 128) = m[j];
+            *(Pack<float, 4> *)((float *)a.second + flat + j * 128) = v[j];
+            store_param<P>(a, t, i + j * 128, whole, p);
+        }
+    }
+}
+
+// States of 8 bits.  What bounds it is instructions, so products and sums are fused, and the hardware's root and reciprocal (2^-22, exact next to
+// 8 bits) are used.
+template <class P, class G>
+__global__ void __launch_bounds__(256, 4) adamw_narrow_kernel(const __grid_constant__ AdamArgs a)
+{
+    const int lane = threadIdx.x & 31;
+    const StepConstants c = step_constants(a);
+    const float gradient_m = a.gradient_scale * a.other1, gradient_u = a.gradient_scale * sqrtf(a.other2), root_b2 = sqrtf(a.b2);
+    int at = 0;
+    for (long long b = (long long)blockIdx.x * 8 + threadIdx.x / 32; b < a.blocks; b += (long long)gridDim.x * 8) {
+        const long long block = a.t[0].block + b;
+        while (at + 1 < a.tensors && a.t[at + 1].block <= block) at++;
+        const AdamTensor &t = a.t[at];
+        const long long flat = block * kBlock + lane * 8, i = flat - t.block * kBlock;
+        const bool whole = is_whole<P, G>(t, i);
+        const uint2 codes_m = *(const uint2 *)((const unsigned char *)a.first + flat), codes_u = *(const uint2 *)((const unsigned char *)a.second + flat);
+        const float held_m = a.first_scales[block] * a.b1, held_u = a.second_scales[block] * root_b2;
+        Pack<P, 8> p8;
+        Pack<G, 8> g8;
+        if (whole) load_all((const P *)t.param, i, p8), load_all((const G *)t.gradient, i, g8);      // the warp is of one mind: no load waits for another
+        else load_some((const P *)t.param, i, t.count, p8), load_some((const G *)t.gradient, i, t.count, g8);
+        float p[8], m[8], u[8];
+        decode4(codes_m.x, m), decode4(codes_m.y, m + 4), decode4(codes_u.x, u), decode4(codes_u.y, u + 4);
+        float largest_m = 0.f, largest_u = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float g = to_float(g8.v[k]), by_u = g * gradient_u;
+            m[k] = fmaf(g, gradient_m, m[k] * held_m);
+            u[k] *= held_u;
+            u[k] = root_fast(fmaf(by_u, by_u, u[k] * u[k]));
+            const float moved = m[k] * reciprocal_fast(fmaf(u[k], c.root_correction, a.eps));
+            p[k] = fmaf(-c.step_size, moved, to_float(p8.v[k]) * a.decay);
+            largest_m = fmaxf(largest_m, fabsf(m[k]));               // NaN is passed over
+            largest_u = fmaxf(largest_u, u[k]);
+        }
+        store_param<P>(a, t, i, whole, p);
+        // magnitudes: their bits have their order
+        largest_m = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(largest_m)));
+        largest_u = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(largest_u)));
+        if (!finite(largest_m) || !finite(largest_u)) {
+            // infinities are held as NaN and have no part in the scale
+            largest_m = largest_u = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                if (finite(m[k])) largest_m = fmaxf(largest_m, fabsf(m[k]));
+                else m[k] = __int_as_float(0x7fffffff);
+                if (finite(u[k])) largest_u = fmaxf(largest_u, u[k]);
+                else u[k] = __int_as_float(0x7fffffff);
+            }
+            largest_m = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(largest_m)));
+            largest_u = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(largest_u)));
+        }
+        const float scale_m = fmaxf(largest_m * (float)(1.0 / 448.0), kLeastScale), scale_u = fmaxf(largest_u * (float)(1.0 / 448.0), kLeastScale);
+        const float inverse_m = __fdiv_rn(1.f, scale_m), inverse_u = __fdiv_rn(1.f, scale_u);
+        if (lane == 0) a.first_scales[block] = scale_m, a.second_scales[block] = scale_u;
+        unsigned random[8];
+        float qm[8], qu[8];
+        bool normal = true;
+        const unsigned from = (unsigned)flat * 0x9e3779b1u + c.key;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            random[k] = mix(from + k * 0x9e3779b1u);
+            qm[k] = fabsf(m[k]) * inverse_m, qu[k] = u[k] * inverse_u;
+            normal &= qm[k] >= 0.015625f && qu[k] >= 0.015625f;          // not for NaN
+        }
+        if (__all_sync(~0u, normal)) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) qm[k] = round_normal(qm[k], random[k] >> 16), qu[k] = round_normal(qu[k], random[k] & 0xffff);
+        } else {                                                  // zeros, NaN, and one in thousands of usual values
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                qm[k] = qm[k] >= 0.015625f ? round_normal(qm[k], random[k] >> 16) : round_small(qm[k], random[k] >> 16);
+                qu[k] = qu[k] >= 0.015625f ? round_normal(qu[k], random[k] & 0xffff) : round_small(qu[k], random[k] & 0xffff);
+                if (u[k] > 0.f) qu[k] = fmaxf(qu[k], kLeastCode);
             }
         }
-        if (kNarrow) {
 #pragma unroll
-            for (int o = 16; o; o /= 2) {
-                largest_m = fmaxf(largest_m, __shfl_xor_sync(~0u, largest_m, o));
-                largest_u = fmaxf(largest_u, __shfl_xor_sync(~0u, largest_u, o));
-            }
-            if (!finite(largest_m) || !finite(largest_u)) {
-                // infinities are held as NaN and have no part in the scale
-                largest_m = largest_u = 0.f;
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        if (finite(m[j][k])) largest_m = fmaxf(largest_m, fabsf(m[j][k]));
-                        else m[j][k] = __int_as_float(0x7fffffff);
-                        if (finite(u[j][k])) largest_u = fmaxf(largest_u, u[j][k]);
-                        else u[j][k] = __int_as_float(0x7fffffff);
-                    }
-#pragma unroll
-                for (int o = 16; o; o /= 2) {
-                    largest_m = fmaxf(largest_m, __shfl_xor_sync(~0u, largest_m, o));
-                    largest_u = fmaxf(largest_u, __shfl_xor_sync(~0u, largest_u, o));
-                }
-            }
-            scale_m = fmaxf(__fmul_rn(largest_m, (float)(1.0 / 448.0)), kLeastScale);
-            scale_u = fmaxf(__fmul_rn(largest_u, (float)(1.0 / 448.0)), kLeastScale);
-            const float inverse_m = __fdiv_rn(1.f, scale_m), inverse_u = __fdiv_rn(1.f, scale_u);
-            if (lane == 0) a.first_scales[block] = scale_m, a.second_scales[block] = scale_u;
-            const unsigned flat = (unsigned)(block * kBlock) + lane * 4;
-            bool small = false;
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                unsigned random[4];
-                float qm[4], qu[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    random[k] = mix((flat + j * 128 + k) * 0x9e3779b1u + key);
-                    qm[k] = __fmul_rn(fabsf(m[j][k]), inverse_m), qu[k] = __fmul_rn(u[j][k], inverse_u);
-                    small |= !(qm[k] >= 0.015625f) | !(qu[k] >= 0.015625f);
-                }
-                if (!__any_sync(~0u, small)) {
-#pragma unroll
-                    for (int k = 0; k < 4; k++) qm[k] = round_normal(qm[k], random[k] >> 16), qu[k] = round_normal(qu[k], random[k] & 0xffff);
-                } else {                                             // zeros, NaN, and one in thousands of usual values
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        qm[k] = qm[k] >= 0.015625f ? round_normal(qm[k], random[k] >> 16) : round_small(qm[k], random[k] >> 16);
-                        qu[k] = qu[k] >= 0.015625f ? round_normal(qu[k], random[k] & 0xffff) : round_small(qu[k], random[k] & 0xffff);
-                        if (u[j][k] > 0.f) qu[k] = fmaxf(qu[k], kLeastCode);
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 4; k++) qm[k] = copysignf(qm[k], m[j][k]);
-                codes_m[j] = encode4(qm), codes_u[j] = encode4(qu);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const long long i = i0 + j * 128 + lane * 4, flat = block * kBlock + j * 128 + lane * 4;
-            store4((P *)t.param, i, n, wide_p, p[j]);
-            if (t.copy) {
-                // the copy of the parameter as it is held
-#pragma unroll
-                for (int k = 0; k < 4; k++) p[j][k] = to_float(from_float<P>(p[j][k]));
-                const bool wide_c = (uintptr_t)t.copy % 8 == 0;
-                if (a.copy_type == GTM_BF16) store4((__nv_bfloat16 *)t.copy, i, n, wide_c, p[j]);
-                else store4((__half *)t.copy, i, n, wide_c, p[j]);
-            }
-            if (kNarrow) {
-                *(unsigned *)((unsigned char *)a.first + flat) = codes_m[j];
-                *(unsigned *)((unsigned char *)a.second + flat) = codes_u[j];
-            } else {
-                store4((float *)a.first, flat, flat + 4, true, m[j]);
-                store4((float *)a.second, flat, flat + 4, true, u[j]);
-            }
-        }
+        for (int k = 0; k < 8; k++) qm[k] = copysignf(qm[k], m[k]);
+        *(uint2 *)((unsigned char *)a.first + flat) = make_uint2(encode4(qm), encode4(qm + 4));
+        *(uint2 *)((unsigned char *)a.second + flat) = make_uint2(encode4(qu), encode4(qu + 4));
     }
 }
 
@@ -269,8 +300,8 @@ int launch(const AdamArgs &a, bool narrow, cudaStream_t stream)
     GTM_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
     const long long want = (a.blocks + 7) / 8, most = (long long)sms * 8;
     const unsigned grid = (unsigned)(want < most ? want : most);
-    if (narrow) adamw_kernel<P, G, true><<<grid, 256, 0, stream>>>(a);
-    else adamw_kernel<P, G, false><<<grid, 256, 0, stream>>>(a);
+    if (narrow) adamw_narrow_kernel<P, G><<<grid, 256, 0, stream>>>(a);
+    else adamw_kernel<P, G><<<grid, 256, 0, stream>>>(a);
     GTM_CU(cudaGetLastError());
     return GTM_OK;
 }

@@ -6,7 +6,7 @@
 // Both are one operation: rows gathered by an index list that is cut into segments, each segment added up in 32 bits and
 // rounded once.  Forward the list is `ids` and the segments are the bags; for the gradient the list is the bag of every
 // position, sorted by id (stable radix sort), and the segments are the table's rows.  Sums have one order, that of the list, in
-// pieces of kPiece: there are no atomics and results do not change from run to run.
+// pieces of a span: there are no atomics on values and results do not change from run to run.
 #include "gtm_readout.cuh"
 
 #include <type_traits>
@@ -15,20 +15,22 @@
 namespace gtm_readout {
 namespace {
 
-// A warp adds up to kPiece rows.  Longer segments leave their first kPiece rows in `head` and the rest in `part`, one slot
-// per kPiece positions of the list: at most one such segment begins in a span of kPiece positions, and at most one goes on
-// through it, so that a slot has one owner.  `ends[span]` is the long segment that ends in a span, -1: none does.
-constexpr int kPiece = 128;
-
+// The list is cut into spans of 32, 64 or 128 positions, and a team of 4 to 32 lanes (as many as have a row's columns, 16 bytes each) adds up
+// the rows of one span, whatever the segments are: teams have equal work with one id in a segment or a million.  A segment that
+// goes on from one span to the next leaves its sums in 32 bits: the first in `head`, the others in `part`, one slot per
+// span each, since only one segment can enter a span and one leave it.  `ends[span]` is the segment that entered it and ends there (-1:
+// none); a second kernel adds its slots in order.  Segments without positions are zeroed by other teams.
 struct GatherArgs {
     const void *src;
     long long src_stride, rows;      // elements, rows of src
+    const uint2 *pairs;              // (segment, row of src) of every position, or null: from list and offsets
     const void *list;                // row of src per position
     int list_wide;
     const void *offsets;             // segments [offsets[s], offsets[s + 1]) of the list
     int offsets_wide;
     long long positions, segments;
-    int columns;
+    int columns, span;
+    long long spans;
     float scale;
     void *out;
     long long out_stride;
@@ -43,21 +45,35 @@ __device__ __forceinline__ long long clamp_offset(const void *offsets, int wide,
     return o < 0 ? 0 : o > positions ? positions : o;
 }
 
-__device__ __forceinline__ long long clamp_offset(const GatherArgs &a, long long s) { return clamp_offset(a.offsets, a.offsets_wide, a.positions, s); }
-
-// Last segment that begins at or before `position`; -1: none does.  A warp asks together, 32 segments at a time.
-__device__ long long segment_at(const void *offsets, int wide, long long positions, long long segments, long long position)
+// Last segment that begins at or before `position`; -1: none does.  kLanes lanes ask together.
+template <int kLanes>
+__device__ long long segment_at(const void *offsets, int wide, long long positions, long long segments, long long position, unsigned team)
 {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x % kLanes;
     long long low = -1, high = segments;          // offsets[low] <= position < offsets[high]
     while (high - low > 1) {
-        const long long step = (high - low - 1 + 31) / 32, at = low + 1 + lane * step;
-        const unsigned before = __ballot_sync(~0u, at < high && clamp_offset(offsets, wide, positions, at) <= position);
-        const int n = __popc(before);             // offsets do not decrease: the first n lanes
-        if (n < 32) high = min(high, low + 1 + n * step);
+        const long long step = (high - low - 1 + kLanes - 1) / kLanes, at = low + 1 + lane * step;
+        const unsigned before = __ballot_sync(team, at < high && clamp_offset(offsets, wide, positions, at) <= position);
+        const int n = __popc(before & team);      // offsets do not decrease: the first n lanes
+        if (n < kLanes) high = min(high, low + 1 + n * step);
         if (n > 0) low = low + 1 + (n - 1) * step;
     }
     return low;
+}
+
+// Segment of a position at or behind the beginning of segment `from` (-1: of none), -1 where it is in none.  Mostly the same or one
+// of the next; behind many empty ones, found by halves.
+__device__ __forceinline__ long long segment_from(const void *offsets, int wide, long long positions, long long segments, long long &from, long long position)
+{
+    for (int tries = 0; tries < 8 && from + 1 < segments && clamp_offset(offsets, wide, positions, from + 1) <= position; tries++) from++;
+    long long high = segments;
+    if (from + 1 < segments && clamp_offset(offsets, wide, positions, from + 1) <= position)
+        while (high - from > 1) {
+            const long long mid = (from + high) / 2;
+            if (clamp_offset(offsets, wide, positions, mid) <= position) from = mid;
+            else high = mid;
+        }
+    return from >= 0 && position < clamp_offset(offsets, wide, positions, from + 1) ? from : -1;
 }
 
 __device__ __forceinline__ void add2(float2 &a, float x, float y)
@@ -77,149 +93,162 @@ __device__ __forceinline__ void accumulate(float2 (&acc)[(V + 1) / 2], const Pac
         for (int v = 0; v < V; v += 2) add2(acc[v / 2], to_float(p.v[v]), to_float(p.v[v + 1]));
 }
 
-// kLanes lanes have a row's columns, U runs of V next to each other, kLanes * V apart; the 32 / kLanes groups of a warp take rows in turn.
-template <class T, int V, int U, int kLanes>
-struct Gather {
-    static constexpr int kGroups = 32 / kLanes, kAhead = U == 1 ? 8 : 4, kColumns = kLanes * V * U;
-    float2 acc[U][(V + 1) / 2];
-    bool bad = false;                // an id beyond the table
+// Four rows ahead at 28 warps an SM: 72 us for 819,200 rows of 256 bf16 in bags (5.8 TB/s, from L2); eight rows at 20 warps: 80.
+constexpr int kGatherThreads = 128, kGatherBlocks = 7;
 
-    __device__ __forceinline__ void add(const GatherArgs &a, long long begin, long long end, int column0, int *compact)
-    {
-        const int lane = threadIdx.x & 31, group = lane / kLanes;
-        const T *column[U];
+// A lane has U runs of V columns next to each other, kLanes * V apart.
+template <class T, int V, int U, int kLanes>
+__global__ void __launch_bounds__(kGatherThreads, kGatherBlocks) gather_sum_kernel(const GatherArgs a)
+{
+    constexpr int kColumns = kLanes * V * U, kAhead = 4;
+    const int lane = threadIdx.x % kLanes, column0 = blockIdx.y * kColumns;
+    const unsigned team = kLanes == 32 ? ~0u : ((1u << kLanes % 32) - 1) << ((threadIdx.x & 31) / kLanes * kLanes);
+    const long long unit = (long long)blockIdx.x * (kGatherThreads / kLanes) + threadIdx.x / kLanes;
+    float2 acc[U][(V + 1) / 2];
+    bool bad = false;                             // an id beyond the table
+    const auto clear = [&] {
+        bad = false;
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            // lanes behind the last column read the first one, and drop it
-            const int c = column0 + (u * kLanes + lane % kLanes) * V;
-            column[u] = (const T *)a.src + (c < a.columns ? c : 0);
+        for (int u = 0; u < U; u++)
 #pragma unroll
             for (int v = 0; v < (V + 1) / 2; v++) acc[u][v] = make_float2(0.f, 0.f);
+    };
+    const auto write = [&](long long segment) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = column0 + (u * kLanes + lane) * V;
+            if (c >= a.columns) continue;
+            Pack<T, V> p;
+#pragma unroll
+            for (int v = 0; v < V; v++) p.v[v] = from_float<T>(bad ? __int_as_float(0x7fffffff) : (v % 2 ? acc[u][v / 2].y : acc[u][v / 2].x) * a.scale);
+            *(Pack<T, V> *)((T *)a.out + segment * a.out_stride + c) = p;
         }
-        for (long long base = begin; base < end; base += 32) {
-            int n = (int)min(32ll, end - base), mine = -1;
-            if (lane < n) {
-                const long long id = index_at(a.list, a.list_wide, base + lane);
-                mine = id >= a.rows ? -2 : id < 0 ? -1 : (int)id;
+    };
+    clear();
+    if (unit >= a.spans) {
+        // zeros of kLanes segments
+        const long long first = (unit - a.spans) * kLanes, mine = first + lane;
+        const bool none = mine < a.segments && clamp_offset(a.offsets, a.offsets_wide, a.positions, mine) >= clamp_offset(a.offsets, a.offsets_wide, a.positions, mine + 1);
+        for (unsigned which = (__ballot_sync(team, none) & team) >> ((threadIdx.x & 31) / kLanes * kLanes); which; which &= which - 1) write(first + __ffs(which) - 1);
+        return;
+    }
+    const T *column[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int c = column0 + (u * kLanes + lane) * V;
+        column[u] = (const T *)a.src + (c < a.columns ? c : 0);      // lanes behind the last column read the first one, and drop it
+    }
+    const long long first = unit * a.span, last = min(first + a.span, a.positions);
+    long long base = -1;                          // a segment at or before the lane's next position
+    if (!a.pairs) base = segment_at<kLanes>(a.offsets, a.offsets_wide, a.positions, a.segments, first ? first - 1 : 0, team);
+    const auto segment_of = [&](long long position) -> int {
+        if (a.pairs) return a.pairs[position].x < (unsigned long long)a.segments ? (int)a.pairs[position].x : -1;
+        return (int)segment_from(a.offsets, a.offsets_wide, a.positions, a.segments, base, position);
+    };
+    int now = first ? segment_of(first - 1) : -1, entered = now, ended = -1;      // a segment that is -1 is none
+    const auto leave = [&](bool goes_on) {
+        if (now >= 0) {
+            if (now != entered && !goes_on) write(now);
+            else {
+                float *to = (now == entered ? a.part : a.head) + unit * a.partial_stride;
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int v = 0; v < V; v++) {
+                        const int c = column0 + (u * kLanes + lane) * V + v;
+                        if (c < a.columns) to[c] = bad ? __int_as_float(0x7fffffff) : v % 2 ? acc[u][v / 2].y : acc[u][v / 2].x;
+                    }
+                if (now == entered && !goes_on) ended = now;
             }
-            const unsigned real = __ballot_sync(~0u, mine >= 0);
-            if (__popc(real) < n) {              // padding: the others move up
-                bad |= __any_sync(~0u, mine == -2);
-                n = __popc(real);
-                if (mine >= 0) compact[__popc(real & ((1u << lane) - 1))] = mine;
-                __syncwarp();
-                if (lane < n) mine = compact[lane];
-                __syncwarp();
-            }
-            int i = 0;
-            for (; i + kAhead * kGroups <= n; i += kAhead * kGroups) {
+        }
+        clear();
+    };
+    bool begun = false;                           // whether the span has a position of `now`
+    int next_row = -1, next_segment = -1;         // of the lane's next position, read before the rows of the positions at hand
+    const auto look = [&](long long position) {
+        next_row = next_segment = -1;
+        if (position >= last) return;
+        if (a.pairs) {
+            const uint2 pair = a.pairs[position];
+            next_segment = pair.x < (unsigned long long)a.segments ? (int)pair.x : -1, next_row = (int)pair.y;
+        } else {
+            const long long id = index_at(a.list, a.list_wide, position);
+            next_segment = segment_of(position);
+            next_row = id >= a.rows ? -2 : id < 0 ? -1 : (int)id;
+        }
+        if (next_segment < 0) next_row = -1;
+    };
+    look(first + lane);
+    for (long long at = first; at < last; at += kLanes) {
+        const int row = next_row, segment = next_segment;
+        look(at + kLanes + lane);
+        const int n = (int)min((long long)kLanes, last - at);
+        const auto enter = [&](int next) {
+            if (next == now) return;
+            if (begun) leave(false);
+            else entered = -1;                                    // it ended with the span before
+            now = next;
+        };
+        enter(__shfl_sync(team, segment, 0, kLanes));
+        begun = true;
+        if (n == kLanes && __all_sync(team, segment == now && row >= 0)) {
+            // all of one segment
+#pragma unroll 1
+            for (int i = 0; i < kLanes; i += kAhead) {
                 Pack<T, V> got[kAhead][U];
 #pragma unroll
                 for (int k = 0; k < kAhead; k++) {
-                    const long long at = (long long)__shfl_sync(~0u, mine, i + k * kGroups + group) * a.src_stride;
+                    const unsigned long long from = (unsigned long long)(unsigned)__shfl_sync(team, row, i + k, kLanes) * (unsigned)a.src_stride;
 #pragma unroll
-                    for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + at);
+                    for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + from);
                 }
 #pragma unroll
                 for (int k = 0; k < kAhead; k++)
 #pragma unroll
                     for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
             }
-            for (; i < n; i += 4 * kGroups) {
-                Pack<T, V> got[4][U];
+            continue;
+        }
+#pragma unroll 1
+        for (int i = 0; i < n; i += kAhead) {
+            Pack<T, V> got[kAhead][U];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int r = i + k * kGroups + group;
-                    const long long at = (long long)__shfl_sync(~0u, mine, r & 31) * a.src_stride;
-                    if (r < n)
+            for (int k = 0; k < kAhead; k++) {
+                // a position without a row reads the first one, and drops it
+                const unsigned long long from = (unsigned long long)(unsigned)max(__shfl_sync(team, row, i + k, kLanes), 0) * (unsigned)a.src_stride;
+                if (a.rows > 0)
 #pragma unroll
-                        for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + at);
-                }
+                    for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + from);
+            }
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (i + k * kGroups + group < n)
+            for (int k = 0; k < kAhead; k++) {
+                const int next = __shfl_sync(team, segment, i + k, kLanes), which = __shfl_sync(team, row, i + k, kLanes);
+                if (i + k >= n) continue;
+                enter(next);
+                if (which >= 0)
 #pragma unroll
-                        for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
+                    for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
+                else bad |= which == -2;
             }
         }
-        if constexpr (kGroups > 1)
-#pragma unroll
-            for (int o = kLanes; o < 32; o *= 2)
-#pragma unroll
-                for (int u = 0; u < U; u++)
-#pragma unroll
-                    for (int v = 0; v < (V + 1) / 2; v++) {
-                        acc[u][v].x += __shfl_xor_sync(~0u, acc[u][v].x, o);
-                        if (V > 1) acc[u][v].y += __shfl_xor_sync(~0u, acc[u][v].y, o);
-                    }
     }
-
-    __device__ __forceinline__ float value(int u, int v) const
-    {
-        return bad ? __int_as_float(0x7fffffff) : v % 2 ? acc[u][v / 2].y : acc[u][v / 2].x;
-    }
-};
-
-template <class T, int V, int U, int kLanes>
-__global__ void __launch_bounds__(256, 3) gather_sum_kernel(const GatherArgs a)
-{
-    __shared__ int compact[8][32];
-    using G = Gather<T, V, U, kLanes>;
-    const long long unit = (long long)blockIdx.x * 8 + threadIdx.x / 32;
-    const int lane = threadIdx.x & 31, column0 = blockIdx.y * G::kColumns;
-    long long begin, end;
-    float *to = nullptr;
-    if (unit < a.segments) {
-        begin = clamp_offset(a, unit), end = clamp_offset(a, unit + 1);
-        if (end - begin > kPiece) {
-            to = a.head + begin / kPiece * a.partial_stride;
-            end = begin + kPiece;
-        }
-    } else {
-        const long long span = unit - a.segments;
-        if (a.positions <= kPiece || span * kPiece >= a.positions) return;
-        const long long s = segment_at(a.offsets, a.offsets_wide, a.positions, a.segments, span * kPiece);
-        begin = end = 0;
-        long long last = 0;
-        if (s >= 0) {
-            last = clamp_offset(a, s + 1);
-            begin = max(span * kPiece, clamp_offset(a, s) + kPiece);
-            end = min((span + 1) * kPiece, last);
-        }
-        if (blockIdx.y == 0 && lane == 0) a.ends[span] = begin < end && end == last ? (int)s : -1;
-        if (begin >= end) return;
-        to = a.part + span * a.partial_stride;
-    }
-    G g;
-    g.add(a, begin, end, column0, compact[threadIdx.x / 32]);
-    if (lane >= kLanes) return;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        const int c = column0 + (u * kLanes + lane) * V;
-        if (c >= a.columns) continue;
-        if (to) {
-#pragma unroll
-            for (int v = 0; v < V; v++) to[c + v] = g.value(u, v);
-        } else {
-            Pack<T, V> p;
-#pragma unroll
-            for (int v = 0; v < V; v++) p.v[v] = from_float<T>(g.value(u, v) * a.scale);
-            *(Pack<T, V> *)((T *)a.out + unit * a.out_stride + c) = p;
-        }
-    }
+    // every lane's `base` is at or before its last position: any of them finds the next one's segment
+    leave(last < a.positions && now >= 0 && segment_of(last) == now);
+    if (blockIdx.y == 0 && lane == 0) a.ends[unit] = ended;
 }
 
-// Segments longer than kPiece: head and parts, added in the order of the list.  A warp has the segment that ends in its span (if one
-// does) and 128 columns; where a segment has more than kAlone parts, the block's eight warps take every eighth.
+// Segments of several spans: head and parts, added in the order of the list.  A warp has the segment that ends in its span (if one
+// does) and 128 columns; where a segment has more than kAlone parts, the block's warps take them in turn.
 template <class T>
 __global__ void __launch_bounds__(256) gather_join_kernel(const GatherArgs a)
 {
-    constexpr int kAlone = 64;
-    __shared__ float4 sums[8][32];
-    __shared__ long long longest[8];
+    constexpr int kAlone = 16, kWarps = 8;
+    __shared__ float4 sums[kWarps][32];
+    __shared__ long long longest[kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, c = blockIdx.y * 128 + lane * 4;
-    const long long span = (long long)blockIdx.x * 8 + warp;
+    const long long span = (long long)blockIdx.x * kWarps + warp;
     const bool inside = c < a.partial_stride;
+    const auto begin_of = [&](long long s) { return clamp_offset(a.offsets, a.offsets_wide, a.positions, s) / a.span; };
     const auto sum_of = [&](long long first, long long n, int step) {
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         if (inside)
@@ -230,63 +259,100 @@ __global__ void __launch_bounds__(256) gather_join_kernel(const GatherArgs a)
             }
         return sum;
     };
-    const auto write = [&](long long s, float4 sum) {
-        const float4 head = inside ? *(const float4 *)(a.head + clamp_offset(a, s) / kPiece * a.partial_stride + c) : sum;
+    const auto head_of = [&](long long unit) { return inside ? *(const float4 *)(a.head + unit * a.partial_stride + c) : make_float4(0.f, 0.f, 0.f, 0.f); };
+    const auto write = [&](long long s, float4 head, float4 sum) {
         const float v[4] = {head.x + sum.x, head.y + sum.y, head.z + sum.z, head.w + sum.w};
 #pragma unroll
         for (int k = 0; k < 4; k++)
             if (c + k < a.columns) ((T *)a.out)[s * a.out_stride + c + k] = from_float<T>(v[k] * a.scale);
     };
-    const long long s = span * kPiece < a.positions ? a.ends[span] : -1;
+    const long long s = span < a.spans ? a.ends[span] : -1;
     long long first = 0, n = 0;
     if (s >= 0) {
-        first = clamp_offset(a, s) / kPiece + 1;
+        first = begin_of(s) + 1;
         n = span - first + 1;
     }
-    if (n > 0 && n <= kAlone) write(s, sum_of(first, n, 1));
+    if (n > 0 && n <= kAlone) {
+        const float4 head = head_of(first - 1);
+        write(s, head, sum_of(first, n, 1));
+    }
     if (lane == 0) longest[warp] = n > kAlone ? s : -1;
     __syncthreads();
-    for (int w = 0; w < 8; w++) {
+    for (int w = 0; w < kWarps; w++) {
         const long long one = longest[w];
         if (one < 0) continue;                  // the block together
-        const long long begin = clamp_offset(a, one) / kPiece + 1, parts = (long long)blockIdx.x * 8 + w - begin + 1;
-        sums[warp][lane] = sum_of(begin + warp, parts - warp, 8);
+        const long long begin = begin_of(one) + 1, parts = (long long)blockIdx.x * kWarps + w - begin + 1;
+        sums[warp][lane] = sum_of(begin + warp, parts - warp, kWarps);
         __syncthreads();
         if (warp == 0) {
             float4 sum = sums[0][lane];
-            for (int k = 1; k < 8; k++) sum.x += sums[k][lane].x, sum.y += sums[k][lane].y, sum.z += sums[k][lane].z, sum.w += sums[k][lane].w;
-            write(one, sum);
+            for (int k = 1; k < kWarps; k++) sum.x += sums[k][lane].x, sum.y += sums[k][lane].y, sum.z += sums[k][lane].z, sum.w += sums[k][lane].w;
+            write(one, head_of(begin - 1), sum);
         }
         __syncthreads();
     }
 }
 
+// Lanes that have a row's columns, 16 bytes each: as few as there are, so that a warp has several narrow rows.
+int team_lanes(int64_t columns, size_t element)
+{
+    const int64_t wide = 16 / element;
+    return columns <= 4 * wide ? 4 : columns <= 8 * wide ? 8 : columns <= 16 * wide ? 16 : 32;
+}
+
+// Long spans (fewer slots of sums) as long as there are 16 warps per SM of them.
+int span_of(int64_t positions, int64_t columns, size_t element)
+{
+    if (positions <= 128) return 128;                 // one span: nothing to join
+    const int lanes = team_lanes(columns, element);
+    const int64_t blocks = (columns * element + lanes * 16 - 1) / (lanes * 16), teams = (int64_t)148 * 16 * 32 / lanes;
+    for (int span = 128; span > 32; span /= 2)
+        if (positions / span * blocks >= teams) return span;
+    return 32;
+}
+
+int64_t partial_stride(int64_t columns) { return (int64_t)round_up(columns, 4); }
+
+// Slots of sums, and where the segments end.
+struct GatherSpace {
+    uint64_t head, part, ends, total;
+};
+
+GatherSpace gather_space(uint64_t at, int64_t positions, int64_t columns)
+{
+    // of the shortest spans: a caller's workspace serves every element type
+    const uint64_t spans = (uint64_t)(positions + 31) / 32, sums = round_up(spans * partial_stride(columns) * 4, 256);
+    return {at, at + sums, at + 2 * sums, at + 2 * sums + round_up(spans * 4, 256)};
+}
+
 template <class T, int V, int U, int kLanes>
 int launch_gather(const GatherArgs &a, cudaStream_t stream)
 {
-    const long long spans = a.positions > kPiece ? (a.positions + kPiece - 1) / kPiece : 0, units = a.segments + spans;
-    const int wide = Gather<T, V, U, kLanes>::kColumns;
-    const dim3 grid((unsigned)((units + 7) / 8), (unsigned)((a.columns + wide - 1) / wide));
-    gather_sum_kernel<T, V, U, kLanes><<<grid, 256, 0, stream>>>(a);
+    constexpr int kWide = kLanes * V * U, kTeams = kGatherThreads / kLanes;
+    const long long units = a.spans + (a.segments + kLanes - 1) / kLanes;
+    const dim3 grid((unsigned)((units + kTeams - 1) / kTeams), (unsigned)((a.columns + kWide - 1) / kWide));
+    gather_sum_kernel<T, V, U, kLanes><<<grid, kGatherThreads, 0, stream>>>(a);
     GTM_CU(cudaGetLastError());
-    if (spans) {
-        gather_join_kernel<T><<<dim3((unsigned)((spans + 7) / 8), (unsigned)((a.columns + 127) / 128)), 256, 0, stream>>>(a);
+    if (a.spans > 1) {
+        gather_join_kernel<T><<<dim3((unsigned)((a.spans + 7) / 8), (unsigned)((a.columns + 127) / 128)), 256, 0, stream>>>(a);
         GTM_CU(cudaGetLastError());
     }
     return GTM_OK;
 }
 
-// As few lanes as have a row's columns, so that a warp has several narrow rows.  A lane has 16 bytes of a row whatever the loads, and with
-// that sums have the same order for every alignment.
 template <class T, int V>
 int launch_lanes(const GatherArgs &a, cudaStream_t stream)
 {
-    constexpr int kWide = 16 / sizeof(T), U = kWide / V;
-    return a.columns <= 4 * kWide ? launch_gather<T, V, U, 4>(a, stream) : a.columns <= 8 * kWide ? launch_gather<T, V, U, 8>(a, stream)
-         : a.columns <= 16 * kWide ? launch_gather<T, V, U, 16>(a, stream) : launch_gather<T, V, U, 32>(a, stream);
+    constexpr int U = 16 / sizeof(T) / V;
+    switch (team_lanes(a.columns, sizeof(T))) {
+    case 4: return launch_gather<T, V, U, 4>(a, stream);
+    case 8: return launch_gather<T, V, U, 8>(a, stream);
+    case 16: return launch_gather<T, V, U, 16>(a, stream);
+    default: return launch_gather<T, V, U, 32>(a, stream);
+    }
 }
 
-// The widest loads that rows of both arrays start at a boundary of.
+// The widest loads that rows of both arrays start at a boundary of.  Which lane has a column changes with that, the order of a sum does not.
 template <class T>
 int launch_gather(const GatherArgs &a, cudaStream_t stream)
 {
@@ -298,8 +364,12 @@ int launch_gather(const GatherArgs &a, cudaStream_t stream)
     return launch_lanes<T, 1>(a, stream);
 }
 
-int launch_gather(const GatherArgs &a, int type, cudaStream_t stream)
+int launch_gather(GatherArgs &a, int type, char *workspace, const GatherSpace &space, cudaStream_t stream)
 {
+    a.span = span_of(a.positions, a.columns, type_bytes(type));
+    a.spans = (a.positions + a.span - 1) / a.span;
+    a.head = (float *)(workspace + space.head), a.part = (float *)(workspace + space.part), a.ends = (int *)(workspace + space.ends);
+    a.partial_stride = (int)partial_stride(a.columns);
     return type == GTM_F32 ? launch_gather<float>(a, stream) : type == GTM_BF16 ? launch_gather<__nv_bfloat16>(a, stream) : launch_gather<__half>(a, stream);
 }
 
@@ -388,28 +458,14 @@ __global__ void __launch_bounds__(kSortThreads) sort_keys_kernel(const void *ids
     hist[threadIdx.x] = 0;
     __syncthreads();
     const long long first = sort_first<kEach>(), lane = threadIdx.x & 31;
-    long long bag = -1;
-    if (offsets && first - lane < n) bag = segment_at(offsets, offsets_wide, n, bags, first - lane);
+    long long base = -1;
+    if (offsets && first - lane < n) base = segment_at<32>(offsets, offsets_wide, n, bags, first - lane, ~0u);
 #pragma unroll
     for (int k = 0; k < kEach; k++) {
         const long long i = first + k * 32;
         if (i >= n) break;
-        const long long id = index_at(ids, ids_wide, i);
-        unsigned key = id < 0 || id >= (long long)rows ? rows : (unsigned)id;
-        if (offsets) {
-            // the bag of a later position is the same or one of the next; behind many empty ones, by halves
-            for (int tries = 0; tries < 8 && bag + 1 < bags && clamp_offset(offsets, offsets_wide, n, bag + 1) <= i; tries++) bag++;
-            long long high = bags;
-            if (bag + 1 < bags && clamp_offset(offsets, offsets_wide, n, bag + 1) <= i)
-                while (high - bag > 1) {
-                    const long long mid = (bag + high) / 2;
-                    if (clamp_offset(offsets, offsets_wide, n, mid) <= i) bag = mid;
-                    else high = mid;
-                }
-            if (bag < 0 || i >= clamp_offset(offsets, offsets_wide, n, bag + 1)) key = rows;
-        } else {
-            bag = i;
-        }
+        const long long id = index_at(ids, ids_wide, i), bag = offsets ? segment_from(offsets, offsets_wide, n, bags, base, i) : i;
+        const unsigned key = bag < 0 || id < 0 || id >= (long long)rows ? rows : (unsigned)id;
         pairs[i] = make_uint2(key, bag < 0 ? 0 : (unsigned)bag);
         atomicAdd(&hist[key & (kDigits - 1)], 1u);
     }
@@ -515,18 +571,16 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const uint2 *p
         if (first + k * 32 < n) sorted[warp_hist[warp][(pair[k].x >> shift) & (kDigits - 1)] + rank[k]] = pair[k];
 }
 
-// Where each row's positions begin in the sorted list (offsets[rows]: where ids that are no row begin), and the list of bags.  The
+// Where each row's positions begin in the sorted list (offsets[rows]: where ids that are no row begin).  The
 // pair at a position writes the offsets of the rows behind the pair before it; of many such rows, its warp does.
-__global__ void __launch_bounds__(256) sort_rows_kernel(const uint2 *sorted, long long n, long long rows, int *offsets, int *bags)
+__global__ void __launch_bounds__(256) sort_rows_kernel(const uint2 *sorted, long long n, long long rows, int *offsets)
 {
     const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
     const int lane = threadIdx.x & 31;
     long long low = 0, high = 0;                   // offsets [low, high) are t
     if (t <= n) {
-        const uint2 pair = t < n ? sorted[t] : make_uint2((unsigned)rows, 0u);
         low = t == 0 ? 0 : (long long)sorted[t - 1].x + 1;
-        high = t == n ? rows + 1 : (long long)pair.x + 1;
-        if (t < n) bags[t] = (int)pair.y;
+        high = t == n ? rows + 1 : (long long)sorted[t].x + 1;
     }
     if (high - low <= 8) {
         for (long long r = low; r < high; r++) offsets[r] = (int)t;
@@ -541,12 +595,11 @@ __global__ void __launch_bounds__(256) sort_rows_kernel(const uint2 *sorted, lon
 }
 
 struct GradientSpace {
-    uint64_t pairs[2], counts, offsets, bags, head, part, ends, total;
-    long long tiles, spans;
+    uint64_t pairs[2], counts, offsets, total;
+    GatherSpace gather;
+    long long tiles;
     int each;
 };
-
-int64_t partial_stride(int64_t columns) { return (int64_t)round_up(columns, 4); }
 
 GradientSpace gradient_space(long long ids, long long rows, long long columns)
 {
@@ -556,17 +609,12 @@ GradientSpace gradient_space(long long ids, long long rows, long long columns)
     // small blocks of pairs as long as they do not fill the GPU, large ones (fewer counts) then
     s.each = ids > 148 * 4 * kSortThreads * 4 ? 16 : 4;
     s.tiles = (ids + kSortThreads * s.each - 1) / (kSortThreads * s.each);
-    s.spans = (ids + kPiece - 1) / kPiece;
     s.pairs[0] = take(ids * 8);
     s.pairs[1] = take(ids * 8);
     s.counts = take(s.tiles * kDigits * 4);
     s.offsets = take((rows + 1) * 4);
-    s.bags = take(ids * 4);
-    const bool pieces = ids > kPiece;
-    s.head = take(pieces ? s.spans * partial_stride(columns) * 4 : 0);
-    s.part = take(pieces ? s.spans * partial_stride(columns) * 4 : 0);
-    s.ends = take(pieces ? s.spans * 4 : 0);
-    s.total = at;
+    s.gather = gather_space(at, ids, columns);
+    s.total = s.gather.total;
     return s;
 }
 
@@ -589,8 +637,7 @@ extern "C" int gtm_embed_workspace(int64_t ids, int64_t columns, int bags, uint6
 {
     if (!bytes_out) return fail(GTM_ERR_ARG, "gtm_embed_workspace: null output");
     GTM_TRY(check_sizes("gtm_embed_workspace", GTM_F32, 1, columns, ids, 0));
-    const uint64_t spans = bags && ids > kPiece ? (uint64_t)((ids + kPiece - 1) / kPiece) : 0;
-    *bytes_out = 2 * round_up(spans * partial_stride(columns) * 4, 256) + round_up(spans * 4, 256);
+    *bytes_out = bags ? gather_space(0, ids, columns).total : 0;
     return GTM_OK;
 }
 
@@ -602,7 +649,7 @@ extern "C" int gtm_embed(int device, void *cuda_stream, int type, const void *ta
     const int64_t segments = offsets ? number_of_bags : number_of_ids;
     if (segments == 0) return GTM_OK;
     if (!table || !out || (!ids && number_of_ids)) return fail(GTM_ERR_ARG, "gtm_embed: null array");
-    if (row_stride < 0) return fail(GTM_ERR_ARG, "gtm_embed: row stride %lld of the table", (long long)row_stride);
+    if (row_stride < 0 || row_stride >= kMostRows) return fail(GTM_ERR_ARG, "gtm_embed: row stride %lld of the table", (long long)row_stride);
     if ((uintptr_t)out % 16) return fail(GTM_ERR_ARG, "gtm_embed: the result does not start at a 16-byte boundary");
     uint64_t need = 0;
     GTM_TRY(gtm_embed_workspace(number_of_ids, columns, offsets != nullptr, &need));
@@ -620,10 +667,8 @@ extern "C" int gtm_embed(int device, void *cuda_stream, int type, const void *ta
     a.list = ids, a.list_wide = ids_64, a.positions = number_of_ids;
     a.offsets = offsets, a.offsets_wide = offsets_64, a.segments = segments;
     a.columns = (int)columns, a.scale = scale, a.out = out, a.out_stride = columns;
-    const uint64_t spans = (uint64_t)((number_of_ids + kPiece - 1) / kPiece), half = round_up(spans * partial_stride(columns) * 4, 256);
-    a.head = (float *)workspace, a.part = (float *)((char *)workspace + half), a.ends = (int *)((char *)workspace + 2 * half);
-    a.partial_stride = (int)partial_stride(columns);
-    return launch_gather(a, type, stream);
+    a.pairs = nullptr;
+    return launch_gather(a, type, (char *)workspace, gather_space(0, number_of_ids, columns), stream);
 }
 
 extern "C" int gtm_embed_gradient_workspace(int64_t ids, int64_t rows, int64_t columns, uint64_t *bytes_out)
@@ -640,7 +685,7 @@ extern "C" int gtm_embed_gradient(int device, void *cuda_stream, int type, const
 {
     GTM_TRY(check_sizes("gtm_embed_gradient", type, rows, columns, number_of_ids, number_of_bags));
     if (!table_gradient || (number_of_ids && (!ids || !gradient))) return fail(GTM_ERR_ARG, "gtm_embed_gradient: null array");
-    if (gradient_stride < 0 || row_stride < columns)
+    if (gradient_stride < 0 || gradient_stride >= kMostRows || row_stride < columns)
         return fail(GTM_ERR_ARG, "gtm_embed_gradient: row stride %lld of the gradient, %lld of the result", (long long)gradient_stride, (long long)row_stride);
     const GradientSpace space = gradient_space(number_of_ids, rows, columns);
     if (workspace_bytes < space.total || !workspace || (uintptr_t)workspace % 16)
@@ -671,14 +716,12 @@ extern "C" int gtm_embed_gradient(int device, void *cuda_stream, int type, const
         };
         GTM_TRY(space.each == 4 ? sort(std::integral_constant<int, 4>()) : sort(std::integral_constant<int, 16>()));
     }
-    sort_rows_kernel<<<(unsigned)((n + 256) / 256), 256, 0, stream>>>(from, n, rows, (int *)(w + space.offsets), (int *)(w + space.bags));
+    sort_rows_kernel<<<(unsigned)((n + 256) / 256), 256, 0, stream>>>(from, n, rows, (int *)(w + space.offsets));
     GTM_CU(cudaGetLastError());
     GatherArgs a;
     a.src = gradient, a.src_stride = gradient_stride, a.rows = offsets ? number_of_bags : n;
-    a.list = w + space.bags, a.list_wide = 0, a.positions = n;
+    a.pairs = from, a.list = nullptr, a.list_wide = 0, a.positions = n;
     a.offsets = w + space.offsets, a.offsets_wide = 0, a.segments = rows;
     a.columns = (int)columns, a.scale = scale, a.out = table_gradient, a.out_stride = row_stride;
-    a.head = (float *)(w + space.head), a.part = (float *)(w + space.part), a.ends = (int *)(w + space.ends);
-    a.partial_stride = (int)partial_stride(columns);
-    return launch_gather(a, type, stream);
+    return launch_gather(a, type, w, space.gather, stream);
 }
