@@ -82,13 +82,12 @@ PROTOTYPES = {
                   C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_uint64],
     "gtm_embed_gradient_workspace": [C.c_int64, C.c_int64, C.c_int64, C.POINTER(C.c_uint64)],
     "gtm_embed_gradient": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int,
-                           C.c_int64, C.c_float, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_uint64],
+                           C.c_int64, C.c_float, C.c_void_p, C.c_int64, C.c_void_p, C.c_uint64],
     "gtm_softmax_workspace": [C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.POINTER(C.c_uint64)],
     "gtm_softmax_loss": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int,
                          C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64],
     "gtm_softmax_loss_gradient": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p,
-                                  C.c_int, C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p,
-                                  C.c_uint64],
+                                  C.c_int, C.c_int64, C.c_float, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64],
     "gtm_softmax_predict": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_float, C.c_void_p,
                             C.c_void_p, C.c_void_p, C.c_uint64],
     "gtm_softmax_failed": [C.c_int, C.POINTER(C.c_int)],

@@ -681,12 +681,12 @@ extern "C" int gtm_embed_gradient_workspace(int64_t ids, int64_t rows, int64_t c
 
 extern "C" int gtm_embed_gradient(int device, void *cuda_stream, int type, const void *gradient, int64_t columns, int64_t gradient_stride,
                                   const void *ids, int ids_64, int64_t number_of_ids, const void *offsets, int offsets_64, int64_t number_of_bags,
-                                  float scale, void *table_gradient, int64_t rows, int64_t row_stride, void *workspace, uint64_t workspace_bytes)
+                                  float scale, void *table_gradient, int64_t rows, void *workspace, uint64_t workspace_bytes)
 {
     GTM_TRY(check_sizes("gtm_embed_gradient", type, rows, columns, number_of_ids, number_of_bags));
     if (!table_gradient || (number_of_ids && (!ids || !gradient))) return fail(GTM_ERR_ARG, "gtm_embed_gradient: null array");
-    if (gradient_stride < 0 || gradient_stride >= kMostRows || row_stride < columns)
-        return fail(GTM_ERR_ARG, "gtm_embed_gradient: row stride %lld of the gradient, %lld of the result", (long long)gradient_stride, (long long)row_stride);
+    if (gradient_stride < 0 || gradient_stride >= kMostRows) return fail(GTM_ERR_ARG, "gtm_embed_gradient: row stride %lld of the gradient", (long long)gradient_stride);
+    if ((uintptr_t)table_gradient % 16) return fail(GTM_ERR_ARG, "gtm_embed_gradient: the result does not start at a 16-byte boundary");
     const GradientSpace space = gradient_space(number_of_ids, rows, columns);
     if (workspace_bytes < space.total || !workspace || (uintptr_t)workspace % 16)
         return fail(GTM_ERR_ARG, "gtm_embed_gradient: workspace of %llu bytes, %llu needed (16-byte aligned)", (unsigned long long)workspace_bytes, (unsigned long long)space.total);
@@ -722,6 +722,6 @@ extern "C" int gtm_embed_gradient(int device, void *cuda_stream, int type, const
     a.src = gradient, a.src_stride = gradient_stride, a.rows = offsets ? number_of_bags : n;
     a.pairs = from, a.list = nullptr, a.list_wide = 0, a.positions = n;
     a.offsets = w + space.offsets, a.offsets_wide = 0, a.segments = rows;
-    a.columns = (int)columns, a.scale = scale, a.out = table_gradient, a.out_stride = row_stride;
+    a.columns = (int)columns, a.scale = scale, a.out = table_gradient, a.out_stride = columns;
     return launch_gather(a, type, w, space.gather, stream);
 }

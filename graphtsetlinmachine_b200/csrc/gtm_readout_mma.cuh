@@ -95,11 +95,11 @@ __device__ __forceinline__ unsigned long long operand(unsigned address, unsigned
     return (unsigned long long)((address & 0x3ffff) >> 4) | (unsigned long long)(leading >> 4) << 16 | (unsigned long long)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
 
-// Products of two 16-bit types (0: fp16, 1: bf16) in 32 bits, 256 rows over the pair.  `a_rows`, `b_rows`: the operand's rows
-// (and not its sum's index) lie next to each other in memory.
-__host__ __device__ constexpr unsigned product(int type, int columns, bool a_rows, bool b_rows)
+// Products of two 16-bit types (0: fp16, 1: bf16) in 32 bits, 256 rows over the pair.  `a_rows`: operand A's rows (and not its
+// sum's index) lie next to each other in memory.
+__host__ __device__ constexpr unsigned product(int type, int columns, bool a_rows)
 {
-    return 1u << 4 | (unsigned)type << 7 | (unsigned)type << 10 | (unsigned)a_rows << 15 | (unsigned)b_rows << 16 | (unsigned)(columns / 8) << 17 | (256u / 16) << 24;
+    return 1u << 4 | (unsigned)type << 7 | (unsigned)type << 10 | (unsigned)a_rows << 15 | (unsigned)(columns / 8) << 17 | (256u / 16) << 24;
 }
 
 __device__ __forceinline__ void multiply(unsigned to, unsigned long long a, unsigned long long b, unsigned what, bool add)
@@ -113,19 +113,25 @@ __device__ __forceinline__ void commit_to_pair(unsigned barrier)
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(barrier), "h"((unsigned short)3) : "memory");
 }
 
-// 32 columns of the warp's 32 rows: column i in v[i].
-__device__ __forceinline__ void tmem_load(unsigned from, float (&v)[32])
+// 64 columns of the warp's 32 rows: column i in v[i].
+__device__ __forceinline__ void tmem_load64(unsigned from, float (&v)[64])
 {
     unsigned *r = (unsigned *)v;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-                   "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-                   "=r"(r[31])
-                 : "r"(from));
+#pragma unroll
+    for (int h = 0; h < 64; h += 32)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                     "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                     : "=r"(r[h + 0]), "=r"(r[h + 1]), "=r"(r[h + 2]), "=r"(r[h + 3]), "=r"(r[h + 4]), "=r"(r[h + 5]), "=r"(r[h + 6]), "=r"(r[h + 7]), "=r"(r[h + 8]),
+                       "=r"(r[h + 9]), "=r"(r[h + 10]), "=r"(r[h + 11]), "=r"(r[h + 12]), "=r"(r[h + 13]), "=r"(r[h + 14]), "=r"(r[h + 15]), "=r"(r[h + 16]),
+                       "=r"(r[h + 17]), "=r"(r[h + 18]), "=r"(r[h + 19]), "=r"(r[h + 20]), "=r"(r[h + 21]), "=r"(r[h + 22]), "=r"(r[h + 23]), "=r"(r[h + 24]),
+                       "=r"(r[h + 25]), "=r"(r[h + 26]), "=r"(r[h + 27]), "=r"(r[h + 28]), "=r"(r[h + 29]), "=r"(r[h + 30]), "=r"(r[h + 31])
+                     : "r"(from + h));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+
+// The kernel behind this one may be set up while this one ends, and waits for its end before it reads what others have written.
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float exp2_fast(float x)
 {

@@ -7,7 +7,9 @@
 // every row, which a second kernel joins.  Backward, the labels are taken in pieces: a piece's logits are computed again, P of
 // the piece goes to the workspace in the operands' 16-bit type, and two products use it.  All products are one kernel on
 // tcgen05 over pairs of thread blocks: tiles of 256 x 256 (or 128), operands by TMA through a ring in shared memory, sums in tensor
-// memory, two tiles deep, so that a tile's epilogue runs under the next tile's products.
+// memory, two tiles deep, so that a tile's epilogue runs under the next tile's products; results leave by TMA too.  dw and dx of a piece are one
+// launch: dw's tiles go round, and dx's work fills up what is left of the last round.  For up to four examples (eight in 32 bits) the forward
+// pass is a kernel of plain dot products, whose time is that of reading w.
 //
 // 16-bit inputs are multiplied as they are, with sums in 32 bits.  32-bit inputs are split into three bf16 parts (24 bits of fraction),
 // and the six products of parts that reach 2^-24 are added, the smallest first.  P is rounded to the operands' type, to as many bits as
@@ -16,21 +18,24 @@
 #include "gtm_readout_mma.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace gtm_readout {
 namespace {
 
-constexpr int kStages = 6, kDepth = 64;                    // ring, and elements of a sum's index per stage
+constexpr int kDepth = 64;                                 // elements of a sum's index per stage of the ring
 constexpr int kHalfBytes = 128 * kDepth * 2;               // an operand's share of a stage in one thread block
 constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kThreads = 384, kEpilogue = 8;               // warps 0: copies, 1: products, 2: tensor memory; 4..11: epilogue
+constexpr int kBoxBytes = 32 * 128;                        // 32 rows of 128 bytes: what a warp of the epilogue stores at once, from two buffers in turn
 constexpr int kPairs = 74;                                 // pairs of SMs
-constexpr size_t kShared = 1024 + kStages * kStageBytes;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int64_t kPieceBytes = 128 << 20;                 // of P in the workspace at a time
 constexpr int64_t kStatBytes = 64 << 20;                   // of partial sums of exponentials at a time
 
 enum Epilogue { kSums = 0, kBest = 1, kProb = 2, kOut = 3 };
+__host__ __device__ constexpr int stages_of(int mode) { return mode == kSums || mode == kBest ? 6 : 5; }
+__host__ __device__ constexpr size_t shared_of(int mode) { return 1024 + stages_of(mode) * kStageBytes + (mode == kSums || mode == kBest ? 0 : kEpilogue * 2 * kBoxBytes); }
 
 // Parts of a 32-bit operand that are multiplied, the smallest products first: pairs (a, b) of two bits each.
 constexpr int kPartProducts = 6;
@@ -41,15 +46,61 @@ __device__ __forceinline__ void parts_of(int products, int i, int &a, int &b)
     b = products == 1 ? 0 : bs >> (2 * i) & 3;
 }
 
-struct Problem {
+// One product.  Its work is tiles of 256 rows over blocks of the sum's index (`blocks` of kDepth each, times products of parts).
+struct Product {
     long long rows, columns;                    // of the result
-    int m_tiles, n_tiles, splits, tile_columns; // 256 or 128 columns of a tile
+    int m_tiles, n_tiles, tile_columns;         // 256 or 128 columns of a tile
     int m_fast;                                 // tiles of one column block follow each other
-    int depth_blocks, products, per_split;      // blocks of kDepth of the sum's index; blocks (times products) of a split
-    int a_rows, b_rows;                         // operands whose rows, not the sum's index, lie next to each other
-    int a_first, b_first;                       // offset of the sum's index in the operand's tensor (a row of W)
+    int depth_blocks, products, blocks, per_split;  // blocks of a tile are cut into splits of per_split
+    int a_rows;                                 // operand A's rows, not the sum's index, lie next to each other (operand B's never do: that is a third slower)
+    int a_first;                                // offset of the sum's index in operand A (a row of W)
     int b_row;                                  // offset of the result's columns in operand B (a row of W)
     unsigned what;                              // instruction descriptor
+    int add;                                    // the result is added to what is there
+    int type;                                   // of the result: GTM_F32 (slices of sums too) or a 16-bit type
+    const unsigned *out_scale;                  // bits of the largest |factor|: the result is 2^-14 times this, null: 1
+
+    __host__ __device__ int tiles() const { return m_tiles * n_tiles; }
+    __host__ __device__ int splits() const { return (blocks + per_split - 1) / per_split; }
+    __host__ __device__ void tile(int t, int &m, int &n) const
+    {
+        if (m_fast) m = t % m_tiles, n = t / m_tiles;
+        else n = t % n_tiles, m = t / n_tiles;
+    }
+};
+
+// Who does what: the splits of the first product's tiles go to the pairs of SMs in turn; the blocks of the second one's tiles, in a row, are cut so
+// that all pairs end together, wherever in a tile that is.  The pieces of a tile are slices of sums, added up later.  A pair begins with the second product, whose
+// results are the larger ones: they leave while it works on the first.
+struct Schedule {
+    int items, pairs, longer;                   // of the first product; pairs that have one item more
+    int others;                                 // pairs behind those that share the rest of the second product's blocks
+    long long units, units_of_longer;           // blocks of the second product; of these, the share of the longer pairs
+
+    __host__ __device__ long long begin(int pair) const
+    {
+        if (pair <= longer) return longer ? units_of_longer * pair / longer : 0;
+        const int at = pair - longer < others ? pair - longer : others;
+        return units_of_longer + (units - units_of_longer) * at / others;
+    }
+    __host__ __device__ int pair_of(long long unit) const
+    {
+        int i = unit < units_of_longer ? (int)(unit * longer / units_of_longer) : longer + (int)((unit - units_of_longer) * others / (units - units_of_longer));
+        while (i > 0 && begin(i) > unit) i--;
+        while (i + 1 < pairs && begin(i + 1) <= unit) i++;
+        return i;
+    }
+    __host__ __device__ int slices(long long blocks, int tile) const { return pair_of((tile + 1) * blocks - 1) - pair_of(tile * blocks) + 1; }
+};
+
+// Tensor maps are the launch's own arguments; the second product's are used in kOut alone.
+struct Maps {
+    CUtensorMap a[2], b[2], out[2];
+};
+
+struct Launch {
+    Product p[2];
+    Schedule schedule;
     int *error;
     // kSums, kBest
     float2 *sums;                               // [part][rows]: largest product and sum of exponentials (kBest: all but the largest's)
@@ -62,87 +113,163 @@ struct Problem {
     // kProb
     const float *normalisers, *factors;         // [rows]
     const unsigned *largest;                    // bits of the largest |factor|, null: factors as they are
-    void *prob;
-    long long prob_stride, prob_part;           // elements
-    // kProb, kOut
-    int type;                                   // of the result
-    // kOut
-    void *out;
-    long long out_stride;
-    float *partial;                             // [split][rows][columns], instead of out
-    int add;                                    // to what partial holds
-    const unsigned *out_scale;                  // bits of the largest |factor|: the result is 2^-14 times this, null: 1
 };
 
-__device__ __forceinline__ void tile_at(const Problem &p, int t, int &m, int &n, int &split)
-{
-    const int tiles = p.m_tiles * p.n_tiles;
-    split = t / tiles;
-    t -= split * tiles;
-    if (p.m_fast) m = t % p.m_tiles, n = t / p.m_tiles;
-    else n = t % p.n_tiles, m = t / p.n_tiles;
-}
+// A pair's work, piece by piece.
+struct Work {
+    const Launch &l;
+    int pair, item;
+    long long unit, end;
+    // the piece at hand: product, tile, blocks [first, last)
+    int which, m, n, first, last, split;
 
-template <class T>
-__device__ __forceinline__ void store_columns(T *to, const float (&v)[32], int n)
-{
-    constexpr int kWide = 16 / sizeof(T);
-    if (n == 32 && (uintptr_t)to % 16 == 0) {
-#pragma unroll
-        for (int j = 0; j < 32; j += kWide) {
-            Pack<T, kWide> q;
-#pragma unroll
-            for (int k = 0; k < kWide; k++) q.v[k] = from_float<T>(v[j + k]);
-            *(Pack<T, kWide> *)(to + j) = q;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; j++)
-            if (j < n) to[j] = from_float<T>(v[j]);
+    __device__ __forceinline__ explicit Work(const Launch &launch) : l(launch)
+    {
+        pair = blockIdx.x / 2, item = pair;
+        unit = l.schedule.units ? l.schedule.begin(pair) : 0;
+        end = l.schedule.units ? l.schedule.begin(pair + 1) : 0;
     }
-}
+    __device__ __forceinline__ bool next()
+    {
+        if (unit < end) {
+            which = 1;
+            const int tile = (int)(unit / l.p[1].blocks);
+            l.p[1].tile(tile, m, n);
+            first = (int)(unit - (long long)tile * l.p[1].blocks), last = (int)min((long long)l.p[1].blocks, first + end - unit);
+            split = tile;                        // its slice is looked up by who needs it
+            unit += last - first;
+            return true;
+        }
+        if (item >= l.schedule.items) return false;
+        which = 0;
+        split = item / l.p[0].tiles();
+        l.p[0].tile(item - split * l.p[0].tiles(), m, n);
+        first = split * l.p[0].per_split, last = min(l.p[0].blocks, first + l.p[0].per_split);
+        item += l.schedule.pairs;
+        return true;
+    }
+    __device__ __forceinline__ int slice() const { return which == 0 ? split : pair - l.schedule.pair_of((long long)split * l.p[1].blocks); }
+};
 
-// Softmax statistics of a row, over the 32 products `v` at a time.
+// Softmax statistics of a row, over some of its products at a time.
 struct RowSums {
-    float largest = -INFINITY, sum = 0.f;
-    __device__ __forceinline__ void take(const float (&v)[32], float slope)
+    float largest, sum;
+    __device__ __forceinline__ static RowSums none() { return {-INFINITY, 0.f}; }
+    template <int N>
+    __device__ __forceinline__ void take(const float (&v)[N], float slope)
     {
         float top = v[0];
 #pragma unroll
-        for (int j = 1; j < 32; j++) top = fmaxf(top, v[j]);
+        for (int j = 1; j < N; j++) top = fmaxf(top, v[j]);
         const float next = fmaxf(largest, top), from = next == -INFINITY ? 0.f : next;
         if (largest > -INFINITY) sum *= exp2_fast((largest - from) * slope);
 #pragma unroll
-        for (int j = 0; j < 32; j++) sum += exp2_fast((v[j] - from) * slope);
+        for (int j = 0; j < N; j++) sum += exp2_fast((v[j] - from) * slope);
         largest = next;
     }
 };
 
 // The same with the first largest one's index and without its own 1 in the sum.
 struct RowBest {
-    float largest = -INFINITY, rest = 0.f;
-    int index = -1;
-    __device__ __forceinline__ void take(const float (&v)[32], float slope, int first)
+    float largest, rest;
+    int index;
+    __device__ __forceinline__ static RowBest none() { return {-INFINITY, 0.f, -1}; }
+    template <int N>
+    __device__ __forceinline__ void take(const float (&v)[N], float slope, int first)
     {
         float top = v[0];
         int at = 0;
 #pragma unroll
-        for (int j = 1; j < 32; j++)
+        for (int j = 1; j < N; j++)
             if (v[j] > top || !(top == top)) top = v[j], at = j;
         const float from = top == -INFINITY || !(top == top) ? 0.f : top;
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 32; j++) sum += j == at && top > -INFINITY ? 0.f : exp2_fast((v[j] - from) * slope);
+        for (int j = 0; j < N; j++) sum += j == at && top > -INFINITY ? 0.f : exp2_fast((v[j] - from) * slope);
+        add(top, sum, slope, first + at);
+    }
+    __device__ __forceinline__ void add(float top, float sum, float slope, int at)
+    {
         if (!(top > -INFINITY)) rest += sum;                       // nothing but -inf (sum is 0) or NaN
-        else if (top > largest) rest = (largest > -INFINITY ? (rest + 1.f) * exp2_fast((largest - top) * slope) : rest) + sum, largest = top, index = first + at;
+        else if (top > largest) rest = (largest > -INFINITY ? (rest + 1.f) * exp2_fast((largest - top) * slope) : rest) + sum, largest = top, index = at;
         else rest += (sum + 1.f) * exp2_fast((top - largest) * slope);
     }
 };
 
-template <int kMode>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-softmax_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Problem p)
+// A warp's boxes on their way to memory: written to one of two buffers, rows of 128 bytes swizzled as the map says, and stored from there.
+struct BoxStore {
+    unsigned buffers;
+    int turn = 0;
+    // 16-byte piece `j` (of 8) of the lane's row
+    __device__ __forceinline__ void put(int j, uint4 v) const
+    {
+        const unsigned lane = threadIdx.x & 31;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buffers + turn * kBoxBytes + lane * 128 + ((j ^ (lane & 7)) * 16)), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    }
+    // The buffer whose turn it is has been read.
+    __device__ __forceinline__ void begin() const
+    {
+        if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        __syncwarp();
+    }
+    __device__ __forceinline__ void send(const CUtensorMap *map, int x, int y, int z, bool add)
+    {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) {
+            if (add) asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(buffers + turn * kBoxBytes), "r"(x), "r"(y), "r"(z) : "memory");
+            else asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(buffers + turn * kBoxBytes), "r"(x), "r"(y), "r"(z) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        turn ^= 1;
+    }
+    __device__ __forceinline__ static void finish()
+    {
+        if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+};
+
+__device__ __forceinline__ unsigned pack2(float a, float b, bool fp16)
 {
+    if (fp16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return reinterpret_cast<const unsigned &>(h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return reinterpret_cast<const unsigned &>(h);
+}
+
+// 64 columns of 16 bits: one box.
+__device__ __forceinline__ void send_16(BoxStore &to, const float (&v)[64], bool fp16, const CUtensorMap *map, int x, int y, int z)
+{
+    to.begin();
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        to.put(j, make_uint4(pack2(v[j * 8], v[j * 8 + 1], fp16), pack2(v[j * 8 + 2], v[j * 8 + 3], fp16), pack2(v[j * 8 + 4], v[j * 8 + 5], fp16), pack2(v[j * 8 + 6], v[j * 8 + 7], fp16)));
+    to.send(map, x, y, z, false);
+}
+
+// 64 columns of 32 bits: two boxes, the second only where there are columns for it.
+__device__ __forceinline__ void send_32(BoxStore &to, const float (&v)[64], const CUtensorMap *map, int x, int y, int z, bool add, long long left)
+{
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (left <= h * 32) break;
+        to.begin();
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float *q = v + h * 32 + j * 4;
+            to.put(j, make_uint4(__float_as_uint(q[0]), __float_as_uint(q[1]), __float_as_uint(q[2]), __float_as_uint(q[3])));
+        }
+        to.send(map, x + h * 32, y, z, add);
+    }
+}
+
+template <int kMode>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax_product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Launch l)
+{
+    constexpr int kStages = stages_of(kMode);
+    constexpr bool kStores = kMode == kProb || kMode == kOut;
     extern __shared__ unsigned char shared_raw[];
     __shared__ alignas(8) unsigned long long barriers[2 * kStages + 4];
     __shared__ unsigned tmem_shared;
@@ -150,6 +277,7 @@ softmax_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     const unsigned full = smem_address(barriers), empty = full + 8 * kStages, sums_full = empty + 8 * kStages, sums_empty = sums_full + 16;
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
     const unsigned rank = cluster_rank();
+    next_may_start();
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; i++) barrier_init(full + 8 * i, 1), barrier_init(empty + 8 * i, 1);
         for (int i = 0; i < 2; i++) barrier_init(sums_full + 8 * i, 1), barrier_init(sums_empty + 8 * i, 2 * kEpilogue);
@@ -161,31 +289,30 @@ softmax_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     cluster_sync();
     tmem_after_sync();
     const unsigned tmem = tmem_shared;
+    wait_for_previous();
 
-    const int tiles = p.m_tiles * p.n_tiles * p.splits, first_tile = blockIdx.x / 2, tile_step = gridDim.x / 2;
-    const int half_columns = p.tile_columns / 2, all_blocks = p.depth_blocks * p.products;
     bool fine = true;
     if (warp == 0 && lane == 0) {
         // copies: the ring's stages of this block, counted on the leader's barriers
         int stage = 0, phase = 0;
-        for (int t = first_tile; t < tiles && fine; t += tile_step) {
-            int m, n, split;
-            tile_at(p, t, m, n, split);
-            const int m0 = m * 256 + (int)rank * 128, n0 = n * p.tile_columns + (int)rank * half_columns + p.b_row;
-            const int last = min(all_blocks, (split + 1) * p.per_split);
-            for (int i = split * p.per_split; i < last; i++) {
+        for (Work w(l); fine && w.next();) {
+            const Product &p = l.p[w.which];
+            const CUtensorMap *map_a = &maps.a[w.which], *map_b = &maps.b[w.which];
+            const int half_columns = p.tile_columns / 2;
+            const int m0 = w.m * 256 + (int)rank * 128, n0 = w.n * p.tile_columns + (int)rank * half_columns + p.b_row;
+            int product = w.first / p.depth_blocks, block = w.first - product * p.depth_blocks;
+            for (int i = w.first; i < w.last; i++) {
                 if (!(fine = barrier_wait(empty + 8 * stage, phase ^ 1))) break;
                 const unsigned to = ring + stage * kStageBytes, bar = in_leader(full + 8 * stage);
                 if (rank == 0) barrier_expect(full + 8 * stage, 2 * (kHalfBytes + half_columns * kDepth * 2));
                 int part_a, part_b;
-                parts_of(p.products, i / p.depth_blocks, part_a, part_b);
-                const int k = i % p.depth_blocks * kDepth;
+                parts_of(p.products, product, part_a, part_b);
+                const int k = block * kDepth;
                 if (p.a_rows)
-                    for (int g = 0; g < 2; g++) load_box(&map_a, to + g * 8192, bar, m0 + g * 64, p.a_first + k, part_a);
-                else load_box(&map_a, to, bar, p.a_first + k, m0, part_a);
-                if (p.b_rows)
-                    for (int g = 0; g < half_columns / 64; g++) load_box(&map_b, to + kHalfBytes + g * 8192, bar, n0 + g * 64, p.b_first + k, part_b);
-                else load_box(&map_b, to + kHalfBytes, bar, p.b_first + k, n0, part_b);
+                    for (int g = 0; g < 2; g++) load_box(map_a, to + g * 8192, bar, m0 + g * 64, p.a_first + k, part_a);
+                else load_box(map_a, to, bar, k, m0, part_a);
+                load_box(map_b, to + kHalfBytes, bar, k, n0, part_b);
+                if (++block == p.depth_blocks) block = 0, product++;
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
         }
@@ -199,23 +326,21 @@ softmax_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             for (const unsigned long long began = nanoseconds(); nanoseconds() - began < 20000000ull;) __nanosleep(1000);
     } else if (warp == 1 && lane == 0 && rank == 0) {
         int stage = 0, phase = 0, buffer = 0, buffer_phase = 0;
-        // rows next to each other: 64 of them and 8 of the sum's index are 1024 bytes, 64 more rows one box further; a step of 16 is 2048 bytes.
-        // the sum's index next to each other: 8 rows are 1024 bytes; a step of 16 is 32 bytes
-        const unsigned a_leading = p.a_rows ? 8192 : 16, b_leading = p.b_rows ? 8192 : 16, a_step = p.a_rows ? 2048 : 32, b_step = p.b_rows ? 2048 : 32;
-        for (int t = first_tile; t < tiles && fine; t += tile_step) {
-            int m, n, split;
-            tile_at(p, t, m, n, split);
+        for (Work w(l); fine && w.next();) {
+            const Product &p = l.p[w.which];
+            // rows next to each other: 64 of them and 8 of the sum's index are 1024 bytes, 64 more rows one box further; a step of 16 is 2048 bytes.
+            // the sum's index next to each other: 8 rows are 1024 bytes; a step of 16 is 32 bytes
+            const unsigned a_leading = p.a_rows ? 8192 : 16, a_step = p.a_rows ? 2048 : 32, what = p.what;
             if (!(fine = barrier_wait(sums_empty + 8 * buffer, buffer_phase ^ 1))) break;
             tmem_after_sync();
             const unsigned to = tmem + buffer * 256;
-            const int first = split * p.per_split, last = min(all_blocks, first + p.per_split);
-            for (int i = first; i < last; i++) {
+            for (int i = w.first; i < w.last; i++) {
                 if (!(fine = barrier_wait(full + 8 * stage, phase))) break;
                 tmem_after_sync();
                 const unsigned a = ring + stage * kStageBytes, b = a + kHalfBytes;
 #pragma unroll
                 for (int k = 0; k < kDepth / 16; k++)
-                    multiply(to, operand(a + k * a_step, a_leading, 1024), operand(b + k * b_step, b_leading, 1024), p.what, i > first || k > 0);
+                    multiply(to, operand(a + k * a_step, a_leading, 1024), operand(b + k * 32, 16, 1024), what, i > w.first || k > 0);
                 commit_to_pair(empty + 8 * stage);
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
@@ -224,106 +349,105 @@ softmax_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
             if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
         }
     } else if (warp >= 4) {
-        const int w = (warp - 4) & 3, half = (warp - 4) / 4;
+        const int quarter = (warp - 4) & 3, half = (warp - 4) / 4;
         int buffer = 0, buffer_phase = 0;
-        for (int t = first_tile; t < tiles; t += tile_step) {
-            int m, n, split;
-            tile_at(p, t, m, n, split);
-            fine = barrier_wait(sums_full + 8 * buffer, buffer_phase);
-            if (!__all_sync(~0u, fine)) break;
-            tmem_after_sync();
-            const long long row = (long long)m * 256 + rank * 128 + w * 32 + lane;
+        BoxStore store = {ring + kStages * kStageBytes + (warp - 4) * 2 * kBoxBytes};
+        for (Work w(l); w.next();) {
+            const Product &p = l.p[w.which];
+            const int half_columns = p.tile_columns / 2;
+            const long long row0 = (long long)w.m * 256 + rank * 128 + quarter * 32, row = row0 + lane;
             const bool real = row < p.rows;
-            const unsigned from = tmem + buffer * 256 + half * half_columns + ((unsigned)(w * 32) << 16);
-            const long long column0 = (long long)n * p.tile_columns + half * half_columns;
-            RowSums sums;
-            RowBest best;
+            const long long column0 = (long long)w.n * p.tile_columns + half * half_columns;
+            RowSums sums = RowSums::none();
+            RowBest best = RowBest::none();
             float normaliser = 0.f, factor = 0.f;
-            int label = -1;
-            if ((kMode == kSums || kMode == kProb) && real && p.labels) label = p.labels[row] - p.first_label;
+            int label = -1, slice = 0;
+            if ((kMode == kSums || kMode == kProb) && real && l.labels) label = l.labels[row] - l.first_label;
             if (kMode == kProb && real) {
-                normaliser = p.normalisers[row], factor = p.factors[row];
-                if (p.largest) {
-                    const float largest = __uint_as_float(*p.largest);
+                normaliser = l.normalisers[row], factor = l.factors[row];
+                if (l.largest) {
+                    const float largest = __uint_as_float(*l.largest);
                     factor = largest == 0.f ? 0.f : factor / largest * 16384.f;
                 }
             }
+            if (kMode == kOut) slice = w.slice();
             const float out_scale = kMode == kOut && p.out_scale ? __uint_as_float(*p.out_scale) * (1.f / 16384.f) : 1.f;
-            for (int c = 0; c < half_columns; c += 32) {
-                float v[32];
-                tmem_load(from + c, v);
+            fine = barrier_wait(sums_full + 8 * buffer, buffer_phase);
+            if (!__all_sync(~0u, fine)) break;
+            tmem_after_sync();
+            const unsigned from = tmem + buffer * 256 + half * half_columns + ((unsigned)(quarter * 32) << 16);
+#pragma unroll 1
+            for (int c = 0; c < half_columns; c += 64) {
                 const long long column = column0 + c, left = p.columns - column;
-                if (left <= 0) continue;                                    // the warp together
+                if (left <= 0) break;                                       // the warp together
+                float v[64];
+                tmem_load64(from + c, v);
+                if (c + 64 >= half_columns || left <= 64) {
+                    // the tile's last columns are in registers: the next but one may overwrite it
+                    tmem_before_sync();
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive_leader(in_leader(sums_empty + 8 * buffer));
+                }
                 if (kMode == kSums || kMode == kBest) {
-                    if (left < 32)
+                    if (left < 64)
 #pragma unroll
-                        for (int j = 0; j < 32; j++)
+                        for (int j = 0; j < 64; j++)
                             if (j >= left) v[j] = -INFINITY;
                     if (kMode == kSums) {
-                        sums.take(v, p.scale * kLog2e);
+                        sums.take(v, l.scale * kLog2e);
                         const long long at = label - column;
-                        if (__any_sync(~0u, at >= 0 && at < 32 && label >= 0)) {
+                        if (__any_sync(~0u, at >= 0 && at < 64 && label >= 0)) {
                             float mine = 0.f;
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
+                            for (int j = 0; j < 64; j++)
                                 if (at == j) mine = v[j];
-                            if (label >= 0 && at >= 0 && at < 32 && real) p.label_logit[row] = mine;
+                            if (label >= 0 && at >= 0 && at < 64 && real) l.label_logit[row] = mine;
                         }
                     } else {
-                        best.take(v, p.scale * kLog2e, (int)column);
+                        best.take(v, l.scale * kLog2e, (int)column);
                     }
                 } else if (kMode == kProb) {
+#pragma unroll
+                    for (int j = 0; j < 64; j++) v[j] = exp2_fast(fmaf(v[j], l.scale, -normaliser) * kLog2e);
                     const long long at = label - column;
+                    if (__any_sync(~0u, at >= 0 && at < 64))
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        float q = exp2_fast(fmaf(v[j], p.scale, -normaliser) * kLog2e);
-                        if (at == j) q -= 1.f;
-                        v[j] = factor == 0.f ? 0.f : q * factor;
-                    }
-                    if (real) {
-                        const long long to = row * p.prob_stride + column;
-                        if (p.type == GTM_F16) store_columns((__half *)p.prob + to, v, 32);
-                        else {
-                            store_columns((__nv_bfloat16 *)p.prob + to, v, 32);
-                            if (p.products > 1)
-                                for (int part = 1; part < 3; part++) {
+                        for (int j = 0; j < 64; j++)
+                            if (at == j) v[j] -= 1.f;
 #pragma unroll
-                                    for (int j = 0; j < 32; j++) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
-                                    store_columns((__nv_bfloat16 *)p.prob + part * p.prob_part + to, v, 32);
-                                }
+                    for (int j = 0; j < 64; j++) v[j] = factor == 0.f ? 0.f : v[j] * factor;
+                    if (row0 >= p.rows) continue;                           // the warp together
+                    send_16(store, v, p.type == GTM_F16, &maps.out[0], (int)column, (int)row0, 0);
+                    if (p.products > 1)
+#pragma unroll 1
+                        for (int part = 1; part < 3; part++) {
+#pragma unroll
+                            for (int j = 0; j < 64; j++) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
+                            send_16(store, v, false, &maps.out[0], (int)column, (int)row0, part);
                         }
-                    }
-                } else if (real) {
-                    const int n_left = left < 32 ? (int)left : 32;
-                    if (p.partial) {
-                        float *to = p.partial + (split * p.rows + row) * p.columns + column;
-                        if (p.add)
+                } else {
 #pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (j < n_left) v[j] += to[j];
-                        store_columns(to, v, n_left);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] *= out_scale;
-                        const long long to = row * p.out_stride + column;
-                        if (p.type == GTM_F32) store_columns((float *)p.out + to, v, n_left);
-                        else if (p.type == GTM_F16) store_columns((__half *)p.out + to, v, n_left);
-                        else store_columns((__nv_bfloat16 *)p.out + to, v, n_left);
-                    }
+                    for (int j = 0; j < 64; j++) v[j] *= out_scale;
+                    if (row0 >= p.rows) continue;
+                    if (p.type == GTM_F32) send_32(store, v, &maps.out[w.which], (int)column, (int)row0, slice, p.add, left);
+                    else send_16(store, v, p.type == GTM_F16, &maps.out[w.which], (int)column, (int)row0, slice);
                 }
             }
-            if ((kMode == kSums || kMode == kBest) && real) {
-                const long long at = (n * 2ll + half) * p.rows + row;
-                p.sums[at] = kMode == kSums ? make_float2(sums.largest, sums.sum) : make_float2(best.largest, best.rest);
-                if (kMode == kBest) p.best[at] = best.index;
+            if (column0 >= p.columns) {                                     // no column of this half
+                tmem_before_sync();
+                __syncwarp();
+                if (lane == 0) barrier_arrive_leader(in_leader(sums_empty + 8 * buffer));
             }
-            tmem_before_sync();
-            __syncwarp();
-            if (lane == 0) barrier_arrive_leader(in_leader(sums_empty + 8 * buffer));
+            if ((kMode == kSums || kMode == kBest) && real) {
+                const long long at = (w.n * 2ll + half) * p.rows + row;
+                l.sums[at] = kMode == kSums ? make_float2(sums.largest, sums.sum) : make_float2(best.largest, best.rest);
+                if (kMode == kBest) l.best[at] = best.index;
+            }
             if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
         }
+        if (kStores) BoxStore::finish();
     }
-    if (!fine) atomicExch(p.error, 1);
+    if (!fine) atomicExch(l.error, 1);
     __syncwarp();
     tmem_before_sync();
     cluster_sync();
@@ -331,26 +455,209 @@ softmax_product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     if (warp == 2) tmem_free(tmem, 512);
 }
 
-// ------------------------------------------------------------------------------------------- around the products
-// Rows of a matrix with 16-byte boundaries, in parts where they are 32-bit ones; rows of examples that are ignored are zero.
-template <class T>
-__global__ void __launch_bounds__(256) softmax_lay_out_kernel(const T *from, long long stride, long long rows, int columns, const int *labels, void *to, long long to_stride, long long part)
+// The forward pass for few examples, whose time is that of reading the weights: dot products in 32 bits, four rows of weights in a warp at
+// a time, of every lane 16 bytes (or, where rows start anywhere, an element).  A lane keeps the statistics of one of the four rows' products with one example;
+// a block leaves one part.
+constexpr int kFewRows = 4, kFewThreads = 256;
+
+struct FewArgs {
+    const void *x, *w;
+    long long x_stride, w_stride;
+    int examples, labels, columns;
+    float scale;
+    const int *wanted;                          // labels of the examples, null: none
+    float2 *sums;
+    int *best;
+    float *label_logit;
+};
+
+template <class T, int kExamples, bool kWhole, bool kFindBest>
+__global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs a)
 {
-    const long long all = rows * columns;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
-        const long long r = i / columns, c = i - r * columns;
-        const bool kept = !labels || labels[r] != -1;
-        if constexpr (sizeof(T) == 4) {
-            float v = kept ? from[r * stride + c] : 0.f;
-            __nv_bfloat16 *q = (__nv_bfloat16 *)to + r * to_stride + c;
+    constexpr int V = kWhole ? 16 / sizeof(T) : 1, kValues = kExamples * kFewRows, kStep = 32 * V;
+    extern __shared__ float4 shared_x4[];
+    float *shared_x = (float *)shared_x4;       // [example][columns, rounded up to the step]
+    __shared__ RowSums block_sums[kFewThreads / 32][kValues];
+    __shared__ RowBest block_best[kFewThreads / 32][kValues];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, padded = (a.columns + kStep - 1) / kStep * kStep;
+    for (int i = threadIdx.x; i < kExamples * padded; i += kFewThreads) {
+        const int e = i / padded, c = i - e * padded;
+        shared_x[i] = e < a.examples && c < a.columns ? to_float(((const T *)a.x)[e * a.x_stride + c]) : 0.f;
+    }
+    __syncthreads();
+    RowSums sums = RowSums::none();
+    RowBest best = RowBest::none();
+    const int my_row = lane / kExamples, my_example = lane % kExamples;     // lanes behind kValues keep nothing
+    const int wanted = a.wanted && lane < kValues && my_example < a.examples ? a.wanted[my_example] : -1;
+    for (long long v0 = ((long long)blockIdx.x * (kFewThreads / 32) + warp) * kFewRows; v0 < a.labels; v0 += (long long)gridDim.x * (kFewThreads / 32) * kFewRows) {
+        float dot[kFewRows][kExamples];
+        const T *row[kFewRows];
 #pragma unroll
-            for (int k = 0; k < 3; k++) {
-                const __nv_bfloat16 b = __float2bfloat16_rn(v);
-                q[k * part] = b;
-                v = fabsf(__bfloat162float(b)) <= 3.4e38f ? v - __bfloat162float(b) : 0.f;
+        for (int r = 0; r < kFewRows; r++) {
+            row[r] = (const T *)a.w + min(v0 + r, (long long)a.labels - 1) * a.w_stride;
+#pragma unroll
+            for (int e = 0; e < kExamples; e++) dot[r][e] = 0.f;
+        }
+#pragma unroll 2
+        for (int c0 = 0; c0 < a.columns; c0 += kStep) {
+            const int c = c0 + lane * V;
+            Pack<T, V> w[kFewRows];
+#pragma unroll
+            for (int r = 0; r < kFewRows; r++)
+                if (c < a.columns) w[r] = *(const Pack<T, V> *)(row[r] + c);
+                else
+#pragma unroll
+                    for (int i = 0; i < V; i++) w[r].v[i] = from_float<T>(0.f);
+#pragma unroll
+            for (int e = 0; e < kExamples; e++) {
+                float x[V];
+                if constexpr (kWhole)
+#pragma unroll
+                    for (int i = 0; i < V; i += 4) reinterpret_cast<float4 &>(x[i]) = *(const float4 *)(shared_x + e * padded + c + i);
+                else x[0] = shared_x[e * padded + c];
+#pragma unroll
+                for (int r = 0; r < kFewRows; r++)
+#pragma unroll
+                    for (int i = 0; i < V; i++) dot[r][e] = fmaf(to_float(w[r].v[i]), x[i], dot[r][e]);
+            }
+        }
+        float mine = 0.f;
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++)
+#pragma unroll
+            for (int e = 0; e < kExamples; e++) {
+#pragma unroll
+                for (int o = 16; o; o /= 2) dot[r][e] += __shfl_xor_sync(~0u, dot[r][e], o);
+                if (lane == r * kExamples + e) mine = dot[r][e];
+            }
+        if (lane < kValues && v0 + my_row < a.labels) {
+            const float one[1] = {mine};
+            if (kFindBest) best.take(one, a.scale * kLog2e, (int)(v0 + my_row));
+            else sums.take(one, a.scale * kLog2e);
+            if (wanted == v0 + my_row) a.label_logit[my_example] = mine;
+        }
+    }
+    if (lane < kValues) block_sums[warp][lane] = sums, block_best[warp][lane] = best;
+    __syncthreads();
+    if (threadIdx.x >= kExamples || threadIdx.x >= a.examples) return;
+    const float slope = a.scale * kLog2e;
+    RowSums all = RowSums::none();
+    RowBest top = RowBest::none();
+    for (int w = 0; w < kFewThreads / 32; w++)
+        for (int r = 0; r < kFewRows; r++) {
+            const RowSums s = block_sums[w][r * kExamples + threadIdx.x];
+            const RowBest b = block_best[w][r * kExamples + threadIdx.x];
+            if (kFindBest) {
+                // labels of different warps are in no order: of equal products the lower label is the best
+                const bool lower = b.largest == top.largest && b.index < top.index;
+                const int index = b.index;
+                top.add(b.largest, b.rest, slope, index);
+                if (lower && b.largest > -INFINITY) top.index = index;
+            } else {
+                const float next = fmaxf(all.largest, s.largest);
+                if (next == -INFINITY) all.sum += s.sum;
+                else all.sum = (all.largest > -INFINITY ? all.sum * exp2_fast((all.largest - next) * slope) : all.sum) + (s.largest > -INFINITY ? s.sum * exp2_fast((s.largest - next) * slope) : s.sum);
+                all.largest = next;
+            }
+        }
+    const long long at = (long long)blockIdx.x * a.examples + threadIdx.x;
+    a.sums[at] = kFindBest ? make_float2(top.largest, top.rest) : make_float2(all.largest, all.sum);
+    if (kFindBest) a.best[at] = top.index;
+}
+
+// ------------------------------------------------------------------------------------------- around the products
+// Rows of a matrix with 16-byte boundaries, in parts where they are 32-bit ones; rows of examples that are ignored are zero.  A thread has eight
+// elements in a row; kWhole: rows start at 16-byte boundaries and have all eight.
+template <class T, bool kWhole>
+__global__ void __launch_bounds__(256) softmax_lay_out_kernel(const T *from, long long stride, long long rows, int columns, const int *labels, __nv_bfloat16 *to, long long to_stride, long long part)
+{
+    constexpr int kWide = 16 / sizeof(T);
+    const int per_row = (columns + 7) / 8;
+    const long long all = rows * per_row;
+    const bool narrow = all < 1ll << 32;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+        const long long r = narrow ? (long long)((unsigned)i / (unsigned)per_row) : i / per_row;
+        const int c = (int)(i - r * per_row) * 8;
+        const bool kept = !labels || labels[r] != -1;
+        Pack<T, 8> v;
+        if (kWhole && kept) {
+#pragma unroll
+            for (int k = 0; k < 8; k += kWide) reinterpret_cast<Pack<T, kWide> &>(v.v[k]) = *(const Pack<T, kWide> *)(from + r * stride + c + k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v.v[k] = kept && c + k < columns ? from[r * stride + c + k] : from_float<T>(0.f);
+        }
+        // the copy's rows have room up to a multiple of eight
+        __nv_bfloat16 *q = to + r * to_stride + c;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int p = 0; p < 3; p++) {
+                Pack<__nv_bfloat16, 8> b;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    b.v[k] = __float2bfloat16_rn(v.v[k]);
+                    const float held = __bfloat162float(b.v[k]);
+                    v.v[k] = fabsf(held) <= 3.4e38f ? v.v[k] - held : 0.f;
+                }
+                *(Pack<__nv_bfloat16, 8> *)(q + p * part) = b;
             }
         } else {
-            ((T *)to)[r * to_stride + c] = kept ? from[r * stride + c] : from_float<T>(0.f);
+            *(Pack<T, 8> *)q = v;
+        }
+    }
+}
+
+// The gradient's x: rows as above, and the same matrix with rows for columns, which dw's product takes.  A block has 64 rows and 64 columns.
+template <class T>
+__global__ void __launch_bounds__(256) softmax_lay_out_both_kernel(const T *from, long long stride, long long rows, int columns, const int *labels, __nv_bfloat16 *to, long long to_stride, long long part,
+                                                                   __nv_bfloat16 *turned, long long turned_stride, long long turned_part, bool whole)
+{
+    using Out = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
+    constexpr int kParts = sizeof(T) == 4 ? 3 : 1, kWide = 16 / sizeof(T);
+    __shared__ Out tile[kParts][64][72];                      // rows of 144 bytes: eight of them read as columns meet different banks
+    const long long row0 = (long long)blockIdx.x * 64;
+    const int column0 = blockIdx.y * 64, c8 = threadIdx.x % 8 * 8, r0 = threadIdx.x / 8;
+#pragma unroll
+    for (int h = 0; h < 64; h += 32) {
+        const long long r = row0 + r0 + h;
+        const int c = column0 + c8;
+        const bool kept = r < rows && (!labels || labels[r] != -1);
+        Pack<T, 8> v;
+        if (whole && kept && c < columns) {
+#pragma unroll
+            for (int k = 0; k < 8; k += kWide) reinterpret_cast<Pack<T, kWide> &>(v.v[k]) = *(const Pack<T, kWide> *)(from + r * stride + c + k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) v.v[k] = kept && c + k < columns ? from[r * stride + c + k] : from_float<T>(0.f);
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+            Pack<Out, 8> b;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                if constexpr (kParts == 1) b.v[k] = v.v[k];
+                else {
+                    b.v[k] = __float2bfloat16_rn(v.v[k]);
+                    const float held = __bfloat162float(b.v[k]);
+                    v.v[k] = fabsf(held) <= 3.4e38f ? v.v[k] - held : 0.f;
+                }
+            }
+            if (r < rows && c < columns) *(Pack<Out, 8> *)((Out *)to + p * part + r * to_stride + c) = b;
+            *(Pack<Out, 8> *)&tile[p][r0 + h][c8] = b;
+        }
+    }
+    __syncthreads();
+    // the columns: eight rows of one at a time
+#pragma unroll
+    for (int h = 0; h < 64; h += 32) {
+        const int c = threadIdx.x % 32 + h, r8 = threadIdx.x / 32 * 8;
+        if (column0 + c >= columns || row0 + r8 >= rows) continue;
+#pragma unroll
+        for (int p = 0; p < kParts; p++) {
+            Pack<Out, 8> b;
+#pragma unroll
+            for (int k = 0; k < 8; k++) b.v[k] = tile[p][r8 + k][c];
+            *(Pack<Out, 8> *)((Out *)turned + p * turned_part + (column0 + c) * turned_stride + row0 + r8) = b;
         }
     }
 }
@@ -370,92 +677,181 @@ __global__ void __launch_bounds__(256) softmax_rows_kernel(const void *labels, i
     if (largest) atomicMax(largest, __float_as_uint(fabsf(f)));      // of magnitudes: the bits have their order, NaN above all
 }
 
-// Joins the parts of 32 rows; a row's parts are read by 32 threads.
+// Statistics of two sets of a row's products, joined.
+struct JoinSums {
+    float top, sum;
+    __device__ __forceinline__ static JoinSums none() { return {-INFINITY, 0.f}; }
+    __device__ __forceinline__ void join(JoinSums o, float scale)
+    {
+        const float next = fmaxf(top, o.top);
+        if (next == -INFINITY) sum += o.sum;
+        else sum = (top == -INFINITY ? sum : sum * expf((top - next) * scale)) + (o.top == -INFINITY ? o.sum : o.sum * expf((o.top - next) * scale));
+        top = next;
+    }
+    __device__ __forceinline__ JoinSums from(int lane_xor) const
+    {
+        JoinSums o;
+        o.top = __shfl_xor_sync(~0u, top, lane_xor), o.sum = __shfl_xor_sync(~0u, sum, lane_xor);
+        return o;
+    }
+    __device__ __forceinline__ static JoinSums read(const float2 *sums, const int *, long long at)
+    {
+        JoinSums s;
+        s.top = sums[at].x, s.sum = sums[at].y;
+        return s;
+    }
+};
+
+struct JoinBest {
+    float top, rest;
+    int index;
+    __device__ __forceinline__ static JoinBest none() { return {-INFINITY, 0.f, 0x7fffffff}; }
+    __device__ __forceinline__ void join(JoinBest o, float scale)
+    {
+        if (o.top == -INFINITY) { rest += o.rest; return; }
+        if (top == -INFINITY) { o.rest += rest; *this = o; return; }
+        const bool other = o.top > top || (o.top == top && o.index < index);
+        const float low = other ? top : o.top, high = other ? o.top : top;
+        rest = (other ? o.rest : rest) + (1.f + (other ? rest : o.rest)) * expf((low - high) * scale);
+        top = high, index = other ? o.index : index;
+    }
+    __device__ __forceinline__ JoinBest from(int lane_xor) const
+    {
+        JoinBest o;
+        o.top = __shfl_xor_sync(~0u, top, lane_xor), o.rest = __shfl_xor_sync(~0u, rest, lane_xor), o.index = __shfl_xor_sync(~0u, index, lane_xor);
+        return o;
+    }
+    __device__ __forceinline__ static JoinBest read(const float2 *sums, const int *best, long long at)
+    {
+        JoinBest s;
+        s.top = sums[at].x, s.rest = sums[at].y, s.index = best[at];
+        return s;
+    }
+};
+
+// Joins the parts of kRows rows: a row's parts are read by 1024 / kRows threads, four at a time, joined by warps and then by one warp.  Returns
+// the row of the thread and whether it has the result.
+template <class J, int kRows>
+__device__ __forceinline__ bool join_parts(const float2 *sums, const int *best, long long rows, int parts, float scale, J &mine, long long &row)
+{
+    constexpr int kEach = 1024 / kRows, kWarps = kEach / 32;          // threads and warps of a row
+    __shared__ J shared[kRows][kEach + 1];
+    const int x = threadIdx.x % kRows, y = threadIdx.x / kRows;
+    const long long from = (long long)blockIdx.x * kRows + x;
+    J all = J::none();
+    if (from < rows)
+        for (int i = y; i < parts; i += 4 * kEach) {
+            J part[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i + k * kEach < parts) part[k] = J::read(sums, best, (long long)(i + k * kEach) * rows + from);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i + k * kEach < parts) all.join(part[k], scale);
+        }
+    shared[x][y] = all;
+    __syncthreads();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, r = warp / kWarps;
+    mine = shared[r][warp % kWarps * 32 + lane];
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) mine.join(mine.from(o), scale);
+    row = (long long)blockIdx.x * kRows + r;
+    if (kWarps == 1) return lane == 0 && row < rows;
+    __shared__ J last[32];
+    if (lane == 0) last[warp] = mine;
+    __syncthreads();
+    if (warp) return false;
+    mine = last[lane];
+#pragma unroll
+    for (int o = 1; o < kWarps; o *= 2) mine.join(mine.from(o), scale);
+    row = (long long)blockIdx.x * kRows + lane / kWarps;
+    return lane % kWarps == 0 && row < rows;
+}
+
+template <int kRows>
 __global__ void __launch_bounds__(1024) softmax_loss_kernel(const float2 *sums, const float *label_logit, const int *labels, long long rows, int parts, float scale, float *losses,
                                                             float *normalisers)
 {
-    __shared__ float tops[32][33], all[32][33];
-    const int x = threadIdx.x & 31, y = threadIdx.x / 32;
-    const long long row = (long long)blockIdx.x * 32 + x;
-    float top = -INFINITY, sum = 0.f;
-    const auto join = [&](float t, float s) {
-        const float next = fmaxf(top, t);
-        if (next == -INFINITY) { sum += s; return; }
-        sum = (top == -INFINITY ? sum : sum * expf((top - next) * scale)) + (t == -INFINITY ? s : s * expf((t - next) * scale));
-        top = next;
-    };
-    if (row < rows)
-        for (int i = y; i < parts; i += 32) {
-            const float2 s = sums[(long long)i * rows + row];
-            join(s.x, s.y);
-        }
-    tops[y][x] = top, all[y][x] = sum;
-    __syncthreads();
-    // a warp joins one row's 32
-    const long long mine = (long long)blockIdx.x * 32 + y;
-    top = tops[x][y], sum = all[x][y];
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        const float t = __shfl_xor_sync(~0u, top, o), s = __shfl_xor_sync(~0u, sum, o);
-        join(t, s);
-    }
-    if (x || mine >= rows) return;
-    const float log_sum = logf(sum);
-    normalisers[mine] = fmaf(top, scale, log_sum);
-    if (losses) {
-        const int label = labels[mine];
-        losses[mine] = label == -1 ? 0.f : label == -2 ? __int_as_float(0x7fffffff) : fmaf(top - label_logit[mine], scale, log_sum);
-    }
+    JoinSums s;
+    long long row;
+    if (!join_parts<JoinSums, kRows>(sums, nullptr, rows, parts, scale, s, row)) return;
+    const float log_sum = logf(s.sum);
+    normalisers[row] = fmaf(s.top, scale, log_sum);
+    const int label = labels[row];
+    losses[row] = label == -1 ? 0.f : label == -2 ? __int_as_float(0x7fffffff) : fmaf(s.top - label_logit[row], scale, log_sum);
 }
 
+template <int kRows>
 __global__ void __launch_bounds__(1024) softmax_best_kernel(const float2 *sums, const int *best, long long rows, int parts, float scale, long long *labels, float *log_probabilities)
 {
-    __shared__ float tops[32][33], all[32][33];
-    __shared__ int indices[32][33];
-    const int x = threadIdx.x & 31, y = threadIdx.x / 32;
-    const long long row = (long long)blockIdx.x * 32 + x;
-    float top = -INFINITY, rest = 0.f;
-    int index = 0x7fffffff;
-    const auto join = [&](float t, float r, int i) {
-        if (t == -INFINITY) { rest += r; return; }
-        if (top == -INFINITY) { top = t, rest += r, index = i; return; }
-        const bool other = t > top || (t == top && i < index);
-        const float high = other ? t : top, low = other ? top : t;
-        rest = (other ? r : rest) + (1.f + (other ? rest : r)) * expf((low - high) * scale);
-        top = high, index = other ? i : index;
-    };
-    if (row < rows)
-        for (int i = y; i < parts; i += 32) {
-            const float2 s = sums[(long long)i * rows + row];
-            join(s.x, s.y, best[(long long)i * rows + row]);
-        }
-    tops[y][x] = top, all[y][x] = rest, indices[y][x] = index;
-    __syncthreads();
-    const long long mine = (long long)blockIdx.x * 32 + y;
-    top = tops[x][y], rest = all[x][y], index = indices[x][y];
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-        const float t = __shfl_xor_sync(~0u, top, o), r = __shfl_xor_sync(~0u, rest, o);
-        const int i = __shfl_xor_sync(~0u, index, o);
-        join(t, r, i);
-    }
-    if (x || mine >= rows) return;
-    const float log_probability = top == -INFINITY ? __int_as_float(0x7fffffff) : -log1pf(rest);
-    log_probabilities[mine] = log_probability;
-    labels[mine] = log_probability == log_probability ? index : -1;
+    JoinBest s;
+    long long row;
+    if (!join_parts<JoinBest, kRows>(sums, best, rows, parts, scale, s, row)) return;
+    const float log_probability = s.top == -INFINITY ? __int_as_float(0x7fffffff) : -log1pf(s.rest);
+    log_probabilities[row] = log_probability;
+    labels[row] = log_probability == log_probability ? s.index : -1;
 }
 
-// Adds the slices of a product up, in their order.
+// Adds the splits of dw up, in their order, a thread four columns of a row.
 template <class T>
-__global__ void __launch_bounds__(256) softmax_finish_kernel(const float *partial, int slices, long long rows, int columns, const unsigned *out_scale, T *out, long long stride)
+__global__ void __launch_bounds__(256) softmax_finish_kernel(const float *partial, long long partial_stride, long long split_size, int splits, long long rows, int columns, const unsigned *out_scale, T *out,
+                                                             bool whole)
 {
     const float factor = out_scale ? __uint_as_float(*out_scale) * (1.f / 16384.f) : 1.f;
-    const long long all = rows * columns;
+    const int per_row = (columns + 3) / 4;
+    const long long all = rows * per_row;
+    const bool narrow = all < 1ll << 32;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
-        float sum = 0.f;
-        for (int s = 0; s < slices; s++) sum += partial[s * all + i];
-        out[i / columns * stride + i % columns] = from_float<T>(sum * factor);
+        const long long r = narrow ? (long long)((unsigned)i / (unsigned)per_row) : i / per_row;
+        const int c = (int)(i - r * per_row) * 4;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (int s = 0; s < splits; s++) {
+            const float4 v = *(const float4 *)(partial + s * split_size + r * partial_stride + c);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        Pack<T, 4> q;
+        q.v[0] = from_float<T>(sum.x * factor), q.v[1] = from_float<T>(sum.y * factor), q.v[2] = from_float<T>(sum.z * factor), q.v[3] = from_float<T>(sum.w * factor);
+        T *to = out + r * columns + c;
+        if (whole) *(Pack<T, 4> *)to = q;
+        else
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (c + k < columns) to[k] = q.v[k];
     }
+}
+
+// Adds the slices of dx up, in their order, and turns it: the product's rows are the columns of features, its columns the examples.  A block has 32 rows
+// of a tile and 64 of its columns.
+template <class T>
+__global__ void __launch_bounds__(256) softmax_turn_kernel(const float *partial, long long partial_stride, long long slice_size, const Product p, const Schedule schedule, const unsigned *out_scale, T *out)
+{
+    __shared__ float tile[32][65];
+    const int across = p.tile_columns / 64, t = blockIdx.x / (8 * across), strip = blockIdx.x / across % 8, part = blockIdx.x % across;
+    int m, n;
+    p.tile(t, m, n);
+    const long long row0 = m * 256ll + strip * 32, column0 = (long long)n * p.tile_columns + part * 64;
+    if (row0 >= p.rows || column0 >= p.columns) return;
+    const int slices = schedule.slices(p.blocks, t);
+    const float factor = out_scale ? __uint_as_float(*out_scale) * (1.f / 16384.f) : 1.f;
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+        const int r = threadIdx.x / 16 + h, c = threadIdx.x % 16 * 4;
+        if (row0 + r < p.rows && column0 + c < p.columns) {
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float *from = partial + (row0 + r) * partial_stride + column0 + c;
+#pragma unroll 2
+            for (int s = 0; s < slices; s++) {
+                const float4 v = *(const float4 *)(from + s * slice_size);
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+            tile[r][c] = sum.x, tile[r][c + 1] = sum.y, tile[r][c + 2] = sum.z, tile[r][c + 3] = sum.w;
+        }
+    }
+    __syncthreads();
+    const int r = threadIdx.x % 32;
+    if (row0 + r >= p.rows) return;
+    for (int c = threadIdx.x / 32; c < 64 && column0 + c < p.columns; c += 8) out[(column0 + c) * p.rows + row0 + r] = from_float<T>(tile[r][c] * factor);
 }
 
 // -------------------------------------------------------------------------------------------------------- host side
@@ -476,46 +872,53 @@ int encode_tiled(EncodeTiled *out)
     return GTM_OK;
 }
 
-// A matrix as the kernels read it: rows at 16-byte boundaries, one part or three.
+// A matrix as the kernels read or write it: rows at 16-byte boundaries, in one part or several.
 struct Matrix {
     const void *data;
     int64_t rows, columns, stride, part;         // elements
     int parts;
-    bool fp16;
+    int type;
 };
 
 int make_map(CUtensorMap *map, const Matrix &a, unsigned box_columns, unsigned box_rows)
 {
     EncodeTiled encode;
     GTM_TRY(encode_tiled(&encode));
+    const cuuint64_t size = type_bytes(a.type);
     const cuuint64_t sizes[3] = {(cuuint64_t)a.columns, (cuuint64_t)a.rows, (cuuint64_t)a.parts};
-    const cuuint64_t strides[2] = {(cuuint64_t)a.stride * 2, (cuuint64_t)(a.parts > 1 ? a.part : a.stride * a.rows) * 2};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.stride * size, (cuuint64_t)(a.parts > 1 ? a.part : a.stride * a.rows) * size};
     const cuuint32_t box[3] = {box_columns, box_rows, 1}, steps[3] = {1, 1, 1};
-    const CUresult r = encode(map, a.fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void *)a.data, sizes, strides, box, steps,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUtensorMapDataType kind = a.type == GTM_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : a.type == GTM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUresult r = encode(map, kind, 3, (void *)a.data, sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(GTM_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %lld x %lld elements, stride %lld", (int)r, (long long)a.rows, (long long)a.columns, (long long)a.stride);
     return GTM_OK;
 }
 
 __device__ int softmax_error;                    // set by a wait that ran out
 
-template <int kMode>
-int launch_product(Problem p, const Matrix &a, const Matrix &b, cudaStream_t stream)
+int set_operands(Maps &maps, Product &p, int which, const Matrix &a, const Matrix &b, const Matrix *out)
 {
-    CUtensorMap map_a, map_b;
-    GTM_TRY(make_map(&map_a, a, 64, p.a_rows ? 64 : 128));
-    GTM_TRY(make_map(&map_b, b, 64, p.b_rows ? 64 : p.tile_columns / 2));
-    p.what = product(a.fp16 ? 0 : 1, p.tile_columns, p.a_rows, p.b_rows);
+    GTM_TRY(make_map(&maps.a[which], a, 64, p.a_rows ? 64 : 128));
+    GTM_TRY(make_map(&maps.b[which], b, 64, p.tile_columns / 2));
+    if (out) GTM_TRY(make_map(&maps.out[which], *out, out->type == GTM_F32 ? 32 : 64, 32));
+    p.what = product(a.type == GTM_F16 ? 0 : 1, p.tile_columns, p.a_rows);
+    return GTM_OK;
+}
+
+template <int kMode>
+int launch_product(const Maps &maps, Launch &l, cudaStream_t stream)
+{
     void *error = nullptr;
     GTM_CU(cudaGetSymbolAddress(&error, softmax_error));
-    p.error = (int *)error;
-    GTM_CU(cudaFuncSetAttribute(softmax_product_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared));
-    int device = 0, sms = 0;
-    GTM_CU(cudaGetDevice(&device));
-    GTM_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-    const int tiles = p.m_tiles * p.n_tiles * p.splits;
-    softmax_product_kernel<kMode><<<2 * std::min(tiles, sms / 2), kThreads, kShared, stream>>>(map_a, map_b, p);
-    GTM_CU(cudaGetLastError());
+    l.error = (int *)error;
+    GTM_CU(cudaFuncSetAttribute(softmax_product_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared_of(kMode)));
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(2 * (l.schedule.units ? l.schedule.pairs : std::min(l.schedule.items, l.schedule.pairs))), config.blockDim = dim3(kThreads), config.dynamicSmemBytes = shared_of(kMode), config.stream = stream;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization, attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute, config.numAttrs = 1;
+    GTM_CU(cudaLaunchKernelEx(&config, softmax_product_kernel<kMode>, maps, l));
     return GTM_OK;
 }
 
@@ -525,30 +928,42 @@ int tile_columns(int64_t rows, int64_t columns)
     return columns <= 128 || (rows + 255) / 256 * ((columns + 255) / 256) < kPairs ? 128 : 256;
 }
 
-struct Shape {
-    int m_tiles, n_tiles, tile, splits, per_split, depth_blocks;
-};
-
-// Tiles of a product; where they are fewer than the pairs of SMs, the sum's index is split, into eight blocks or more.
-Shape shape_of(int64_t rows, int64_t columns, int64_t depth, int products, bool split)
+Product product_of(int64_t rows, int64_t columns, int64_t depth, int products)
 {
-    Shape s;
-    s.tile = tile_columns(rows, columns);
-    s.m_tiles = (int)((rows + 255) / 256), s.n_tiles = (int)((columns + s.tile - 1) / s.tile);
-    s.depth_blocks = (int)((depth + kDepth - 1) / kDepth);
-    const int blocks = s.depth_blocks * products, tiles = s.m_tiles * s.n_tiles;
-    s.splits = split ? std::max(1, std::min(kPairs / tiles, blocks / 8)) : 1;
-    s.per_split = (blocks + s.splits - 1) / s.splits;
-    s.splits = (blocks + s.per_split - 1) / s.per_split;
+    Product p = {};
+    p.rows = rows, p.columns = columns, p.products = products;
+    p.tile_columns = tile_columns(rows, columns);
+    p.m_tiles = (int)((rows + 255) / 256), p.n_tiles = (int)((columns + p.tile_columns - 1) / p.tile_columns);
+    p.depth_blocks = (int)((depth + kDepth - 1) / kDepth);
+    p.blocks = p.per_split = p.depth_blocks * products;
+    return p;
+}
+
+// One product alone, its tiles in turn.
+Schedule in_turn(const Product &p) { return {p.tiles() * p.splits(), kPairs, 0, kPairs, 0, 0}; }
+
+// Two products; weights are columns times blocks, an epilogue being worth about six blocks.  No pair has less than eight blocks of the second product
+// (or one pair has them all): slices cost, and a pair without work would leave one unwritten.
+constexpr int kLeastShare = 8;
+Schedule together(const Product &first, const Product &second)
+{
+    Schedule s = {first.tiles() * first.splits(), kPairs, 0, kPairs, (long long)second.tiles() * second.blocks, 0};
+    const double item = (first.per_split + 6.0) * first.tile_columns, unit = second.tile_columns;
+    s.longer = s.items % kPairs;
+    if (s.longer) {
+        const double each = (s.units * unit - (kPairs - s.longer) * item) / kPairs;     // what is left for a longer pair
+        if (each > (kLeastShare + 1) * unit) s.units_of_longer = std::min(s.units, (long long)(each * s.longer / unit));
+    }
+    s.others = (int)std::max<long long>(1, std::min<long long>(kPairs - s.longer, (s.units - s.units_of_longer) / kLeastShare));
     return s;
 }
 
-Problem problem_of(const Shape &s, int64_t rows, int64_t columns, int products)
+int most_slices(const Schedule &s, const Product &p)
 {
-    Problem p = {};
-    p.rows = rows, p.columns = columns, p.m_tiles = s.m_tiles, p.n_tiles = s.n_tiles, p.splits = s.splits, p.tile_columns = s.tile;
-    p.depth_blocks = s.depth_blocks, p.per_split = s.per_split, p.products = products;
-    return p;
+    if (p.tiles() > 1024) return std::min(kPairs, p.blocks / kLeastShare + 2);          // a bound
+    int most = 1;
+    for (int t = 0; t < p.tiles(); t++) most = std::max(most, s.slices(p.blocks, t));
+    return most;
 }
 
 // What a call reads, and where its workspace's parts are.
@@ -560,13 +975,16 @@ struct Call {
     bool lay_out_x, lay_out_w, gradient;
     int64_t x_ld, w_ld;
     // forward
+    bool few, few_whole;
     int64_t piece_rows;
     int stat_parts;
     // gradient
-    int64_t piece_labels, prob_ld;
-    Shape dx, dw;
-    bool dx_partial, dw_partial;
-    uint64_t at_x, at_w, at_rows, at_factors, at_largest, at_sums, at_best, at_logit, at_prob, at_dx, at_dw, total;
+    int64_t piece_labels, prob_ld, sums_ld, turned_ld;
+    Product dx, dw;
+    Schedule schedule;
+    int dx_slices;
+    bool dw_direct;
+    uint64_t at_x, at_turned, at_w, at_rows, at_factors, at_largest, at_sums, at_best, at_logit, at_prob, at_dx, at_dw, total;
 };
 
 bool direct(int type, const void *p, int64_t rows, int64_t stride, int64_t columns)
@@ -576,13 +994,35 @@ bool direct(int type, const void *p, int64_t rows, int64_t stride, int64_t colum
 
 int64_t clamp64(int64_t v, int64_t low, int64_t high) { return v < low ? low : v > high ? high : v; }
 
+// A piece of the labels: P of it within kPieceBytes, and as few rounds of tiles over all pieces as that allows.
+int64_t piece_of(int64_t examples, int64_t labels, int parts)
+{
+    const int64_t m_tiles = (examples + 255) / 256, all = (labels + 255) / 256;
+    const int64_t most = std::min(all, clamp64(kPieceBytes / (examples * 2 * parts) / 256, 1, 4096));
+    if (most == all) return labels;
+    int64_t best = most, least = -1;
+    for (int64_t tiles = most; tiles >= std::max<int64_t>(1, most / 2); tiles--) {
+        const int64_t rounds = (all + tiles - 1) / tiles * ((m_tiles * tiles + kPairs - 1) / kPairs);
+        if (least < 0 || rounds < least) least = rounds, best = tiles;
+    }
+    return best * 256;
+}
+
+constexpr int kFewBlocks = 148 * 4;
+constexpr size_t kFewShared = 96 << 10;
+
 void lay_out_workspace(Call &c)
 {
     c.products = c.type == GTM_F32 ? kPartProducts : 1;
     c.parts = c.type == GTM_F32 ? 3 : 1;
+    const int64_t size = (int64_t)type_bytes(c.type);
+    // as many examples as are multiplied by the plain units while memory delivers the weights: 8 in 32 bits, 4 in 16
+    const int64_t padded = (int64_t)round_up(c.columns, 256);
+    c.few = !c.gradient && c.examples <= (c.type == GTM_F32 ? 8 : 4) && (c.examples <= 4 ? 4 : 8) * padded * 4 <= (int64_t)kFewShared;
+    c.few_whole = aligned(c.w, c.w_stride * size, 16) && c.columns * size % 16 == 0;
     // the gradient's x is laid out anew in any case: examples that are ignored may hold anything
-    c.lay_out_x = c.gradient || !direct(c.type, c.x, c.examples, c.x_stride, c.columns);
-    c.lay_out_w = !direct(c.type, c.w, c.labels, c.w_stride, c.columns);
+    c.lay_out_x = !c.few && (c.gradient || !direct(c.type, c.x, c.examples, c.x_stride, c.columns));
+    c.lay_out_w = !c.few && !direct(c.type, c.w, c.labels, c.w_stride, c.columns);
     const int64_t ld = (int64_t)round_up(c.columns, 8);
     c.x_ld = c.lay_out_x || c.examples == 1 ? ld : c.x_stride;
     c.w_ld = c.lay_out_w || c.labels == 1 ? ld : c.w_stride;
@@ -593,7 +1033,7 @@ void lay_out_workspace(Call &c)
     c.at_rows = take(c.examples * 4);
     if (!c.gradient) {
         const int tile = tile_columns(c.examples, c.labels);
-        c.stat_parts = (int)((c.labels + tile - 1) / tile) * 2;
+        c.stat_parts = c.few ? kFewBlocks : (int)((c.labels + tile - 1) / tile) * 2;
         c.piece_rows = std::min<int64_t>(c.examples, clamp64(kStatBytes / (c.stat_parts * 8) / 256 * 256, 256, (int64_t)1 << 30));
         c.at_sums = take((uint64_t)c.stat_parts * c.piece_rows * 8);
         c.at_best = take((uint64_t)c.stat_parts * c.piece_rows * 4);
@@ -601,17 +1041,22 @@ void lay_out_workspace(Call &c)
     } else {
         c.at_factors = take(c.examples * 4);
         c.at_largest = take(4);
-        const int64_t most = clamp64(kPieceBytes / (c.examples * 2 * c.parts) / 256 * 256, 256, (int64_t)1 << 30);
-        const int64_t pieces = (c.labels + most - 1) / most;
-        c.piece_labels = pieces == 1 ? c.labels : (int64_t)round_up((c.labels + pieces - 1) / pieces, 256);
+        c.piece_labels = piece_of(c.examples, c.labels, c.parts);
         c.prob_ld = (int64_t)round_up(c.piece_labels, 64);
+        c.sums_ld = (int64_t)round_up(c.columns, 4);
+        c.turned_ld = (int64_t)round_up(c.examples, 8);
+        c.at_turned = take((uint64_t)c.parts * c.columns * c.turned_ld * 2);
         c.at_prob = take((uint64_t)c.parts * c.examples * c.prob_ld * 2);
-        c.dx = shape_of(c.examples, c.columns, c.piece_labels, c.products, true);
-        c.dw = shape_of(c.piece_labels, c.columns, c.examples, c.products, true);
-        c.dx_partial = c.dx.splits > 1 || pieces > 1;
-        c.dw_partial = c.dw.splits > 1;
-        c.at_dx = take(c.dx_partial ? (uint64_t)c.dx.splits * c.examples * c.columns * 4 : 0);
-        c.at_dw = take(c.dw_partial ? (uint64_t)c.dw.splits * c.piece_labels * c.columns * 4 : 0);
+        c.dx = product_of(c.columns, c.examples, c.piece_labels, c.products);          // turned: its operand B is P
+        c.dw = product_of(c.piece_labels, c.columns, c.examples, c.products);
+        // dw's tiles are cut where they are less than half of the pairs of SMs, into eight blocks or more
+        const int splits = std::max(1, std::min(kPairs / c.dw.tiles(), c.dw.blocks / 8));
+        c.dw.per_split = (c.dw.blocks + splits - 1) / splits;
+        c.schedule = together(c.dw, c.dx);
+        c.dx_slices = most_slices(c.schedule, c.dx);
+        c.dw_direct = c.dw.splits() == 1 && c.columns * size % 16 == 0;
+        c.at_dx = take((uint64_t)c.dx_slices * c.columns * c.turned_ld * 4);
+        c.at_dw = take(c.dw_direct ? 0 : (uint64_t)c.dw.splits() * c.piece_labels * c.sums_ld * 4);
     }
     c.total = at;
 }
@@ -637,8 +1082,10 @@ int check_workspace(const char *what, const void *workspace, uint64_t bytes, uin
 template <class T>
 void lay_out(const void *from, int64_t stride, int64_t rows, int64_t columns, const int *labels, void *to, int64_t ld, cudaStream_t stream)
 {
-    const int64_t blocks = std::min<int64_t>((rows * columns + 255) / 256, 148 * 16);
-    softmax_lay_out_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>((const T *)from, stride, rows, (int)columns, labels, to, ld, rows * ld);
+    const int64_t blocks = std::min<int64_t>((rows * ((columns + 7) / 8) + 255) / 256, 148 * 16);
+    const bool whole = aligned(from, stride * sizeof(T), 16) && columns % 8 == 0;
+    if (whole) softmax_lay_out_kernel<T, true><<<(unsigned)blocks, 256, 0, stream>>>((const T *)from, stride, rows, (int)columns, labels, (__nv_bfloat16 *)to, ld, rows * ld);
+    else softmax_lay_out_kernel<T, false><<<(unsigned)blocks, 256, 0, stream>>>((const T *)from, stride, rows, (int)columns, labels, (__nv_bfloat16 *)to, ld, rows * ld);
 }
 
 // A matrix as the kernels read it, laid out in the workspace where it is not so already.
@@ -651,30 +1098,99 @@ int operand_of(Matrix *out, int type, const void *data, int64_t stride, int64_t 
         GTM_CU(cudaGetLastError());
         data = to;
     }
-    *out = {data, rows, columns, ld, rows * ld, type == GTM_F32 ? 3 : 1, type == GTM_F16};
+    *out = {data, rows, columns, ld, rows * ld, type == GTM_F32 ? 3 : 1, type == GTM_F16 ? GTM_F16 : GTM_BF16};
     return GTM_OK;
 }
 
-int finish(int type, const float *partial, int slices, int64_t rows, int64_t columns, const unsigned *out_scale, void *out, int64_t stride, cudaStream_t stream)
+template <class T>
+int lay_out_both(const Call &c, const int *labels, char *w, cudaStream_t stream)
 {
-    const unsigned blocks = (unsigned)std::min<int64_t>((rows * columns + 255) / 256, 148 * 16);
-    if (type == GTM_F32) softmax_finish_kernel<float><<<blocks, 256, 0, stream>>>(partial, slices, rows, (int)columns, out_scale, (float *)out, stride);
-    else if (type == GTM_BF16) softmax_finish_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(partial, slices, rows, (int)columns, out_scale, (__nv_bfloat16 *)out, stride);
-    else softmax_finish_kernel<__half><<<blocks, 256, 0, stream>>>(partial, slices, rows, (int)columns, out_scale, (__half *)out, stride);
+    const dim3 grid((unsigned)((c.examples + 63) / 64), (unsigned)((c.columns + 63) / 64));
+    const bool whole = aligned(c.x, c.x_stride * sizeof(T), 16) && c.columns % 8 == 0;
+    softmax_lay_out_both_kernel<T><<<grid, 256, 0, stream>>>((const T *)c.x, c.x_stride, c.examples, (int)c.columns, labels, (__nv_bfloat16 *)(w + c.at_x), c.x_ld, c.examples * c.x_ld,
+                                                             (__nv_bfloat16 *)(w + c.at_turned), c.turned_ld, c.columns * c.turned_ld, whole);
+    GTM_CU(cudaGetLastError());
+    return GTM_OK;
+}
+
+template <class T>
+int finish_dw(const Call &c, const float *dw, int64_t rows, const unsigned *out_scale, void *out, cudaStream_t stream)
+{
+    const unsigned blocks = (unsigned)std::min<int64_t>((rows * ((c.columns + 3) / 4) + 255) / 256, 148 * 16);
+    softmax_finish_kernel<T><<<blocks, 256, 0, stream>>>(dw, c.sums_ld, c.piece_labels * c.sums_ld, c.dw.splits(), rows, (int)c.columns, out_scale, (T *)out, c.columns % 4 == 0);
+    GTM_CU(cudaGetLastError());
+    return GTM_OK;
+}
+
+template <class T>
+int finish_dx(const Call &c, const float *dx, const unsigned *out_scale, void *out, cudaStream_t stream)
+{
+    softmax_turn_kernel<T><<<(unsigned)(c.dx.tiles() * 8 * (c.dx.tile_columns / 64)), 256, 0, stream>>>(dx, c.turned_ld, c.columns * c.turned_ld, c.dx, c.schedule, out_scale, (T *)out);
+    GTM_CU(cudaGetLastError());
+    return GTM_OK;
+}
+
+template <class T, int kExamples, bool kWhole>
+int launch_few(const FewArgs &a, int blocks, cudaStream_t stream)
+{
+    const size_t shared = kExamples * round_up(a.columns, 256) * 4;
+    const auto run = [&](auto kernel) -> int {
+        GTM_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewShared));
+        kernel<<<blocks, kFewThreads, shared, stream>>>(a);
+        GTM_CU(cudaGetLastError());
+        return GTM_OK;
+    };
+    return a.best ? run(softmax_few_kernel<T, kExamples, kWhole, true>) : run(softmax_few_kernel<T, kExamples, kWhole, false>);
+}
+
+template <class T>
+int launch_few(const FewArgs &a, bool whole, int blocks, cudaStream_t stream)
+{
+    if (a.examples == 1) return whole ? launch_few<T, 1, true>(a, blocks, stream) : launch_few<T, 1, false>(a, blocks, stream);
+    if (a.examples == 2) return whole ? launch_few<T, 2, true>(a, blocks, stream) : launch_few<T, 2, false>(a, blocks, stream);
+    if (a.examples <= 4) return whole ? launch_few<T, 4, true>(a, blocks, stream) : launch_few<T, 4, false>(a, blocks, stream);
+    if constexpr (sizeof(T) == 4) return whole ? launch_few<T, 8, true>(a, blocks, stream) : launch_few<T, 8, false>(a, blocks, stream);
+    return fail(GTM_ERR_ARG, "more examples than are few");
+}
+
+// Rows per block of the kernels that join parts: as few as there are.
+template <class Run>
+int by_rows(int64_t rows, Run run)
+{
+    if (rows <= 8) run(std::integral_constant<int, 1>(), (unsigned)rows);
+    else if (rows <= 148 * 8) run(std::integral_constant<int, 8>(), (unsigned)((rows + 7) / 8));
+    else run(std::integral_constant<int, 32>(), (unsigned)((rows + 31) / 32));
     GTM_CU(cudaGetLastError());
     return GTM_OK;
 }
 
 // Loss (labels given) or most probable label.
-int forward(const char *what, Call &c, const void *labels, int labels_64, int64_t ignored, float scale, float *losses, float *normalisers, int64_t *best, float *log_probabilities,
-            char *w, cudaStream_t stream)
+int forward(Call &c, const void *labels, int labels_64, int64_t ignored, float scale, float *losses, float *normalisers, int64_t *best, float *log_probabilities, char *w, cudaStream_t stream)
 {
-    Matrix x, weights;
     int *rows = labels ? (int *)(w + c.at_rows) : nullptr;
     if (labels) {
         softmax_rows_kernel<<<(unsigned)((c.examples + 255) / 256), 256, 0, stream>>>(labels, labels_64, c.examples, c.labels, ignored, nullptr, 0, scale, rows, nullptr, nullptr);
         GTM_CU(cudaGetLastError());
     }
+    float2 *sums = (float2 *)(w + c.at_sums);
+    int *indices = (int *)(w + c.at_best);
+    float *label_logit = (float *)(w + c.at_logit);
+    const auto join = [&](int64_t first, int64_t n, int parts) {
+        return by_rows(n, [&](auto each, unsigned blocks) {
+            constexpr int kRows = decltype(each)::value;
+            if (labels) softmax_loss_kernel<kRows><<<blocks, 1024, 0, stream>>>(sums, label_logit, rows + first, n, parts, scale, losses + first, normalisers + first);
+            else softmax_best_kernel<kRows><<<blocks, 1024, 0, stream>>>(sums, indices, n, parts, scale, (long long *)best + first, log_probabilities + first);
+        });
+    };
+    if (c.few) {
+        const FewArgs a = {c.x, c.w, c.x_stride, c.w_stride, (int)c.examples, (int)c.labels, (int)c.columns, scale, rows, sums, labels ? nullptr : indices, label_logit};
+        const int blocks = (int)std::min<int64_t>(kFewBlocks, (c.labels + kFewRows * kFewThreads / 32 - 1) / (kFewRows * kFewThreads / 32));
+        GTM_TRY(c.type == GTM_F32    ? launch_few<float>(a, c.few_whole, blocks, stream)
+                : c.type == GTM_BF16 ? launch_few<__nv_bfloat16>(a, c.few_whole, blocks, stream)
+                                     : launch_few<__half>(a, c.few_whole, blocks, stream));
+        return join(0, c.examples, blocks);
+    }
+    Matrix x, weights;
     GTM_TRY(operand_of(&x, c.type, c.x, c.x_stride, c.examples, c.columns, c.lay_out_x, nullptr, w + c.at_x, c.x_ld, stream));
     GTM_TRY(operand_of(&weights, c.type, c.w, c.w_stride, c.labels, c.columns, c.lay_out_w, nullptr, w + c.at_w, c.w_ld, stream));
     for (int64_t r = 0; r < c.examples; r += c.piece_rows) {
@@ -682,21 +1198,18 @@ int forward(const char *what, Call &c, const void *labels, int labels_64, int64_
         Matrix piece = x;
         piece.data = (const char *)x.data + r * x.stride * 2;
         piece.rows = n;
-        Shape s = shape_of(n, c.labels, c.columns, c.products, false);
-        s.tile = tile_columns(c.examples, c.labels);         // as the workspace has it
-        s.n_tiles = (int)((c.labels + s.tile - 1) / s.tile);
-        Problem p = problem_of(s, n, c.labels, c.products);
-        p.m_fast = 1, p.scale = scale, p.sums = (float2 *)(w + c.at_sums), p.best = (int *)(w + c.at_best), p.label_logit = (float *)(w + c.at_logit);
-        p.labels = labels ? rows + r : nullptr;
-        const unsigned blocks = (unsigned)((n + 31) / 32);
-        if (labels) {
-            GTM_TRY(launch_product<kSums>(p, piece, weights, stream));
-            softmax_loss_kernel<<<blocks, 1024, 0, stream>>>(p.sums, p.label_logit, rows + r, n, s.n_tiles * 2, scale, losses + r, normalisers + r);
-        } else {
-            GTM_TRY(launch_product<kBest>(p, piece, weights, stream));
-            softmax_best_kernel<<<blocks, 1024, 0, stream>>>(p.sums, p.best, n, s.n_tiles * 2, scale, (long long *)best + r, log_probabilities + r);
-        }
-        GTM_CU(cudaGetLastError());
+        Launch l = {};
+        Maps maps = {};
+        Product &p = l.p[0] = product_of(n, c.labels, c.columns, c.products);
+        p.tile_columns = tile_columns(c.examples, c.labels);         // as the workspace has it
+        p.n_tiles = (int)((c.labels + p.tile_columns - 1) / p.tile_columns);
+        p.m_fast = 1;
+        l.schedule = in_turn(p);
+        l.scale = scale, l.sums = sums, l.best = indices, l.label_logit = label_logit, l.labels = labels ? rows + r : nullptr;
+        GTM_TRY(set_operands(maps, p, 0, piece, weights, nullptr));
+        if (labels) GTM_TRY(launch_product<kSums>(maps, l, stream));
+        else GTM_TRY(launch_product<kBest>(maps, l, stream));
+        GTM_TRY(join(r, n, p.n_tiles * 2));
     }
     return GTM_OK;
 }
@@ -738,7 +1251,7 @@ extern "C" int gtm_softmax_loss(int device, void *cuda_stream, int type, const v
     GTM_TRY(check_workspace("gtm_softmax_loss", workspace, workspace_bytes, c.total));
     DeviceGuard guard(device);
     GTM_TRY(guard.status);
-    return forward("gtm_softmax_loss", c, labels, labels_64, ignore_label, scale, losses, normalisers, nullptr, nullptr, (char *)workspace, (cudaStream_t)cuda_stream);
+    return forward(c, labels, labels_64, ignore_label, scale, losses, normalisers, nullptr, nullptr, (char *)workspace, (cudaStream_t)cuda_stream);
 }
 
 extern "C" int gtm_softmax_predict(int device, void *cuda_stream, int type, const void *features, int64_t examples, int64_t features_stride, const void *weights, int64_t number_of_labels,
@@ -752,24 +1265,24 @@ extern "C" int gtm_softmax_predict(int device, void *cuda_stream, int type, cons
     GTM_TRY(check_workspace("gtm_softmax_predict", workspace, workspace_bytes, c.total));
     DeviceGuard guard(device);
     GTM_TRY(guard.status);
-    return forward("gtm_softmax_predict", c, nullptr, 0, 0, scale, nullptr, nullptr, labels_out, log_probabilities_out, (char *)workspace, (cudaStream_t)cuda_stream);
+    return forward(c, nullptr, 0, 0, scale, nullptr, nullptr, labels_out, log_probabilities_out, (char *)workspace, (cudaStream_t)cuda_stream);
 }
 
 extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type, const void *features, int64_t examples, int64_t features_stride, const void *weights,
                                          int64_t number_of_labels, int64_t weights_stride, int64_t columns, const void *labels, int labels_64, int64_t ignore_label, float scale,
-                                         const float *normalisers, const float *gradients, int64_t gradients_step, void *features_gradient, int64_t features_gradient_stride,
-                                         void *weights_gradient, int64_t weights_gradient_stride, void *workspace, uint64_t workspace_bytes)
+                                         const float *normalisers, const float *gradients, int64_t gradients_step, void *features_gradient, void *weights_gradient, void *workspace,
+                                         uint64_t workspace_bytes)
 {
     Call c = call_of(type, examples, number_of_labels, columns, features, features_stride, weights, weights_stride, true);
     GTM_TRY(check_call("gtm_softmax_loss_gradient", c, scale));
-    if (!weights_gradient || weights_gradient_stride < columns || (examples && features_gradient_stride < columns))
-        return fail(GTM_ERR_ARG, "gtm_softmax_loss_gradient: null result or a row stride below its columns");
+    if (!weights_gradient || (uintptr_t)weights_gradient % 16 || (uintptr_t)features_gradient % 16)
+        return fail(GTM_ERR_ARG, "gtm_softmax_loss_gradient: a result is null or does not start at a 16-byte boundary");
     if (gradients_step != 0 && gradients_step != 1) return fail(GTM_ERR_ARG, "gtm_softmax_loss_gradient: step %lld of the gradients (0 or 1)", (long long)gradients_step);
     cudaStream_t stream = (cudaStream_t)cuda_stream;
     DeviceGuard guard(device);
     GTM_TRY(guard.status);
     if (examples == 0) {
-        GTM_CU(cudaMemset2DAsync(weights_gradient, weights_gradient_stride * type_bytes(type), 0, columns * type_bytes(type), number_of_labels, stream));
+        GTM_CU(cudaMemsetAsync(weights_gradient, 0, (size_t)number_of_labels * columns * type_bytes(type), stream));
         return GTM_OK;
     }
     if (!features || !weights || !labels || !normalisers || !gradients || !features_gradient) return fail(GTM_ERR_ARG, "gtm_softmax_loss_gradient: null array");
@@ -782,37 +1295,49 @@ extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type
     if (largest) GTM_CU(cudaMemsetAsync(largest, 0, 4, stream));
     softmax_rows_kernel<<<(unsigned)((examples + 255) / 256), 256, 0, stream>>>(labels, labels_64, examples, number_of_labels, ignore_label, gradients, (int)gradients_step, scale, rows, factors, largest);
     GTM_CU(cudaGetLastError());
-    Matrix x, wm;
-    GTM_TRY(operand_of(&x, type, features, features_stride, examples, columns, true, rows, w + c.at_x, c.x_ld, stream));
+    GTM_TRY(type == GTM_F32 ? lay_out_both<float>(c, rows, w, stream) : type == GTM_BF16 ? lay_out_both<__nv_bfloat16>(c, rows, w, stream) : lay_out_both<__half>(c, rows, w, stream));
+    const int held = type == GTM_F16 ? GTM_F16 : GTM_BF16;
+    const Matrix x = {w + c.at_x, examples, columns, c.x_ld, examples * c.x_ld, c.parts, held}, turned = {w + c.at_turned, columns, examples, c.turned_ld, columns * c.turned_ld, c.parts, held};
+    Matrix wm;
     GTM_TRY(operand_of(&wm, type, weights, weights_stride, number_of_labels, columns, c.lay_out_w, nullptr, w + c.at_w, c.w_ld, stream));
-    float *dx = c.dx_partial ? (float *)(w + c.at_dx) : nullptr, *dw = c.dw_partial ? (float *)(w + c.at_dw) : nullptr;
+    float *dx = (float *)(w + c.at_dx), *dw = (float *)(w + c.at_dw);
+    const int64_t size = (int64_t)type_bytes(type);
     for (int64_t v = 0; v < number_of_labels; v += c.piece_labels) {
         const int64_t n = std::min(c.piece_labels, number_of_labels - v);
-        const Matrix prob = {w + c.at_prob, examples, n, c.prob_ld, examples * c.prob_ld, c.parts, type == GTM_F16};
-        // P of the piece
+        const Matrix prob = {w + c.at_prob, examples, n, c.prob_ld, examples * c.prob_ld, c.parts, held};
         Matrix piece = wm;                        // rows behind the piece read as zeros
         piece.rows = v + n;
-        Problem p = problem_of(shape_of(examples, n, columns, c.products, false), examples, n, c.products);
-        p.m_fast = 1, p.b_row = (int)v, p.scale = scale, p.labels = rows, p.first_label = (int)v;
-        p.normalisers = normalisers, p.factors = factors, p.largest = largest, p.type = type;
-        p.prob = (void *)prob.data, p.prob_stride = c.prob_ld, p.prob_part = prob.part;
-        GTM_TRY(launch_product<kProb>(p, x, piece, stream));
-        // dw of the piece: sums over examples
-        Shape s = shape_of(n, columns, examples, c.products, false);
-        s.splits = c.dw.splits, s.per_split = c.dw.per_split;       // as the workspace has them, for a smaller last piece too
-        p = problem_of(s, n, columns, c.products);
-        p.a_rows = p.b_rows = 1, p.type = type, p.out_scale = largest, p.partial = dw;
-        p.out = (char *)weights_gradient + v * weights_gradient_stride * type_bytes(type), p.out_stride = weights_gradient_stride;
-        GTM_TRY(launch_product<kOut>(p, prob, x, stream));
-        if (dw) GTM_TRY(finish(type, dw, p.splits, n, columns, largest, p.out, p.out_stride, stream));
-        // dx: sums over the piece's labels
-        p = problem_of(c.dx, examples, columns, c.products);
-        p.b_rows = 1, p.b_first = (int)v, p.type = type, p.out_scale = largest, p.partial = dx, p.add = v > 0;
-        p.out = features_gradient, p.out_stride = features_gradient_stride;
-        GTM_TRY(launch_product<kOut>(p, prob, piece, stream));
+        // P of the piece
+        {
+            Launch l = {};
+            Maps maps = {};
+            Product &p = l.p[0] = product_of(examples, n, columns, c.products);
+            p.m_fast = 1, p.b_row = (int)v, p.type = type;
+            l.schedule = in_turn(p);
+            l.scale = scale, l.labels = rows, l.first_label = (int)v, l.normalisers = normalisers, l.factors = factors, l.largest = largest;
+            GTM_TRY(set_operands(maps, p, 0, x, piece, &prob));
+            GTM_TRY(launch_product<kProb>(maps, l, stream));
+        }
+        // dw of the piece, P turned times x, and its share of dx turned, w turned times P.  A last piece that is smaller has the work of a whole one, zeros
+        // among it, so that the slices of dx are the same
+        Launch l = {};
+        Maps maps = {};
+        l.schedule = c.schedule;
+        Product &pw = l.p[0] = c.dw, &px = l.p[1] = c.dx;
+        char *to = (char *)weights_gradient + v * columns * size;
+        pw.a_rows = 1, pw.rows = n, pw.type = c.dw_direct ? type : GTM_F32, pw.out_scale = c.dw_direct ? largest : nullptr;
+        px.a_rows = 1, px.a_first = (int)v, px.type = GTM_F32, px.add = v > 0;
+        const Matrix dw_out = c.dw_direct ? Matrix{to, n, columns, columns, 0, 1, type} : Matrix{dw, n, columns, c.sums_ld, c.piece_labels * c.sums_ld, pw.splits(), GTM_F32};
+        const Matrix dx_out = {dx, columns, examples, c.turned_ld, columns * c.turned_ld, c.dx_slices, GTM_F32};
+        GTM_TRY(set_operands(maps, pw, 0, prob, turned, &dw_out));
+        GTM_TRY(set_operands(maps, px, 1, piece, prob, &dx_out));
+        GTM_TRY(launch_product<kOut>(maps, l, stream));
+        if (!c.dw_direct)
+            GTM_TRY(type == GTM_F32 ? finish_dw<float>(c, dw, n, largest, to, stream) : type == GTM_BF16 ? finish_dw<__nv_bfloat16>(c, dw, n, largest, to, stream) : finish_dw<__half>(c, dw, n, largest, to, stream));
     }
-    if (dx) GTM_TRY(finish(type, dx, c.dx.splits, examples, columns, largest, features_gradient, features_gradient_stride, stream));
-    return GTM_OK;
+    return type == GTM_F32    ? finish_dx<float>(c, dx, largest, features_gradient, stream)
+           : type == GTM_BF16 ? finish_dx<__nv_bfloat16>(c, dx, largest, features_gradient, stream)
+                              : finish_dx<__half>(c, dx, largest, features_gradient, stream);
 }
 
 extern "C" int gtm_softmax_failed(int device, int *failed_out)

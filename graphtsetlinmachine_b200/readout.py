@@ -141,7 +141,7 @@ def embed_gradient(gradient, ids, rows, offsets=None, scale=1.0):
     _lib.check(lib.gtm_embed_gradient_workspace(ids.numel(), rows, columns, C.byref(need)))
     workspace = _workspace(need.value, device)
     _lib.check(lib.gtm_embed_gradient(device.index, _stream(device), _TYPES[gradient.dtype], gradient.data_ptr(), columns, stride, ids.data_ptr(), wide, ids.numel(),
-                                      None if offsets is None else offsets.data_ptr(), wide_offsets, count, scale, out.data_ptr(), rows, columns,
+                                      None if offsets is None else offsets.data_ptr(), wide_offsets, count, scale, out.data_ptr(), rows,
                                       workspace.data_ptr(), need.value))
     return out
 
@@ -199,9 +199,8 @@ def softmax_loss_gradient(features, weights, labels, normalisers, gradients, sca
         raise ValueError("gradients is not a contiguous float32 tensor of one element, or of one for each of %d examples" % n)
     features_gradient = torch.empty(features.shape, dtype=features.dtype, device=device)
     weights_gradient = torch.empty(weights.shape, dtype=weights.dtype, device=device)
-    columns = features.shape[1]
     _lib.check(lib.gtm_softmax_loss_gradient(*what, labels.data_ptr(), wide, ignore_label, scale, normalisers.data_ptr(), gradients.data_ptr(),
-                                             1 if gradients.numel() == n else 0, features_gradient.data_ptr(), columns, weights_gradient.data_ptr(), columns,
+                                             1 if gradients.numel() == n else 0, features_gradient.data_ptr(), weights_gradient.data_ptr(),
                                              workspace.data_ptr(), size))
     return features_gradient, weights_gradient
 

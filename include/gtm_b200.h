@@ -239,8 +239,8 @@ int gtm_transform_nodewise(gtm_model *model, gtm_dataset *dataset, int number_of
                            int node_stride, int32_t *node_outputs_out, int32_t *class_sums_out);
 
 /* Readout operators.  NO COUNTERPART IN THE REFERENCE, whose `transform` (tm.py:814-851) hands clause outputs to learners of
- * other libraries.  They work on DEVICE arrays without a model: row-major matrices whose rows lie `..._stride` elements apart,
- * element types gtm_type, indices int32 or int64 (`..._64` = 1).  Work is queued on `cuda_stream` of `device` (the caller's
+ * other libraries.  They work on DEVICE arrays without a model: row-major matrices whose rows lie `..._stride` elements apart
+ * (results: one behind the other, from a 16-byte boundary), element types gtm_type, indices int32 or int64 (`..._64` = 1).  Work is queued on `cuda_stream` of `device` (the caller's
  * current device is left as it is) and the call returns without synchronising; nothing is allocated, so that calls can be captured
  * into a CUDA graph.  The caller's workspace (device memory, 256-byte aligned, contents arbitrary) belongs to one call at a time;
  * its size comes from the ..._workspace function for the same arrays and sizes.  Sums are held in 32 bits. */
@@ -258,7 +258,7 @@ int gtm_embed(int device, void *cuda_stream, int type, const void *table, int64_
 int gtm_embed_gradient_workspace(int64_t number_of_ids, int64_t rows, int64_t columns, uint64_t *bytes_out);
 int gtm_embed_gradient(int device, void *cuda_stream, int type, const void *gradient, int64_t columns, int64_t gradient_stride, const void *ids, int ids_64,
                        int64_t number_of_ids, const void *offsets, int offsets_64, int64_t number_of_bags, float scale, void *table_gradient, int64_t rows,
-                       int64_t row_stride, void *workspace, uint64_t workspace_bytes);
+                       void *workspace, uint64_t workspace_bytes);
 
 /* Softmax cross entropy without keeping the logits l[n][v] = scale * features[n] . weights[v], scale > 0: normalisers[n] =
  * log sum_v exp l[n][v], losses[n] = normalisers[n] - l[n][labels[n]].  Examples whose label is ignore_label have loss zero; the
@@ -275,8 +275,7 @@ int gtm_softmax_loss(int device, void *cuda_stream, int type, const void *featur
 int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type, const void *features, int64_t examples, int64_t features_stride, const void *weights,
                               int64_t number_of_labels, int64_t weights_stride, int64_t columns, const void *labels, int labels_64, int64_t ignore_label,
                               float scale, const float *normalisers, const float *gradients, int64_t gradients_step, void *features_gradient,
-                              int64_t features_gradient_stride, void *weights_gradient, int64_t weights_gradient_stride, void *workspace,
-                              uint64_t workspace_bytes);
+                              void *weights_gradient, void *workspace, uint64_t workspace_bytes);
 int gtm_softmax_predict(int device, void *cuda_stream, int type, const void *features, int64_t examples, int64_t features_stride, const void *weights,
                         int64_t number_of_labels, int64_t weights_stride, int64_t columns, float scale, int64_t *labels_out, float *log_probabilities_out,
                         void *workspace, uint64_t workspace_bytes);

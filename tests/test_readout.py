@@ -32,7 +32,7 @@ def _embed(lib, **kw):
 
 def _embed_gradient(lib, **kw):
     a = dict(device=0, stream=None, type=0, gradient=POINTER, columns=8, stride=8, ids=POINTER, wide=1, n=3, offsets=None, wide_offsets=0, bags=0, scale=1.0,
-             out=POINTER, rows=4, out_stride=8, workspace=POINTER, bytes=1 << 40)
+             out=POINTER, rows=4, workspace=POINTER, bytes=1 << 40)
     a.update(kw)
     return lib.gtm_embed_gradient(*a.values())
 
