@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "libgtm_b200.so")
 SOURCES = [os.path.join(HERE, "csrc", f) for f in
            ["gtm_fit_chain_%s_rw%d.cu" % (kind, rw) for kind in ("wide", "narrow") for rw in (1, 4, 16, 32)] +
            ["gtm_api.cu", "gtm_fit_chain.cu", "gtm_fit_global.cu", "gtm_fit_resident.cu", "gtm_readout_adamw.cu",
-            "gtm_readout_embed.cu", "gtm_readout_softmax.cu", "gtm_stage.cu", "gtm_stream.cu", "gtm_tile.cu"]]
+            "gtm_readout_embed.cu", "gtm_readout_few_labels.cu", "gtm_readout_softmax.cu", "gtm_stage.cu", "gtm_stream.cu", "gtm_tile.cu"]]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 
 

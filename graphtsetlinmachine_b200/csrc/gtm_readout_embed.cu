@@ -649,6 +649,8 @@ extern "C" int gtm_embed(int device, void *cuda_stream, int type, const void *ta
     const int64_t segments = offsets ? number_of_bags : number_of_ids;
     if (segments == 0) return GTM_OK;
     if (!table || !out || (!ids && number_of_ids)) return fail(GTM_ERR_ARG, "gtm_embed: null array");
+    if ((uintptr_t)table % type_bytes(type) || (uintptr_t)ids % (ids_64 ? 8 : 4) || (uintptr_t)offsets % (offsets_64 ? 8 : 4))
+        return fail(GTM_ERR_ARG, "gtm_embed: an array does not start at a boundary of its elements");
     if (row_stride < 0 || row_stride >= kMostRows) return fail(GTM_ERR_ARG, "gtm_embed: row stride %lld of the table", (long long)row_stride);
     if ((uintptr_t)out % 16) return fail(GTM_ERR_ARG, "gtm_embed: the result does not start at a 16-byte boundary");
     uint64_t need = 0;
@@ -685,6 +687,8 @@ extern "C" int gtm_embed_gradient(int device, void *cuda_stream, int type, const
 {
     GTM_TRY(check_sizes("gtm_embed_gradient", type, rows, columns, number_of_ids, number_of_bags));
     if (!table_gradient || (number_of_ids && (!ids || !gradient))) return fail(GTM_ERR_ARG, "gtm_embed_gradient: null array");
+    if ((uintptr_t)gradient % type_bytes(type) || (uintptr_t)ids % (ids_64 ? 8 : 4) || (uintptr_t)offsets % (offsets_64 ? 8 : 4))
+        return fail(GTM_ERR_ARG, "gtm_embed_gradient: an array does not start at a boundary of its elements");
     if (gradient_stride < 0 || gradient_stride >= kMostRows) return fail(GTM_ERR_ARG, "gtm_embed_gradient: row stride %lld of the gradient", (long long)gradient_stride);
     if ((uintptr_t)table_gradient % 16) return fail(GTM_ERR_ARG, "gtm_embed_gradient: the result does not start at a 16-byte boundary");
     const GradientSpace space = gradient_space(number_of_ids, rows, columns);

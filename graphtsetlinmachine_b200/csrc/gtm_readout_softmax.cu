@@ -16,8 +16,10 @@
 // dx and dw are; fp16 has too small a range for that, so P is scaled by 2^14 over the largest |gradient * scale| there.
 #include "gtm_readout.cuh"
 #include "gtm_readout_mma.cuh"
+#include "gtm_readout_softmax.h"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace gtm_readout {
@@ -860,13 +862,14 @@ typedef CUresult (*EncodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, 
 
 int encode_tiled(EncodeTiled *out)
 {
-    static EncodeTiled found = nullptr;          // the same whichever thread finds it
+    static std::atomic<EncodeTiled> known;       // the same whichever thread finds it
+    EncodeTiled found = known.load();
     if (!found) {
         void *f = nullptr;
         cudaDriverEntryPointQueryResult result;
         GTM_CU(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &result));
         if (result != cudaDriverEntryPointSuccess || !f) return fail(GTM_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
-        found = (EncodeTiled)f;
+        known.store(found = (EncodeTiled)f);
     }
     *out = found;
     return GTM_OK;
@@ -909,10 +912,17 @@ int set_operands(Maps &maps, Product &p, int which, const Matrix &a, const Matri
 template <int kMode>
 int launch_product(const Maps &maps, Launch &l, cudaStream_t stream)
 {
-    void *error = nullptr;
-    GTM_CU(cudaGetSymbolAddress(&error, softmax_error));
+    // what does not change on a device is asked for once
+    static std::atomic<void *> errors[64];
+    int device = 0;
+    GTM_CU(cudaGetDevice(&device));
+    void *error = device < 64 ? errors[device].load() : nullptr;
+    if (!error) {
+        GTM_CU(cudaGetSymbolAddress(&error, softmax_error));
+        GTM_CU(cudaFuncSetAttribute(softmax_product_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared_of(kMode)));
+        if (device < 64) errors[device].store(error);
+    }
     l.error = (int *)error;
-    GTM_CU(cudaFuncSetAttribute(softmax_product_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared_of(kMode)));
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(2 * (l.schedule.units ? l.schedule.pairs : std::min(l.schedule.items, l.schedule.pairs))), config.blockDim = dim3(kThreads), config.dynamicSmemBytes = shared_of(kMode), config.stream = stream;
     cudaLaunchAttribute attribute;
@@ -1068,6 +1078,7 @@ int check_call(const char *what, const Call &c, float scale)
     if (c.labels < 1 || c.labels >= kMostRows / 4) return fail(GTM_ERR_ARG, "%s: %lld labels (1 to 2^29 - 1)", what, (long long)c.labels);
     if (c.columns < 1 || c.columns > (1 << 20)) return fail(GTM_ERR_ARG, "%s: %lld columns (1 to 2^20)", what, (long long)c.columns);
     if (c.x_stride < 0 || c.w_stride < 0) return fail(GTM_ERR_ARG, "%s: negative row stride", what);
+    if ((uintptr_t)c.x % type_bytes(c.type) || (uintptr_t)c.w % type_bytes(c.type)) return fail(GTM_ERR_ARG, "%s: an array does not start at a boundary of its elements", what);
     if (!(scale > 0.f) || scale > 3.4e38f) return fail(GTM_ERR_ARG, "%s: scale %g is not above zero and finite", what, (double)scale);
     return GTM_OK;
 }
@@ -1234,6 +1245,10 @@ extern "C" int gtm_softmax_workspace(int type, const void *features, int64_t exa
     GTM_TRY(check_call("gtm_softmax_workspace", c, 1.f));
     *bytes_out = 0;
     if (examples == 0) return GTM_OK;
+    if (few_labels(type, examples, labels, columns, c.gradient)) {
+        *bytes_out = few_labels_workspace(examples, labels, columns, c.gradient);
+        return GTM_OK;
+    }
     lay_out_workspace(c);
     *bytes_out = c.total;
     return GTM_OK;
@@ -1247,10 +1262,17 @@ extern "C" int gtm_softmax_loss(int device, void *cuda_stream, int type, const v
     GTM_TRY(check_call("gtm_softmax_loss", c, scale));
     if (examples == 0) return GTM_OK;
     if (!features || !weights || !labels || !losses || !normalisers) return fail(GTM_ERR_ARG, "gtm_softmax_loss: null array");
-    lay_out_workspace(c);
-    GTM_TRY(check_workspace("gtm_softmax_loss", workspace, workspace_bytes, c.total));
+    const bool few_ones = few_labels(type, examples, number_of_labels, columns, false);
+    if (!few_ones) {
+        lay_out_workspace(c);
+        GTM_TRY(check_workspace("gtm_softmax_loss", workspace, workspace_bytes, c.total));
+    }
     DeviceGuard guard(device);
     GTM_TRY(guard.status);
+    if (few_ones) {
+        const FewLabels few = {type, examples, number_of_labels, columns, features, weights, features_stride, weights_stride, labels, labels_64, ignore_label, scale};
+        return few_labels_loss(few, losses, normalisers, (cudaStream_t)cuda_stream);
+    }
     return forward(c, labels, labels_64, ignore_label, scale, losses, normalisers, nullptr, nullptr, (char *)workspace, (cudaStream_t)cuda_stream);
 }
 
@@ -1261,10 +1283,17 @@ extern "C" int gtm_softmax_predict(int device, void *cuda_stream, int type, cons
     GTM_TRY(check_call("gtm_softmax_predict", c, scale));
     if (examples == 0) return GTM_OK;
     if (!features || !weights || !labels_out || !log_probabilities_out) return fail(GTM_ERR_ARG, "gtm_softmax_predict: null array");
-    lay_out_workspace(c);
-    GTM_TRY(check_workspace("gtm_softmax_predict", workspace, workspace_bytes, c.total));
+    const bool few_ones = few_labels(type, examples, number_of_labels, columns, false);
+    if (!few_ones) {
+        lay_out_workspace(c);
+        GTM_TRY(check_workspace("gtm_softmax_predict", workspace, workspace_bytes, c.total));
+    }
     DeviceGuard guard(device);
     GTM_TRY(guard.status);
+    if (few_ones) {
+        const FewLabels few = {type, examples, number_of_labels, columns, features, weights, features_stride, weights_stride, nullptr, 0, 0, scale};
+        return few_labels_predict(few, labels_out, log_probabilities_out, (cudaStream_t)cuda_stream);
+    }
     return forward(c, nullptr, 0, 0, scale, nullptr, nullptr, labels_out, log_probabilities_out, (char *)workspace, (cudaStream_t)cuda_stream);
 }
 
@@ -1286,6 +1315,11 @@ extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type
         return GTM_OK;
     }
     if (!features || !weights || !labels || !normalisers || !gradients || !features_gradient) return fail(GTM_ERR_ARG, "gtm_softmax_loss_gradient: null array");
+    if (few_labels(type, examples, number_of_labels, columns, true)) {
+        GTM_TRY(check_workspace("gtm_softmax_loss_gradient", workspace, workspace_bytes, few_labels_workspace(examples, number_of_labels, columns, true)));
+        const FewLabels few = {type, examples, number_of_labels, columns, features, weights, features_stride, weights_stride, labels, labels_64, ignore_label, scale};
+        return few_labels_gradient(few, normalisers, gradients, gradients_step, features_gradient, weights_gradient, workspace, stream);
+    }
     lay_out_workspace(c);
     GTM_TRY(check_workspace("gtm_softmax_loss_gradient", workspace, workspace_bytes, c.total));
     char *w = (char *)workspace;

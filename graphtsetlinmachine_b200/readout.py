@@ -23,6 +23,8 @@ __all__ = ["embed", "embed_gradient", "softmax_loss", "softmax_loss_gradient", "
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INDEX = {torch.int32: 0, torch.int64: 1}
+# the current stream's handle, without the object around it where torch has that
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 BLOCK = 256      # elements; every tensor starts at a multiple of it in the flat states of `adamw_step`
 
 
@@ -70,7 +72,7 @@ def _vector(name, t, size):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return _current_stream(device.index)
 
 
 def _workspace(size, device):
@@ -215,8 +217,8 @@ def softmax_predict(features, weights, scale=1.0):
     return labels, log_probabilities
 
 
-def _padded(params):
-    return sum(-(-p.numel() // BLOCK) for p in params) * BLOCK
+def _padded(sizes):
+    return sum([-(-n // BLOCK) for n in sizes]) * BLOCK
 
 
 def adamw_state(params, state_bits=32):
@@ -228,7 +230,7 @@ def adamw_state(params, state_bits=32):
         raise ValueError("no tensors")
     if state_bits not in (8, 32):
         raise ValueError("states of %r bits: 8 or 32" % (state_bits,))
-    device, total = _cuda("params[0]", params[0]).device, _padded(params)
+    device, total = _cuda("params[0]", params[0]).device, _padded([p.numel() for p in params])
     kind = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
     state = {"steps": torch.zeros(1, dtype=torch.int64, device=device)}
     for name in ("first", "second"):
@@ -239,13 +241,19 @@ def adamw_state(params, state_bits=32):
 
 
 def _pointers(name, tensors, shapes, device):
-    """Data pointers of a list of contiguous tensors of one type on one device, and that type."""
-    kind = tensors[0].dtype if isinstance(tensors[0], torch.Tensor) else None
+    """Data pointers of a list of contiguous tensors of one type on one device, of the given shapes, and that type."""
+    for i, t in enumerate(tensors):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("%s[%d] is a torch tensor, not %s" % (name, i, type(t).__name__))
+    kind = tensors[0].dtype
     if kind not in _TYPES:
         raise TypeError("%s[0] is of %s: float32, bfloat16 and float16 are taken" % (name, kind))
-    for i, t in enumerate(tensors):
-        if not isinstance(t, torch.Tensor) or t.dtype != kind or t.device != device or not t.is_contiguous() or (shapes is not None and t.shape != shapes[i]):
-            raise ValueError("%s[%d] is not a contiguous %s tensor on %s%s" % (name, i, kind, device, "" if shapes is None else " of the parameter's shape"))
+    # lists are compared as a whole; which tensor it is matters when they differ
+    if ([t.dtype for t in tensors] != [kind] * len(tensors) or [t.device for t in tensors] != [device] * len(tensors)
+            or not all([t.is_contiguous() for t in tensors]) or [t.shape for t in tensors] != shapes):
+        for i, t in enumerate(tensors):
+            if t.dtype != kind or t.device != device or not t.is_contiguous() or t.shape != shapes[i]:
+                raise ValueError("%s[%d] is not a contiguous %s tensor on %s of the parameter's shape" % (name, i, kind, device))
     return (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors]), kind
 
 
@@ -261,13 +269,14 @@ def adamw_step(params, gradients, state, lr, betas=(0.9, 0.999), eps=1e-8, weigh
         raise ValueError("%d parameters, %d gradients%s" % (len(params), len(gradients), "" if copies is None else ", %d copies" % len(copies)))
     device = _cuda("params[0]", params[0]).device
     shapes = [p.shape for p in params]
-    param_ptrs, param_kind = _pointers("params", params, None, device)
+    sizes = [p.numel() for p in params]
+    param_ptrs, param_kind = _pointers("params", params, shapes, device)
     gradient_ptrs, gradient_kind = _pointers("gradients", gradients, shapes, device)
     copy_ptrs, copy_kind = (None, torch.bfloat16) if copies is None else _pointers("copies", list(copies), shapes, device)
     if copy_kind == torch.float32:
         raise TypeError("copies are bfloat16 or float16")
-    counts = (C.c_int64 * len(params))(*[p.numel() for p in params])
-    total = _padded(params)
+    counts = (C.c_int64 * len(params))(*sizes)
+    total = _padded(sizes)
     first, second, steps = state["first"], state["second"], state["steps"]
     narrow = first.dtype == torch.float8_e4m3fn
     if not narrow and first.dtype != torch.float32:

@@ -210,7 +210,7 @@ def check_gradient(x, w, labels, normalisers, gradients, scale, ignored=-1):
     return dx, dw
 
 
-SIZES = [(1, 1, 1), (1, 64, 10), (2, 7, 2), (60, 64, 10), (129, 65, 129), (256, 128, 256), (257, 200, 257), (300, 520, 1000), (33, 1024, 5001), (1000, 72, 300), (2100, 16, 40)]
+SIZES = [(1, 1, 1), (1, 64, 10), (2, 7, 2), (60, 64, 10), (129, 65, 129), (256, 128, 256), (257, 200, 257), (300, 520, 1000), (33, 1024, 5001), (1000, 72, 300), (2100, 16, 40), (5000, 33, 7), (700, 300, 32), (3, 64, 33), (5, 1000, 513), (8, 40, 4000)]
 
 
 @pytest.mark.parametrize("kind", TYPES)

@@ -38,14 +38,14 @@ def _embed_gradient(lib, **kw):
 
 
 def _loss(lib, **kw):
-    a = dict(device=0, stream=None, type=1, x=POINTER, n=3, x_stride=8, w=POINTER, v=5, w_stride=8, columns=8, labels=POINTER, wide=1, ignored=-1, scale=1.0,
+    a = dict(device=0, stream=None, type=1, x=POINTER, n=3, x_stride=8, w=POINTER, v=50, w_stride=8, columns=8, labels=POINTER, wide=1, ignored=-1, scale=1.0,
              losses=POINTER, normalisers=POINTER, workspace=POINTER, bytes=1 << 40)
     a.update(kw)
     return lib.gtm_softmax_loss(*a.values())
 
 
 def _predict(lib, **kw):
-    a = dict(device=0, stream=None, type=1, x=POINTER, n=3, x_stride=8, w=POINTER, v=5, w_stride=8, columns=8, scale=1.0, labels=POINTER, out=POINTER,
+    a = dict(device=0, stream=None, type=1, x=POINTER, n=3, x_stride=8, w=POINTER, v=50, w_stride=8, columns=8, scale=1.0, labels=POINTER, out=POINTER,
              workspace=POINTER, bytes=1 << 40)
     a.update(kw)
     return lib.gtm_softmax_predict(*a.values())
@@ -58,7 +58,7 @@ def _predict(lib, **kw):
     (_embed_gradient, dict(workspace=None)), (_embed_gradient, dict(workspace=C.c_void_p(4097))), (_embed_gradient, dict(gradient=None)), (_embed_gradient, dict(out=None)),
     (_loss, dict(type=-1)), (_loss, dict(n=-1)), (_loss, dict(n=1 << 23)), (_loss, dict(v=0)), (_loss, dict(v=1 << 29)), (_loss, dict(columns=0)), (_loss, dict(scale=0.0)),
     (_loss, dict(scale=-1.0)), (_loss, dict(scale=float("nan"))), (_loss, dict(scale=float("inf"))), (_loss, dict(x=None)), (_loss, dict(w=None)), (_loss, dict(labels=None)),
-    (_loss, dict(losses=None)), (_loss, dict(workspace=C.c_void_p(4097))), (_loss, dict(bytes=8)), (_loss, dict(x_stride=-8)), (_predict, dict(labels=None)),
+    (_loss, dict(losses=None)), (_loss, dict(workspace=C.c_void_p(4097))), (_loss, dict(bytes=8)), (_loss, dict(x_stride=-8)), (_loss, dict(x=C.c_void_p(4097))), (_embed, dict(table=C.c_void_p(4098))), (_embed, dict(ids=C.c_void_p(4100))), (_predict, dict(labels=None)),
     (_predict, dict(bytes=8)), (_predict, dict(scale=0.0)),
 ])
 def test_bad_arguments_are_refused(call, bad):
