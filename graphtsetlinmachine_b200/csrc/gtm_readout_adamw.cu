@@ -50,13 +50,6 @@ __device__ __forceinline__ unsigned mix(unsigned x)
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
-__device__ __forceinline__ float root_fast(float v)
-{
-    float r;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
-
 __device__ __forceinline__ float reciprocal_fast(float v)
 {
     float r;
@@ -207,14 +200,13 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
     }
 }
 
-// States of 8 bits.  What bounds it is instructions, so products and sums are fused, and the hardware's root and reciprocal (2^-22, exact next to
-// 8 bits) are used.
+// States of 8 bits.  The moments are computed operation by operation as in 32 bits: a last bit can decide between two codes, and with it what the states
+// are from then on.  The parameter is not among them: its quotient is the hardware's reciprocal (2^-23) in fused operations.
 template <class P, class G>
 __global__ void __launch_bounds__(256, 4) adamw_narrow_kernel(const __grid_constant__ AdamArgs a)
 {
     const int lane = threadIdx.x & 31;
     const StepConstants c = step_constants(a);
-    const float gradient_m = a.gradient_scale * a.other1, gradient_u = a.gradient_scale * sqrtf(a.other2), root_b2 = sqrtf(a.b2);
     int at = 0;
     for (long long b = (long long)blockIdx.x * 8 + threadIdx.x / 32; b < a.blocks; b += (long long)gridDim.x * 8) {
         const long long block = a.t[0].block + b;
@@ -223,7 +215,7 @@ __global__ void __launch_bounds__(256, 4) adamw_narrow_kernel(const __grid_const
         const long long flat = block * kBlock + lane * 8, i = flat - t.block * kBlock;
         const bool whole = is_whole<P, G>(t, i);
         const uint2 codes_m = *(const uint2 *)((const unsigned char *)a.first + flat), codes_u = *(const uint2 *)((const unsigned char *)a.second + flat);
-        const float held_m = a.first_scales[block] * a.b1, held_u = a.second_scales[block] * root_b2;
+        const float held_m = a.first_scales[block], held_u = a.second_scales[block];
         Pack<P, 8> p8;
         Pack<G, 8> g8;
         if (whole) load_all((const P *)t.param, i, p8), load_all((const G *)t.gradient, i, g8);      // the warp is of one mind: no load waits for another
@@ -233,10 +225,10 @@ __global__ void __launch_bounds__(256, 4) adamw_narrow_kernel(const __grid_const
         float largest_m = 0.f, largest_u = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            const float g = to_float(g8.v[k]), by_u = g * gradient_u;
-            m[k] = fmaf(g, gradient_m, m[k] * held_m);
-            u[k] *= held_u;
-            u[k] = root_fast(fmaf(by_u, by_u, u[k] * u[k]));
+            const float g = __fmul_rn(to_float(g8.v[k]), a.gradient_scale);
+            m[k] = __fadd_rn(__fmul_rn(__fmul_rn(m[k], held_m), a.b1), __fmul_rn(g, a.other1));
+            u[k] = __fmul_rn(u[k], held_u);
+            u[k] = __fsqrt_rn(__fadd_rn(__fmul_rn(__fmul_rn(u[k], u[k]), a.b2), __fmul_rn(__fmul_rn(g, g), a.other2)));
             const float moved = m[k] * reciprocal_fast(fmaf(u[k], c.root_correction, a.eps));
             p[k] = fmaf(-c.step_size, moved, to_float(p8.v[k]) * a.decay);
             largest_m = fmaxf(largest_m, fabsf(m[k]));               // NaN is passed over

@@ -113,20 +113,42 @@ __device__ __forceinline__ void commit_to_pair(unsigned barrier)
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(barrier), "h"((unsigned short)3) : "memory");
 }
 
-// 64 columns of the warp's 32 rows: column i in v[i].
+// Columns of the warp's 32 rows: column i in v[i].
+__device__ __forceinline__ void tmem_load32_begin(unsigned from, float *v)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+                   "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]),
+                   "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]),
+                   "=f"(v[31])
+                 : "r"(from));
+}
+
+// Waits for the warp's loads.  The registers are operands, so that nothing is done with them before.
+__device__ __forceinline__ void tmem_load32_end(float *v)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),
+                 "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]),
+                 "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+                 "+f"(v[30]), "+f"(v[31])
+                 :
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_load32(unsigned from, float (&v)[32])
+{
+    tmem_load32_begin(from, v);
+    tmem_load32_end(v);
+}
+
 __device__ __forceinline__ void tmem_load64(unsigned from, float (&v)[64])
 {
-    unsigned *r = (unsigned *)v;
-#pragma unroll
-    for (int h = 0; h < 64; h += 32)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                     "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                     : "=r"(r[h + 0]), "=r"(r[h + 1]), "=r"(r[h + 2]), "=r"(r[h + 3]), "=r"(r[h + 4]), "=r"(r[h + 5]), "=r"(r[h + 6]), "=r"(r[h + 7]), "=r"(r[h + 8]),
-                       "=r"(r[h + 9]), "=r"(r[h + 10]), "=r"(r[h + 11]), "=r"(r[h + 12]), "=r"(r[h + 13]), "=r"(r[h + 14]), "=r"(r[h + 15]), "=r"(r[h + 16]),
-                       "=r"(r[h + 17]), "=r"(r[h + 18]), "=r"(r[h + 19]), "=r"(r[h + 20]), "=r"(r[h + 21]), "=r"(r[h + 22]), "=r"(r[h + 23]), "=r"(r[h + 24]),
-                       "=r"(r[h + 25]), "=r"(r[h + 26]), "=r"(r[h + 27]), "=r"(r[h + 28]), "=r"(r[h + 29]), "=r"(r[h + 30]), "=r"(r[h + 31])
-                     : "r"(from + h));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    tmem_load32_begin(from, v);
+    tmem_load32_begin(from + 32, v + 32);
+    tmem_load32_end(v);
+    tmem_load32_end(v + 32);
 }
 
 // The kernel behind this one may be set up while this one ends, and waits for its end before it reads what others have written.

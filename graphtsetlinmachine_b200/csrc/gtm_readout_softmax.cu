@@ -12,7 +12,9 @@
 // pass is a kernel of plain dot products, whose time is that of reading w.
 //
 // 16-bit inputs are multiplied as they are, with sums in 32 bits.  32-bit inputs are split into three bf16 parts (24 bits of fraction),
-// and the six products of parts that reach 2^-24 are added, the smallest first.  P is rounded to the operands' type, to as many bits as
+// and the six products of parts that reach 2^-24 are added, the smallest first.  The tensor cores cut sums off instead of rounding them, about 1e-8 of
+// the sum at every step of 16 elements and always towards zero; so where inputs have 32 bits, the large products of a logit are summed in two
+// halves, and sums for dw and dx go to memory after 512 elements, where they are added with rounding.  P is rounded to the operands' type, to as many bits as
 // dx and dw are; fp16 has too small a range for that, so P is scaled by 2^14 over the largest |gradient * scale| there.
 #include "gtm_readout.cuh"
 #include "gtm_readout_mma.cuh"
@@ -54,6 +56,7 @@ struct Product {
     int m_tiles, n_tiles, tile_columns;         // 256 or 128 columns of a tile
     int m_fast;                                 // tiles of one column block follow each other
     int depth_blocks, products, blocks, per_split;  // blocks of a tile are cut into splits of per_split
+    int chunk;                                  // blocks of the index whose products of parts follow each other; sums of several products end with them
     int a_rows;                                 // operand A's rows, not the sum's index, lie next to each other (operand B's never do: that is a third slower)
     int a_first;                                // offset of the sum's index in operand A (a row of W)
     int b_row;                                  // offset of the result's columns in operand B (a row of W)
@@ -120,34 +123,47 @@ struct Launch {
 // A pair's work, piece by piece.
 struct Work {
     const Launch &l;
-    int pair, item;
-    long long unit, end;
-    // the piece at hand: product, tile, blocks [first, last)
+    int pair, item, at;                          // the next item of the first product, and where in it
+    long long unit, begin, end;
+    // the piece at hand: product, tile, blocks [first, last), whether its sums are the first of their tile and slice
     int which, m, n, first, last, split;
+    bool fresh;
 
     __device__ __forceinline__ explicit Work(const Launch &launch) : l(launch)
     {
-        pair = blockIdx.x / 2, item = pair;
-        unit = l.schedule.units ? l.schedule.begin(pair) : 0;
+        pair = blockIdx.x / 2, item = pair, at = 0;
+        unit = begin = l.schedule.units ? l.schedule.begin(pair) : 0;
         end = l.schedule.units ? l.schedule.begin(pair + 1) : 0;
+    }
+    // The end of a piece that begins at block `from`.
+    __device__ __forceinline__ static int cut(const Product &p, int from, long long end)
+    {
+        const int chunk = p.chunk * p.products;
+        return (int)min(end, p.products == 1 ? (long long)p.blocks : min((long long)p.blocks, (from / chunk + 1ll) * chunk));
     }
     __device__ __forceinline__ bool next()
     {
         if (unit < end) {
             which = 1;
-            const int tile = (int)(unit / l.p[1].blocks);
-            l.p[1].tile(tile, m, n);
-            first = (int)(unit - (long long)tile * l.p[1].blocks), last = (int)min((long long)l.p[1].blocks, first + end - unit);
+            const Product &p = l.p[1];
+            const int tile = (int)(unit / p.blocks);
+            p.tile(tile, m, n);
+            first = (int)(unit - (long long)tile * p.blocks), last = cut(p, first, first + end - unit);
+            fresh = first == 0 || unit == begin;
             split = tile;                        // its slice is looked up by who needs it
             unit += last - first;
             return true;
         }
         if (item >= l.schedule.items) return false;
         which = 0;
-        split = item / l.p[0].tiles();
-        l.p[0].tile(item - split * l.p[0].tiles(), m, n);
-        first = split * l.p[0].per_split, last = min(l.p[0].blocks, first + l.p[0].per_split);
-        item += l.schedule.pairs;
+        const Product &p = l.p[0];
+        split = item / p.tiles();
+        p.tile(item - split * p.tiles(), m, n);
+        const int from = split * p.per_split, to = min(p.blocks, from + p.per_split);
+        first = from + at, last = cut(p, first, to);
+        fresh = at == 0;
+        at += last - first;
+        if (last == to) item += l.schedule.pairs, at = 0;
         return true;
     }
     __device__ __forceinline__ int slice() const { return which == 0 ? split : pair - l.schedule.pair_of((long long)split * l.p[1].blocks); }
@@ -302,19 +318,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
             const CUtensorMap *map_a = &maps.a[w.which], *map_b = &maps.b[w.which];
             const int half_columns = p.tile_columns / 2;
             const int m0 = w.m * 256 + (int)rank * 128, n0 = w.n * p.tile_columns + (int)rank * half_columns + p.b_row;
-            int product = w.first / p.depth_blocks, block = w.first - product * p.depth_blocks;
+            // the product of parts, and the block of the sum's index, of a chunk at a time
+            const int chunk = w.first / (p.chunk * p.products), chunk_first = chunk * p.chunk, chunk_blocks = min(p.chunk, p.depth_blocks - chunk_first);
+            int product = (w.first - chunk_first * p.products) / chunk_blocks, block = w.first - chunk_first * p.products - product * chunk_blocks;
             for (int i = w.first; i < w.last; i++) {
                 if (!(fine = barrier_wait(empty + 8 * stage, phase ^ 1))) break;
                 const unsigned to = ring + stage * kStageBytes, bar = in_leader(full + 8 * stage);
                 if (rank == 0) barrier_expect(full + 8 * stage, 2 * (kHalfBytes + half_columns * kDepth * 2));
                 int part_a, part_b;
                 parts_of(p.products, product, part_a, part_b);
-                const int k = block * kDepth;
+                const int k = (chunk_first + block) * kDepth;
                 if (p.a_rows)
                     for (int g = 0; g < 2; g++) load_box(map_a, to + g * 8192, bar, m0 + g * 64, p.a_first + k, part_a);
                 else load_box(map_a, to, bar, k, m0, part_a);
                 load_box(map_b, to + kHalfBytes, bar, k, n0, part_b);
-                if (++block == p.depth_blocks) block = 0, product++;
+                if (++block == chunk_blocks) block = 0, product++;
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
         }
@@ -335,20 +353,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
             const unsigned a_leading = p.a_rows ? 8192 : 16, a_step = p.a_rows ? 2048 : 32, what = p.what;
             if (!(fine = barrier_wait(sums_empty + 8 * buffer, buffer_phase ^ 1))) break;
             tmem_after_sync();
-            const unsigned to = tmem + buffer * 256;
+            unsigned to = tmem + buffer * 256;
+            const bool halves = kMode != kOut && p.products > 1;
+            int fresh = w.first;                  // the block that begins a sum
             for (int i = w.first; i < w.last; i++) {
                 if (!(fine = barrier_wait(full + 8 * stage, phase))) break;
                 tmem_after_sync();
                 const unsigned a = ring + stage * kStageBytes, b = a + kHalfBytes;
+                if (halves && i == p.blocks - p.depth_blocks / 2) to += 256, fresh = i;      // the other half of the large products
 #pragma unroll
                 for (int k = 0; k < kDepth / 16; k++)
-                    multiply(to, operand(a + k * a_step, a_leading, 1024), operand(b + k * 32, 16, 1024), what, i > w.first || k > 0);
+                    multiply(to, operand(a + k * a_step, a_leading, 1024), operand(b + k * 32, 16, 1024), what, i > fresh || k > 0);
                 commit_to_pair(empty + 8 * stage);
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
             if (!fine) break;
             commit_to_pair(sums_full + 8 * buffer);
-            if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+            if (halves || ++buffer == 2) buffer = 0, buffer_phase ^= 1;
         }
     } else if (warp >= 4) {
         const int quarter = (warp - 4) & 3, half = (warp - 4) / 4;
@@ -377,6 +398,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
             fine = barrier_wait(sums_full + 8 * buffer, buffer_phase);
             if (!__all_sync(~0u, fine)) break;
             tmem_after_sync();
+            const bool halves = kMode != kOut && p.products > 1;
             const unsigned from = tmem + buffer * 256 + half * half_columns + ((unsigned)(quarter * 32) << 16);
 #pragma unroll 1
             for (int c = 0; c < half_columns; c += 64) {
@@ -384,6 +406,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
                 if (left <= 0) break;                                       // the warp together
                 float v[64];
                 tmem_load64(from + c, v);
+                if (halves && p.depth_blocks > 1)
+#pragma unroll
+                    for (int h = 0; h < 64; h += 32) {
+                        float other[32];
+                        tmem_load32(from + 256 + c + h, other);
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[h + j] += other[j];
+                    }
                 if (c + 64 >= half_columns || left <= 64) {
                     // the tile's last columns are in registers: the next but one may overwrite it
                     tmem_before_sync();
@@ -431,7 +461,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
 #pragma unroll
                     for (int j = 0; j < 64; j++) v[j] *= out_scale;
                     if (row0 >= p.rows) continue;
-                    if (p.type == GTM_F32) send_32(store, v, &maps.out[w.which], (int)column, (int)row0, slice, p.add, left);
+                    // what is added to has to be there, or the order of two additions would be open
+                    if (p.products > 1 && !w.fresh) BoxStore::finish();
+                    if (p.type == GTM_F32) send_32(store, v, &maps.out[w.which], (int)column, (int)row0, slice, p.add || !w.fresh, left);
                     else send_16(store, v, p.type == GTM_F16, &maps.out[w.which], (int)column, (int)row0, slice);
                 }
             }
@@ -445,7 +477,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
                 l.sums[at] = kMode == kSums ? make_float2(sums.largest, sums.sum) : make_float2(best.largest, best.rest);
                 if (kMode == kBest) l.best[at] = best.index;
             }
-            if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+            if (halves || ++buffer == 2) buffer = 0, buffer_phase ^= 1;
         }
         if (kStores) BoxStore::finish();
     }
@@ -946,6 +978,7 @@ Product product_of(int64_t rows, int64_t columns, int64_t depth, int products)
     p.m_tiles = (int)((rows + 255) / 256), p.n_tiles = (int)((columns + p.tile_columns - 1) / p.tile_columns);
     p.depth_blocks = (int)((depth + kDepth - 1) / kDepth);
     p.blocks = p.per_split = p.depth_blocks * products;
+    p.chunk = p.depth_blocks;
     return p;
 }
 
@@ -1059,6 +1092,7 @@ void lay_out_workspace(Call &c)
         c.at_prob = take((uint64_t)c.parts * c.examples * c.prob_ld * 2);
         c.dx = product_of(c.columns, c.examples, c.piece_labels, c.products);          // turned: its operand B is P
         c.dw = product_of(c.piece_labels, c.columns, c.examples, c.products);
+        if (c.products > 1) c.dx.chunk = c.dw.chunk = 8;
         // dw's tiles are cut where they are less than half of the pairs of SMs, into eight blocks or more
         const int splits = std::max(1, std::min(kPairs / c.dw.tiles(), c.dw.blocks / 8));
         c.dw.per_split = (c.dw.blocks + splits - 1) / splits;
