@@ -59,6 +59,23 @@ __device__ __forceinline__ long long index_at(const void *p, int wide, long long
     return wide ? __ldg((const long long *)p + i) : (long long)__ldg((const int *)p + i);
 }
 
+// The kernel behind this one may be set up while this one ends, and waits for its end before it reads what others have written.
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// A launch that may be set up while the kernel before it on the stream ends; its kernel begins with `wait_for_previous`.
+template <class... Params, class... Given>
+inline int launch_early(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream, Given &&...given)
+{
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid, config.blockDim = block, config.dynamicSmemBytes = shared, config.stream = stream;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization, attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute, config.numAttrs = 1;
+    GTM_CU(cudaLaunchKernelEx(&config, kernel, static_cast<Params>(given)...));
+    return GTM_OK;
+}
+
 template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 }  // namespace gtm_readout

@@ -98,8 +98,10 @@ constexpr int kGatherThreads = 128, kGatherBlocks = 7;
 
 // A lane has U runs of V columns next to each other, kLanes * V apart.
 template <class T, int V, int U, int kLanes>
-__global__ void __launch_bounds__(kGatherThreads, kGatherBlocks) gather_sum_kernel(const GatherArgs a)
+__global__ void __launch_bounds__(kGatherThreads, U == 1 ? kGatherBlocks : 4) gather_sum_kernel(const GatherArgs a)
 {
+    next_may_start();
+    wait_for_previous();
     constexpr int kColumns = kLanes * V * U, kAhead = 4;
     const int lane = threadIdx.x % kLanes, column0 = blockIdx.y * kColumns;
     const unsigned team = kLanes == 32 ? ~0u : ((1u << kLanes % 32) - 1) << ((threadIdx.x & 31) / kLanes * kLanes);
@@ -242,6 +244,8 @@ __global__ void __launch_bounds__(kGatherThreads, kGatherBlocks) gather_sum_kern
 template <class T>
 __global__ void __launch_bounds__(256) gather_join_kernel(const GatherArgs a)
 {
+    next_may_start();
+    wait_for_previous();
     constexpr int kAlone = 16, kWarps = 8;
     __shared__ float4 sums[kWarps][32];
     __shared__ long long longest[kWarps];
@@ -331,12 +335,8 @@ int launch_gather(const GatherArgs &a, cudaStream_t stream)
     constexpr int kWide = kLanes * V * U, kTeams = kGatherThreads / kLanes;
     const long long units = a.spans + (a.segments + kLanes - 1) / kLanes;
     const dim3 grid((unsigned)((units + kTeams - 1) / kTeams), (unsigned)((a.columns + kWide - 1) / kWide));
-    gather_sum_kernel<T, V, U, kLanes><<<grid, kGatherThreads, 0, stream>>>(a);
-    GTM_CU(cudaGetLastError());
-    if (a.spans > 1) {
-        gather_join_kernel<T><<<dim3((unsigned)((a.spans + 7) / 8), (unsigned)((a.columns + 127) / 128)), 256, 0, stream>>>(a);
-        GTM_CU(cudaGetLastError());
-    }
+    GTM_TRY(launch_early(gather_sum_kernel<T, V, U, kLanes>, grid, dim3(kGatherThreads), 0, stream, a));
+    if (a.spans > 1) GTM_TRY(launch_early(gather_join_kernel<T>, dim3((unsigned)((a.spans + 7) / 8), (unsigned)((a.columns + 127) / 128)), dim3(256), 0, stream, a));
     return GTM_OK;
 }
 
@@ -394,6 +394,15 @@ __global__ void __launch_bounds__(256) embed_rows_kernel(const T *table, long lo
                 else
 #pragma unroll
                     for (int v = 0; v < V; v++) p[e].v[v] = from_float<T>(id < 0 ? 0.f : __int_as_float(0x7fffffff));
+            } else if (c + V <= columns) {
+                // all of one row
+                const bool real = id >= 0 && id < rows;
+                const T *from = table + (real ? id : 0) * stride + c;
+#pragma unroll
+                for (int v = 0; v < V; v++) p[e].v[v] = from[v];
+                if (!real)
+#pragma unroll
+                    for (int v = 0; v < V; v++) p[e].v[v] = from_float<T>(id < 0 ? 0.f : __int_as_float(0x7fffffff));
             } else {
 #pragma unroll
                 for (int v = 0; v < V; v++) {
@@ -439,6 +448,7 @@ int launch_rows(const void *table, int64_t stride, int64_t rows, const void *ids
 // ------------------------------------------------------------------------------------ ids sorted, for the gradient
 // Radix sort by digits of kDigit bits, the lowest first, of (id, bag) pairs; every pass keeps the order of equal digits.
 // Ids that the table does not have (padding, too large ones, positions outside every bag) sort behind its last row.
+// Every kernel of the chain may be set up while the one before it ends.
 constexpr int kDigit = 8, kDigits = 1 << kDigit, kSortThreads = 256, kSortWarps = kSortThreads / 32;
 
 // A warp has kEach * 32 pairs in a row, 32 at a time.
@@ -454,6 +464,8 @@ template <int kEach>
 __global__ void __launch_bounds__(kSortThreads) sort_keys_kernel(const void *ids, int ids_wide, long long n, const void *offsets, int offsets_wide, long long bags, unsigned rows,
                                                                 uint2 *pairs, unsigned *counts)
 {
+    next_may_start();
+    wait_for_previous();
     __shared__ unsigned hist[kDigits];
     hist[threadIdx.x] = 0;
     __syncthreads();
@@ -475,6 +487,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_keys_kernel(const void *ids
 template <int kEach>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const uint2 *pairs, long long n, int shift, unsigned *counts)
 {
+    next_may_start();
+    wait_for_previous();
     __shared__ unsigned hist[kDigits];
     hist[threadIdx.x] = 0;
     __syncthreads();
@@ -493,6 +507,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const uint2 *p
 // a thread has a digit and every fourth part of the blocks.
 __global__ void __launch_bounds__(1024) sort_scan_kernel(unsigned *counts, int blocks)
 {
+    next_may_start();
+    wait_for_previous();
     __shared__ unsigned sums[4][kDigits], warp_sums[8];
     const int digit = threadIdx.x & (kDigits - 1), part = threadIdx.x / kDigits, lane = threadIdx.x & 31;
     const int per = (blocks + 3) / 4, first = min(blocks, part * per), last = min(blocks, first + per);
@@ -535,6 +551,8 @@ __global__ void __launch_bounds__(1024) sort_scan_kernel(unsigned *counts, int b
 template <int kEach>
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const uint2 *pairs, long long n, int shift, const unsigned *counts, uint2 *sorted)
 {
+    next_may_start();
+    wait_for_previous();
     __shared__ unsigned warp_hist[kSortWarps][kDigits];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
 #pragma unroll
@@ -575,6 +593,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(const uint2 *p
 // pair at a position writes the offsets of the rows behind the pair before it; of many such rows, its warp does.
 __global__ void __launch_bounds__(256) sort_rows_kernel(const uint2 *sorted, long long n, long long rows, int *offsets)
 {
+    next_may_start();
+    wait_for_previous();
     const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
     const int lane = threadIdx.x & 31;
     long long low = 0, high = 0;                   // offsets [low, high) are t
@@ -705,23 +725,18 @@ extern "C" int gtm_embed_gradient(int device, void *cuda_stream, int type, const
         const unsigned tiles = (unsigned)space.tiles;
         const auto sort = [&](auto each) -> int {
             constexpr int kEach = decltype(each)::value;
-            sort_keys_kernel<kEach><<<tiles, kSortThreads, 0, stream>>>(ids, ids_64, n, offsets, offsets_64, number_of_bags, (unsigned)rows, from, counts);
-            GTM_CU(cudaGetLastError());
+            GTM_TRY(launch_early(sort_keys_kernel<kEach>, dim3(tiles), dim3(kSortThreads), 0, stream, ids, ids_64, n, offsets, offsets_64, (long long)number_of_bags, (unsigned)rows, from, counts));
             for (int shift = 0; shift < 32 && ((uint64_t)rows >> shift) != 0; shift += kDigit) {
-                if (shift) sort_count_kernel<kEach><<<tiles, kSortThreads, 0, stream>>>(from, n, shift, counts);
-                GTM_CU(cudaGetLastError());
-                sort_scan_kernel<<<1, 1024, 0, stream>>>(counts, (int)tiles);
-                GTM_CU(cudaGetLastError());
-                sort_place_kernel<kEach><<<tiles, kSortThreads, 0, stream>>>(from, n, shift, counts, to);
-                GTM_CU(cudaGetLastError());
+                if (shift) GTM_TRY(launch_early(sort_count_kernel<kEach>, dim3(tiles), dim3(kSortThreads), 0, stream, from, n, shift, counts));
+                GTM_TRY(launch_early(sort_scan_kernel, dim3(1), dim3(1024), 0, stream, counts, (int)tiles));
+                GTM_TRY(launch_early(sort_place_kernel<kEach>, dim3(tiles), dim3(kSortThreads), 0, stream, from, n, shift, counts, to));
                 std::swap(from, to);
             }
             return GTM_OK;
         };
         GTM_TRY(space.each == 4 ? sort(std::integral_constant<int, 4>()) : sort(std::integral_constant<int, 16>()));
     }
-    sort_rows_kernel<<<(unsigned)((n + 256) / 256), 256, 0, stream>>>(from, n, rows, (int *)(w + space.offsets));
-    GTM_CU(cudaGetLastError());
+    GTM_TRY(launch_early(sort_rows_kernel, dim3((unsigned)((n + 256) / 256)), dim3(256), 0, stream, from, n, (long long)rows, (int *)(w + space.offsets)));
     GatherArgs a;
     a.src = gradient, a.src_stride = gradient_stride, a.rows = offsets ? number_of_bags : n;
     a.pairs = from, a.list = nullptr, a.list_wide = 0, a.positions = n;

@@ -151,10 +151,6 @@ __device__ __forceinline__ void tmem_load64(unsigned from, float (&v)[64])
     tmem_load32_end(v + 32);
 }
 
-// The kernel behind this one may be set up while this one ends, and waits for its end before it reads what others have written.
-__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 __device__ __forceinline__ float exp2_fast(float x)
 {
     float y;
