@@ -160,6 +160,8 @@ __device__ __forceinline__ void store_param(const AdamArgs &a, const AdamTensor 
 template <class P, class G>
 __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamArgs a)
 {
+    next_may_start();
+    wait_for_previous();
     const int lane = threadIdx.x & 31;
     const StepConstants c = step_constants(a);
     int at = 0;
@@ -205,6 +207,8 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
 template <class P, class G>
 __global__ void __launch_bounds__(256, 4) adamw_narrow_kernel(const __grid_constant__ AdamArgs a)
 {
+    next_may_start();
+    wait_for_previous();
     const int lane = threadIdx.x & 31;
     const StepConstants c = step_constants(a);
     int at = 0;
@@ -282,7 +286,12 @@ __global__ void __launch_bounds__(256, 4) adamw_narrow_kernel(const __grid_const
     }
 }
 
-__global__ void adamw_count_kernel(long long *steps) { *steps += 1; }
+__global__ void adamw_count_kernel(long long *steps)
+{
+    next_may_start();
+    wait_for_previous();
+    *steps += 1;
+}
 
 template <class P, class G>
 int launch(const AdamArgs &a, bool narrow, cudaStream_t stream)
@@ -292,10 +301,7 @@ int launch(const AdamArgs &a, bool narrow, cudaStream_t stream)
     GTM_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
     const long long want = (a.blocks + 7) / 8, most = (long long)sms * 8;
     const unsigned grid = (unsigned)(want < most ? want : most);
-    if (narrow) adamw_narrow_kernel<P, G><<<grid, 256, 0, stream>>>(a);
-    else adamw_kernel<P, G><<<grid, 256, 0, stream>>>(a);
-    GTM_CU(cudaGetLastError());
-    return GTM_OK;
+    return launch_early(narrow ? adamw_narrow_kernel<P, G> : adamw_kernel<P, G>, dim3(grid), dim3(256), 0, stream, a);
 }
 
 template <class P>
@@ -357,7 +363,5 @@ extern "C" int gtm_adamw_step(int device, void *cuda_stream, int64_t number_of_t
                 : param_type == GTM_BF16 ? launch<__nv_bfloat16>(a, gradient_type, narrow, stream)
                                          : launch<__half>(a, gradient_type, narrow, stream));
     }
-    adamw_count_kernel<<<1, 1, 0, stream>>>((long long *)steps);
-    GTM_CU(cudaGetLastError());
-    return GTM_OK;
+    return launch_early(adamw_count_kernel, dim3(1), dim3(1), 0, stream, (long long *)steps);
 }

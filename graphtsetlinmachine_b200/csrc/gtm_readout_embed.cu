@@ -378,6 +378,8 @@ int launch_gather(GatherArgs &a, int type, char *workspace, const GatherSpace &s
 template <class T, bool kWhole, bool kNarrow>
 __global__ void __launch_bounds__(256) embed_rows_kernel(const T *table, long long stride, long long rows, const void *ids, int ids_wide, long long count, int columns, float scale, T *out)
 {
+    next_may_start();
+    wait_for_previous();
     constexpr int V = 16 / sizeof(T), kEach = kWhole ? 4 : 2;
     const long long all = count * columns, step = (long long)gridDim.x * 256 * V;
     for (long long first = ((long long)blockIdx.x * 256 + threadIdx.x) * V; first < all; first += step * kEach) {
@@ -436,13 +438,8 @@ int launch_rows(const void *table, int64_t stride, int64_t rows, const void *ids
     const bool whole = aligned(table, stride * sizeof(T), 16) && columns % V == 0, narrow = count * columns < (int64_t)1 << 32;
     const int64_t chunks = (count * columns + V - 1) / V, blocks = (chunks + 255) / 256;
     const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
-#define GTM_ROWS(W, N) embed_rows_kernel<T, W, N><<<grid, 256, 0, stream>>>((const T *)table, stride, rows, ids, ids_wide, count, (int)columns, scale, (T *)out)
-    if (whole) { if (narrow) GTM_ROWS(true, true); else GTM_ROWS(true, false); }
-    else if (narrow) GTM_ROWS(false, true);
-    else GTM_ROWS(false, false);
-#undef GTM_ROWS
-    GTM_CU(cudaGetLastError());
-    return GTM_OK;
+    const auto kernel = whole ? (narrow ? embed_rows_kernel<T, true, true> : embed_rows_kernel<T, true, false>) : narrow ? embed_rows_kernel<T, false, true> : embed_rows_kernel<T, false, false>;
+    return launch_early(kernel, dim3(grid), dim3(256), 0, stream, (const T *)table, (long long)stride, (long long)rows, ids, ids_wide, (long long)count, (int)columns, scale, (T *)out);
 }
 
 // ------------------------------------------------------------------------------------ ids sorted, for the gradient

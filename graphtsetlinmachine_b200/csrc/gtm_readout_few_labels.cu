@@ -53,6 +53,8 @@ enum Mode { kLoss, kPredict, kGradient };
 template <class T, int kLabels, int kMode>
 __global__ void __launch_bounds__(kWarps * 32) few_labels_kernel(const Args a)
 {
+    next_may_start();
+    wait_for_previous();
     extern __shared__ float shared[];
     const FewLabels &p = a.p;
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, columns = (int)p.columns, labels = (int)p.labels;
@@ -162,6 +164,8 @@ __global__ void __launch_bounds__(kWarps * 32) few_labels_kernel(const Args a)
 template <class T>
 __global__ void __launch_bounds__(256) few_labels_join_kernel(const float *partial, int blocks, long long size, T *dw)
 {
+    next_may_start();
+    wait_for_previous();
     const long long i = (long long)blockIdx.x * 32 + (threadIdx.x & 31);
     __shared__ float sums[kWarps][32];
     const int warp = threadIdx.x / 32;
@@ -188,9 +192,7 @@ int run(const Args &a, unsigned blocks, cudaStream_t stream)
 {
     const size_t shared = (size_t)a.p.labels * a.p.columns * 4 + (kMode == kGradient ? (size_t)a.per_block * kLabels * 4 : 0);
     if (shared > 48 << 10) GTM_CU(cudaFuncSetAttribute(few_labels_kernel<T, kLabels, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kLargestShared));
-    few_labels_kernel<T, kLabels, kMode><<<blocks, kWarps * 32, shared, stream>>>(a);
-    GTM_CU(cudaGetLastError());
-    return GTM_OK;
+    return launch_early(few_labels_kernel<T, kLabels, kMode>, dim3(blocks), dim3(kWarps * 32), shared, stream, a);
 }
 
 template <class T, int kMode>
@@ -211,10 +213,9 @@ int run(Args &a, cudaStream_t stream)
 
 }  // namespace
 
-bool few_labels(int type, int64_t examples, int64_t labels, int64_t columns, bool gradient)
+bool few_labels(int64_t examples, int64_t labels, int64_t columns, bool gradient)
 {
-    (void)type;
-    // many examples of a gradient leave their P in shared memory; with many more, or more labels, the tensor cores are faster
+    // a block has P of its examples in shared memory, 28 KB at the most
     return labels <= 32 && labels * columns * 4 <= kLargestShared && examples <= (gradient ? 1 << 16 : 1 << 20);
 }
 
@@ -246,11 +247,9 @@ int few_labels_gradient(const FewLabels &p, const float *normalisers, const floa
     const long long size = p.labels * p.columns;
     const int blocks = (int)((p.examples + a.per_block - 1) / a.per_block);
     const unsigned grid = (unsigned)((size + 31) / 32);
-    if (p.type == GTM_F32) few_labels_join_kernel<float><<<grid, 256, 0, stream>>>(a.partial, blocks, size, (float *)dw);
-    else if (p.type == GTM_BF16) few_labels_join_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a.partial, blocks, size, (__nv_bfloat16 *)dw);
-    else few_labels_join_kernel<__half><<<grid, 256, 0, stream>>>(a.partial, blocks, size, (__half *)dw);
-    GTM_CU(cudaGetLastError());
-    return GTM_OK;
+    if (p.type == GTM_F32) return launch_early(few_labels_join_kernel<float>, dim3(grid), dim3(256), 0, stream, a.partial, blocks, size, (float *)dw);
+    if (p.type == GTM_BF16) return launch_early(few_labels_join_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, stream, a.partial, blocks, size, (__nv_bfloat16 *)dw);
+    return launch_early(few_labels_join_kernel<__half>, dim3(grid), dim3(256), 0, stream, a.partial, blocks, size, (__half *)dw);
 }
 
 }  // namespace gtm_readout

@@ -56,12 +56,12 @@ __device__ __forceinline__ unsigned long long nanoseconds()
     return t;
 }
 
-// Waits for a phase of a barrier, two seconds at most.
+// Waits for a phase of a barrier, ten seconds at most.
 __device__ __forceinline__ bool barrier_wait(unsigned barrier, unsigned parity)
 {
     if (barrier_try(barrier, parity)) return true;
     const unsigned long long began = nanoseconds();
-    while (nanoseconds() - began < 2000000000ull)
+    while (nanoseconds() - began < 10000000000ull)
         for (int i = 0; i < 64; i++)
             if (barrier_try(barrier, parity)) return true;
     return false;

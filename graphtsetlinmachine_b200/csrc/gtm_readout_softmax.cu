@@ -508,6 +508,8 @@ struct FewArgs {
 template <class T, int kExamples, bool kWhole, bool kFindBest>
 __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs a)
 {
+    next_may_start();
+    wait_for_previous();
     constexpr int V = kWhole ? 16 / sizeof(T) : 1, kValues = kExamples * kFewRows, kStep = 32 * V;
     extern __shared__ float4 shared_x4[];
     float *shared_x = (float *)shared_x4;       // [example][columns, rounded up to the step]
@@ -605,6 +607,8 @@ __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs 
 template <class T, bool kWhole>
 __global__ void __launch_bounds__(256) softmax_lay_out_kernel(const T *from, long long stride, long long rows, int columns, const int *labels, __nv_bfloat16 *to, long long to_stride, long long part)
 {
+    next_may_start();
+    wait_for_previous();
     constexpr int kWide = 16 / sizeof(T);
     const int per_row = (columns + 7) / 8;
     const long long all = rows * per_row;
@@ -646,6 +650,8 @@ template <class T>
 __global__ void __launch_bounds__(256) softmax_lay_out_both_kernel(const T *from, long long stride, long long rows, int columns, const int *labels, __nv_bfloat16 *to, long long to_stride, long long part,
                                                                    __nv_bfloat16 *turned, long long turned_stride, long long turned_part, bool whole)
 {
+    next_may_start();
+    wait_for_previous();
     using Out = typename std::conditional<sizeof(T) == 4, __nv_bfloat16, T>::type;
     constexpr int kParts = sizeof(T) == 4 ? 3 : 1, kWide = 16 / sizeof(T);
     __shared__ Out tile[kParts][64][72];                      // rows of 144 bytes: eight of them read as columns meet different banks
@@ -700,6 +706,8 @@ __global__ void __launch_bounds__(256) softmax_lay_out_both_kernel(const T *from
 __global__ void __launch_bounds__(256) softmax_rows_kernel(const void *labels, int labels_64, long long rows, long long number_of_labels, long long ignored, const float *gradients,
                                                            int gradients_step, float scale, int *out, float *factors, unsigned *largest)
 {
+    next_may_start();
+    wait_for_previous();
     const long long r = (long long)blockIdx.x * 256 + threadIdx.x;
     if (r >= rows) return;
     const long long l = index_at(labels, labels_64, r);
@@ -806,6 +814,8 @@ template <int kRows>
 __global__ void __launch_bounds__(1024) softmax_loss_kernel(const float2 *sums, const float *label_logit, const int *labels, long long rows, int parts, float scale, float *losses,
                                                             float *normalisers)
 {
+    next_may_start();
+    wait_for_previous();
     JoinSums s;
     long long row;
     if (!join_parts<JoinSums, kRows>(sums, nullptr, rows, parts, scale, s, row)) return;
@@ -818,6 +828,8 @@ __global__ void __launch_bounds__(1024) softmax_loss_kernel(const float2 *sums, 
 template <int kRows>
 __global__ void __launch_bounds__(1024) softmax_best_kernel(const float2 *sums, const int *best, long long rows, int parts, float scale, long long *labels, float *log_probabilities)
 {
+    next_may_start();
+    wait_for_previous();
     JoinBest s;
     long long row;
     if (!join_parts<JoinBest, kRows>(sums, best, rows, parts, scale, s, row)) return;
@@ -831,6 +843,8 @@ template <class T>
 __global__ void __launch_bounds__(256) softmax_finish_kernel(const float *partial, long long partial_stride, long long split_size, int splits, long long rows, int columns, const unsigned *out_scale, T *out,
                                                              bool whole)
 {
+    next_may_start();
+    wait_for_previous();
     const float factor = out_scale ? __uint_as_float(*out_scale) * (1.f / 16384.f) : 1.f;
     const int per_row = (columns + 3) / 4;
     const long long all = rows * per_row;
@@ -860,6 +874,8 @@ __global__ void __launch_bounds__(256) softmax_finish_kernel(const float *partia
 template <class T>
 __global__ void __launch_bounds__(256) softmax_turn_kernel(const float *partial, long long partial_stride, long long slice_size, const Product p, const Schedule schedule, const unsigned *out_scale, T *out)
 {
+    next_may_start();
+    wait_for_previous();
     __shared__ float tile[32][65];
     const int across = p.tile_columns / 64, t = blockIdx.x / (8 * across), strip = blockIdx.x / across % 8, part = blockIdx.x % across;
     int m, n;
@@ -921,7 +937,7 @@ int make_map(CUtensorMap *map, const Matrix &a, unsigned box_columns, unsigned b
     GTM_TRY(encode_tiled(&encode));
     const cuuint64_t size = type_bytes(a.type);
     const cuuint64_t sizes[3] = {(cuuint64_t)a.columns, (cuuint64_t)a.rows, (cuuint64_t)a.parts};
-    const cuuint64_t strides[2] = {(cuuint64_t)a.stride * size, (cuuint64_t)(a.parts > 1 ? a.part : a.stride * a.rows) * size};
+    const cuuint64_t strides[2] = {(cuuint64_t)a.stride * size, (cuuint64_t)(a.parts > 1 ? a.part : a.stride) * size};      // of one part: any
     const cuuint32_t box[3] = {box_columns, box_rows, 1}, steps[3] = {1, 1, 1};
     const CUtensorMapDataType kind = a.type == GTM_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : a.type == GTM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const CUresult r = encode(map, kind, 3, (void *)a.data, sizes, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1130,22 +1146,21 @@ int check_workspace(const char *what, const void *workspace, uint64_t bytes, uin
 }
 
 template <class T>
-void lay_out(const void *from, int64_t stride, int64_t rows, int64_t columns, const int *labels, void *to, int64_t ld, cudaStream_t stream)
+int lay_out(const void *from, int64_t stride, int64_t rows, int64_t columns, const int *labels, void *to, int64_t ld, cudaStream_t stream)
 {
     const int64_t blocks = std::min<int64_t>((rows * ((columns + 7) / 8) + 255) / 256, 148 * 16);
     const bool whole = aligned(from, stride * sizeof(T), 16) && columns % 8 == 0;
-    if (whole) softmax_lay_out_kernel<T, true><<<(unsigned)blocks, 256, 0, stream>>>((const T *)from, stride, rows, (int)columns, labels, (__nv_bfloat16 *)to, ld, rows * ld);
-    else softmax_lay_out_kernel<T, false><<<(unsigned)blocks, 256, 0, stream>>>((const T *)from, stride, rows, (int)columns, labels, (__nv_bfloat16 *)to, ld, rows * ld);
+    return launch_early(whole ? softmax_lay_out_kernel<T, true> : softmax_lay_out_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, stream, (const T *)from, (long long)stride, (long long)rows, (int)columns,
+                        labels, (__nv_bfloat16 *)to, (long long)ld, (long long)(rows * ld));
 }
 
 // A matrix as the kernels read it, laid out in the workspace where it is not so already.
 int operand_of(Matrix *out, int type, const void *data, int64_t stride, int64_t rows, int64_t columns, bool copy, const int *labels, void *to, int64_t ld, cudaStream_t stream)
 {
     if (copy) {
-        if (type == GTM_F32) lay_out<float>(data, stride, rows, columns, labels, to, ld, stream);
-        else if (type == GTM_BF16) lay_out<__nv_bfloat16>(data, stride, rows, columns, labels, to, ld, stream);
-        else lay_out<__half>(data, stride, rows, columns, labels, to, ld, stream);
-        GTM_CU(cudaGetLastError());
+        GTM_TRY(type == GTM_F32    ? lay_out<float>(data, stride, rows, columns, labels, to, ld, stream)
+                : type == GTM_BF16 ? lay_out<__nv_bfloat16>(data, stride, rows, columns, labels, to, ld, stream)
+                                   : lay_out<__half>(data, stride, rows, columns, labels, to, ld, stream));
         data = to;
     }
     *out = {data, rows, columns, ld, rows * ld, type == GTM_F32 ? 3 : 1, type == GTM_F16 ? GTM_F16 : GTM_BF16};
@@ -1157,27 +1172,23 @@ int lay_out_both(const Call &c, const int *labels, char *w, cudaStream_t stream)
 {
     const dim3 grid((unsigned)((c.examples + 63) / 64), (unsigned)((c.columns + 63) / 64));
     const bool whole = aligned(c.x, c.x_stride * sizeof(T), 16) && c.columns % 8 == 0;
-    softmax_lay_out_both_kernel<T><<<grid, 256, 0, stream>>>((const T *)c.x, c.x_stride, c.examples, (int)c.columns, labels, (__nv_bfloat16 *)(w + c.at_x), c.x_ld, c.examples * c.x_ld,
-                                                             (__nv_bfloat16 *)(w + c.at_turned), c.turned_ld, c.columns * c.turned_ld, whole);
-    GTM_CU(cudaGetLastError());
-    return GTM_OK;
+    return launch_early(softmax_lay_out_both_kernel<T>, grid, dim3(256), 0, stream, (const T *)c.x, (long long)c.x_stride, (long long)c.examples, (int)c.columns, labels, (__nv_bfloat16 *)(w + c.at_x),
+                        (long long)c.x_ld, (long long)(c.examples * c.x_ld), (__nv_bfloat16 *)(w + c.at_turned), (long long)c.turned_ld, (long long)(c.columns * c.turned_ld), whole);
 }
 
 template <class T>
 int finish_dw(const Call &c, const float *dw, int64_t rows, const unsigned *out_scale, void *out, cudaStream_t stream)
 {
     const unsigned blocks = (unsigned)std::min<int64_t>((rows * ((c.columns + 3) / 4) + 255) / 256, 148 * 16);
-    softmax_finish_kernel<T><<<blocks, 256, 0, stream>>>(dw, c.sums_ld, c.piece_labels * c.sums_ld, c.dw.splits(), rows, (int)c.columns, out_scale, (T *)out, c.columns % 4 == 0);
-    GTM_CU(cudaGetLastError());
-    return GTM_OK;
+    return launch_early(softmax_finish_kernel<T>, dim3(blocks), dim3(256), 0, stream, dw, (long long)c.sums_ld, (long long)(c.piece_labels * c.sums_ld), c.dw.splits(), (long long)rows, (int)c.columns, out_scale,
+                        (T *)out, c.columns % 4 == 0);
 }
 
 template <class T>
 int finish_dx(const Call &c, const float *dx, const unsigned *out_scale, void *out, cudaStream_t stream)
 {
-    softmax_turn_kernel<T><<<(unsigned)(c.dx.tiles() * 8 * (c.dx.tile_columns / 64)), 256, 0, stream>>>(dx, c.turned_ld, c.columns * c.turned_ld, c.dx, c.schedule, out_scale, (T *)out);
-    GTM_CU(cudaGetLastError());
-    return GTM_OK;
+    return launch_early(softmax_turn_kernel<T>, dim3((unsigned)(c.dx.tiles() * 8 * (c.dx.tile_columns / 64))), dim3(256), 0, stream, dx, (long long)c.turned_ld, (long long)(c.columns * c.turned_ld), c.dx, c.schedule,
+                        out_scale, (T *)out);
 }
 
 template <class T, int kExamples, bool kWhole>
@@ -1186,9 +1197,7 @@ int launch_few(const FewArgs &a, int blocks, cudaStream_t stream)
     const size_t shared = kExamples * round_up(a.columns, 256) * 4;
     const auto run = [&](auto kernel) -> int {
         GTM_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewShared));
-        kernel<<<blocks, kFewThreads, shared, stream>>>(a);
-        GTM_CU(cudaGetLastError());
-        return GTM_OK;
+        return launch_early(kernel, dim3(blocks), dim3(kFewThreads), shared, stream, a);
     };
     return a.best ? run(softmax_few_kernel<T, kExamples, kWhole, true>) : run(softmax_few_kernel<T, kExamples, kWhole, false>);
 }
@@ -1207,11 +1216,9 @@ int launch_few(const FewArgs &a, bool whole, int blocks, cudaStream_t stream)
 template <class Run>
 int by_rows(int64_t rows, Run run)
 {
-    if (rows <= 8) run(std::integral_constant<int, 1>(), (unsigned)rows);
-    else if (rows <= 148 * 8) run(std::integral_constant<int, 8>(), (unsigned)((rows + 7) / 8));
-    else run(std::integral_constant<int, 32>(), (unsigned)((rows + 31) / 32));
-    GTM_CU(cudaGetLastError());
-    return GTM_OK;
+    if (rows <= 8) return run(std::integral_constant<int, 1>(), dim3((unsigned)rows));
+    if (rows <= 148 * 8) return run(std::integral_constant<int, 8>(), dim3((unsigned)((rows + 7) / 8)));
+    return run(std::integral_constant<int, 32>(), dim3((unsigned)((rows + 31) / 32)));
 }
 
 // Loss (labels given) or most probable label.
@@ -1219,17 +1226,18 @@ int forward(Call &c, const void *labels, int labels_64, int64_t ignored, float s
 {
     int *rows = labels ? (int *)(w + c.at_rows) : nullptr;
     if (labels) {
-        softmax_rows_kernel<<<(unsigned)((c.examples + 255) / 256), 256, 0, stream>>>(labels, labels_64, c.examples, c.labels, ignored, nullptr, 0, scale, rows, nullptr, nullptr);
-        GTM_CU(cudaGetLastError());
+        GTM_TRY(launch_early(softmax_rows_kernel, dim3((unsigned)((c.examples + 255) / 256)), dim3(256), 0, stream, labels, labels_64, (long long)c.examples, (long long)c.labels, (long long)ignored,
+                             nullptr, 0, scale, rows, nullptr, nullptr));
     }
     float2 *sums = (float2 *)(w + c.at_sums);
     int *indices = (int *)(w + c.at_best);
     float *label_logit = (float *)(w + c.at_logit);
     const auto join = [&](int64_t first, int64_t n, int parts, float scale) {
-        return by_rows(n, [&](auto each, unsigned blocks) {
+        return by_rows(n, [&](auto each, dim3 blocks) -> int {
             constexpr int kRows = decltype(each)::value;
-            if (labels) softmax_loss_kernel<kRows><<<blocks, 1024, 0, stream>>>(sums, label_logit, rows + first, n, parts, scale, losses + first, normalisers + first);
-            else softmax_best_kernel<kRows><<<blocks, 1024, 0, stream>>>(sums, indices, n, parts, scale, (long long *)best + first, log_probabilities + first);
+            if (labels)
+                return launch_early(softmax_loss_kernel<kRows>, blocks, dim3(1024), 0, stream, sums, label_logit, rows + first, (long long)n, parts, scale, losses + first, normalisers + first);
+            return launch_early(softmax_best_kernel<kRows>, blocks, dim3(1024), 0, stream, sums, indices, (long long)n, parts, scale, (long long *)best + first, log_probabilities + first);
         });
     };
     if (c.few) {
@@ -1282,7 +1290,7 @@ extern "C" int gtm_softmax_workspace(int type, const void *features, int64_t exa
     GTM_TRY(check_call("gtm_softmax_workspace", c, 1.f));
     *bytes_out = 0;
     if (examples == 0) return GTM_OK;
-    if (few_labels(type, examples, labels, columns, c.gradient)) {
+    if (few_labels(examples, labels, columns, c.gradient)) {
         *bytes_out = few_labels_workspace(examples, labels, columns, c.gradient);
         return GTM_OK;
     }
@@ -1299,7 +1307,7 @@ extern "C" int gtm_softmax_loss(int device, void *cuda_stream, int type, const v
     GTM_TRY(check_call("gtm_softmax_loss", c, scale));
     if (examples == 0) return GTM_OK;
     if (!features || !weights || !labels || !losses || !normalisers) return fail(GTM_ERR_ARG, "gtm_softmax_loss: null array");
-    const bool few_ones = few_labels(type, examples, number_of_labels, columns, false);
+    const bool few_ones = few_labels(examples, number_of_labels, columns, false);
     if (!few_ones) {
         lay_out_workspace(c);
         GTM_TRY(check_workspace("gtm_softmax_loss", workspace, workspace_bytes, c.total));
@@ -1320,7 +1328,7 @@ extern "C" int gtm_softmax_predict(int device, void *cuda_stream, int type, cons
     GTM_TRY(check_call("gtm_softmax_predict", c, scale));
     if (examples == 0) return GTM_OK;
     if (!features || !weights || !labels_out || !log_probabilities_out) return fail(GTM_ERR_ARG, "gtm_softmax_predict: null array");
-    const bool few_ones = few_labels(type, examples, number_of_labels, columns, false);
+    const bool few_ones = few_labels(examples, number_of_labels, columns, false);
     if (!few_ones) {
         lay_out_workspace(c);
         GTM_TRY(check_workspace("gtm_softmax_predict", workspace, workspace_bytes, c.total));
@@ -1352,7 +1360,7 @@ extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type
         return GTM_OK;
     }
     if (!features || !weights || !labels || !normalisers || !gradients || !features_gradient) return fail(GTM_ERR_ARG, "gtm_softmax_loss_gradient: null array");
-    if (few_labels(type, examples, number_of_labels, columns, true)) {
+    if (few_labels(examples, number_of_labels, columns, true)) {
         GTM_TRY(check_workspace("gtm_softmax_loss_gradient", workspace, workspace_bytes, few_labels_workspace(examples, number_of_labels, columns, true)));
         const FewLabels few = {type, examples, number_of_labels, columns, features, weights, features_stride, weights_stride, labels, labels_64, ignore_label, scale};
         return few_labels_gradient(few, normalisers, gradients, gradients_step, features_gradient, weights_gradient, workspace, stream);
@@ -1364,8 +1372,8 @@ extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type
     float *factors = (float *)(w + c.at_factors);
     unsigned *largest = type == GTM_F16 ? (unsigned *)(w + c.at_largest) : nullptr;
     if (largest) GTM_CU(cudaMemsetAsync(largest, 0, 4, stream));
-    softmax_rows_kernel<<<(unsigned)((examples + 255) / 256), 256, 0, stream>>>(labels, labels_64, examples, number_of_labels, ignore_label, gradients, (int)gradients_step, scale, rows, factors, largest);
-    GTM_CU(cudaGetLastError());
+    GTM_TRY(launch_early(softmax_rows_kernel, dim3((unsigned)((examples + 255) / 256)), dim3(256), 0, stream, labels, labels_64, (long long)examples, (long long)number_of_labels, (long long)ignore_label,
+                         gradients, (int)gradients_step, scale, rows, factors, largest));
     GTM_TRY(type == GTM_F32 ? lay_out_both<float>(c, rows, w, stream) : type == GTM_BF16 ? lay_out_both<__nv_bfloat16>(c, rows, w, stream) : lay_out_both<__half>(c, rows, w, stream));
     const int held = type == GTM_F16 ? GTM_F16 : GTM_BF16;
     const Matrix x = {w + c.at_x, examples, columns, c.x_ld, examples * c.x_ld, c.parts, held}, turned = {w + c.at_turned, columns, examples, c.turned_ld, columns * c.turned_ld, c.parts, held};

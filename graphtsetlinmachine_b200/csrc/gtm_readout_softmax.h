@@ -17,7 +17,7 @@ struct FewLabels {
 };
 
 // Whether these kernels take a problem.
-bool few_labels(int type, int64_t examples, int64_t labels, int64_t columns, bool gradient);
+bool few_labels(int64_t examples, int64_t labels, int64_t columns, bool gradient);
 uint64_t few_labels_workspace(int64_t examples, int64_t labels, int64_t columns, bool gradient);
 int few_labels_loss(const FewLabels &p, float *losses, float *normalisers, cudaStream_t stream);
 int few_labels_predict(const FewLabels &p, int64_t *labels, float *log_probabilities, cudaStream_t stream);

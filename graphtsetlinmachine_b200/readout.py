@@ -19,7 +19,8 @@ import torch
 
 from . import _lib
 
-__all__ = ["embed", "embed_gradient", "softmax_loss", "softmax_loss_gradient", "softmax_predict", "adamw_state", "adamw_step", "ClauseReadout"]
+__all__ = ["embed", "embed_gradient", "softmax_loss", "softmax_loss_gradient", "softmax_predict", "softmax_failed", "adamw_state", "adamw_step",
+           "ClauseReadout"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _INDEX = {torch.int32: 0, torch.int64: 1}
@@ -217,6 +218,14 @@ def softmax_predict(features, weights, scale=1.0):
     return labels, log_probabilities
 
 
+def softmax_failed(device=0):
+    """Whether a wait inside a softmax kernel (ten seconds at most) ran out on the device since the last question: results since then are
+    not to be used.  Waits for the device."""
+    failed = C.c_int()
+    _lib.check(_lib.load().gtm_softmax_failed(int(device), C.byref(failed)))
+    return bool(failed.value)
+
+
 def _padded(sizes):
     return sum([-(-n // BLOCK) for n in sizes]) * BLOCK
 
@@ -292,6 +301,8 @@ def adamw_step(params, gradients, state, lr, betas=(0.9, 0.999), eps=1e-8, weigh
         device.index, _stream(device), len(params), counts, _TYPES[param_kind], param_ptrs, _TYPES[gradient_kind], gradient_ptrs, _TYPES[copy_kind], copy_ptrs,
         8 if narrow else 32, first.data_ptr(), second.data_ptr(), scales[0].data_ptr() if narrow else None, scales[1].data_ptr() if narrow else None,
         steps.data_ptr(), lr, betas[0], betas[1], eps, weight_decay, gradient_scale, seed))
+    # whoever has saved one of them for a backward pass learns that it is another now
+    torch.autograd.graph.increment_version(params if copies is None else params + list(copies))
 
 
 class ClauseReadout:
@@ -319,11 +330,16 @@ class ClauseReadout:
 
     def active_clauses(self, graphs):
         """(ids int32, offsets int64) of the clauses that are active for each graph, on the device: bags for ``embed``."""
-        outputs, _ = self.tm.transform(graphs)
-        _, clauses = np.nonzero(outputs)
-        offsets = np.zeros(outputs.shape[0] + 1, dtype=np.int64)
-        np.cumsum(np.count_nonzero(outputs, axis=1), out=offsets[1:])
-        return torch.from_numpy(clauses.astype(np.int32)).to(self.device), torch.from_numpy(offsets).to(self.device)
+        most = max(1, (1 << 28) // self.tm.number_of_clauses)       # graphs at a time: a clause output has four bytes
+        clauses, counts = [], []
+        for first in range(0, graphs.number_of_graphs, most):
+            piece = graphs if most >= graphs.number_of_graphs else graphs[first:min(first + most, graphs.number_of_graphs)]
+            outputs, _ = self.tm.transform(piece)
+            clauses.append(np.nonzero(outputs)[1].astype(np.int32))
+            counts.append(np.count_nonzero(outputs, axis=1))
+        offsets = np.zeros(graphs.number_of_graphs + 1, dtype=np.int64)
+        np.cumsum(np.concatenate(counts), out=offsets[1:])
+        return torch.from_numpy(np.concatenate(clauses)).to(self.device), torch.from_numpy(offsets).to(self.device)
 
     def _init(self, outputs):
         self.number_of_outputs = outputs

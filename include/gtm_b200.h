@@ -280,7 +280,7 @@ int gtm_softmax_predict(int device, void *cuda_stream, int type, const void *fea
                         int64_t number_of_labels, int64_t weights_stride, int64_t columns, float scale, int64_t *labels_out, float *log_probabilities_out,
                         void *workspace, uint64_t workspace_bytes);
 /* Waits for the device and tells whether a wait inside a softmax kernel ran out since the last call (*failed_out = 0 or 1, then cleared).  Such
- * waits are bounded at two seconds; results of a call in which one ran out are not to be used. */
+ * waits are bounded at ten seconds; results of a call in which one ran out are not to be used. */
 int gtm_softmax_failed(int device, int *failed_out);
 
 /* One AdamW step over a list of tensors, in place: with t = *steps + 1 (*steps, int64 in device memory, is then counted up), g = gradient *

@@ -602,3 +602,31 @@ def test_readout_learns_from_clauses(bits):
     assert np.array_equal(tm.score(graphs), sums)
     with pytest.raises(ValueError):
         head.fit(graphs, labels + 1, epochs=1, incremental=True)
+
+
+def test_saved_parameters_are_known_to_have_changed():
+    p = torch.ones(3, device="cuda", requires_grad=True)
+    saved = (p * p).sum()
+    with torch.no_grad():
+        readout.adamw_step([p], [torch.ones(3, device="cuda")], readout.adamw_state([p]), lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()
+    assert not readout.softmax_failed()
+
+
+def test_other_shapes_and_devices_are_refused():
+    x, w, labels = softmax_case(F32, 20, 16, 40)
+    _, n = readout.softmax_loss(x, w, labels)
+    one = torch.ones(1, device="cuda")
+    for call in (lambda: readout.softmax_loss(x.t(), w, labels), lambda: readout.softmax_loss(x, w[:, :8], labels), lambda: readout.softmax_loss(x, w, labels[:5]),
+                 lambda: readout.softmax_loss(x, w, labels, scale=-1.0), lambda: readout.softmax_loss(x, w, labels.cpu()), lambda: readout.softmax_loss(x, w[:0], labels),
+                 lambda: readout.softmax_loss_gradient(x, w, labels, n[:3], one), lambda: readout.softmax_loss_gradient(x, w, labels, n, torch.ones(2, device="cuda")),
+                 lambda: readout.embed(x, labels[::2]), lambda: readout.embed(x[0], labels), lambda: readout.embed(x, labels, labels[:0]),
+                 lambda: readout.embed_gradient(x, labels[:3], 5), lambda: readout.embed_gradient(x, labels, 0), lambda: readout.adamw_step([x], [w], readout.adamw_state([x]), 0.1),
+                 lambda: readout.adamw_step([x], [x.clone()], readout.adamw_state([w]), 0.1), lambda: readout.adamw_step([x], [x.clone()], readout.adamw_state([x]), 0.1, seed=-1)):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: readout.softmax_loss(x, w.half(), labels), lambda: readout.softmax_loss(x.double(), w.double(), labels), lambda: readout.softmax_loss(x, w, labels.float()),
+                 lambda: readout.adamw_step([x], [x.clone()], readout.adamw_state([x]), 0.1, copies=[x.clone()])):
+        with pytest.raises(TypeError):
+            call()
