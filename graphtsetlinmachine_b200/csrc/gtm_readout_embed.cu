@@ -93,12 +93,14 @@ __device__ __forceinline__ void accumulate(float2 (&acc)[(V + 1) / 2], const Pac
         for (int v = 0; v < V; v += 2) add2(acc[v / 2], to_float(p.v[v]), to_float(p.v[v + 1]));
 }
 
-// Four rows ahead at 28 warps an SM: 72 us for 819,200 rows of 256 bf16 in bags (5.8 TB/s, from L2); eight rows at 20 warps: 80.
+// Four rows ahead at 28 warps an SM, eight at 20: 72 us and 80 for 819,200 rows of 256 bf16 in bags of 200.  kLong: 64 us (6.6 TB/s, from L2)
+// and 45 for the gradient of 65,539 rows of 512 fp16 in segments of two; otherwise 72 and 33.
 constexpr int kGatherThreads = 128, kGatherBlocks = 7;
 
-// A lane has U runs of V columns next to each other, kLanes * V apart.
-template <class T, int V, int U, int kLanes>
-__global__ void __launch_bounds__(kGatherThreads, U == 1 ? kGatherBlocks : 4) gather_sum_kernel(const GatherArgs a)
+// A lane has U runs of V columns next to each other, kLanes * V apart.  kLong: segments of several rows, taken one after the other; otherwise rows
+// are loaded whatever their segments are, and each is asked for its own.  The order of the sums is the same.
+template <class T, int V, int U, int kLanes, bool kLong>
+__global__ void __launch_bounds__(kGatherThreads, U == 1 ? kGatherBlocks : 3) gather_sum_kernel(const GatherArgs a)
 {
     next_may_start();
     wait_for_previous();
@@ -193,44 +195,91 @@ __global__ void __launch_bounds__(kGatherThreads, U == 1 ? kGatherBlocks : 4) ga
         };
         enter(__shfl_sync(team, segment, 0, kLanes));
         begun = true;
-        if (n == kLanes && __all_sync(team, segment == now && row >= 0)) {
-            // all of one segment
+        if constexpr (kLong) {
+            // one segment after the other, kAhead rows at once
+            const int shift = (threadIdx.x & 31) / kLanes * kLanes, before = __shfl_up_sync(team, segment, 1, kLanes);
+            const unsigned changes = (__ballot_sync(team, lane > 0 && lane < n && segment != before) & team) >> shift;
+            const bool whole = __all_sync(team, row >= 0 || lane >= n);
+            for (int i = 0; i < n;) {
+                const unsigned later = changes & ~((2u << i) - 1);
+                const int j = later ? __ffs(later) - 1 : n;
+                enter(__shfl_sync(team, segment, i, kLanes));
 #pragma unroll 1
-            for (int i = 0; i < kLanes; i += kAhead) {
+                for (; whole && i + kAhead <= j; i += kAhead) {
+                    Pack<T, V> got[kAhead][U];
+#pragma unroll
+                    for (int k = 0; k < kAhead; k++) {
+                        const unsigned long long from = (unsigned long long)(unsigned)__shfl_sync(team, row, i + k, kLanes) * (unsigned)a.src_stride;
+#pragma unroll
+                        for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + from);
+                    }
+#pragma unroll
+                    for (int k = 0; k < kAhead; k++)
+#pragma unroll
+                        for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
+                }
+#pragma unroll 1
+                for (; i < j; i += kAhead) {
+                    Pack<T, V> got[kAhead][U];
+                    int which[kAhead];
+#pragma unroll
+                    for (int k = 0; k < kAhead; k++) {
+                        which[k] = __shfl_sync(team, row, i + k, kLanes);
+                        if (i + k >= j) which[k] = -1;
+                        if (which[k] >= 0)
+#pragma unroll
+                            for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + (unsigned long long)(unsigned)which[k] * (unsigned)a.src_stride);
+                    }
+#pragma unroll
+                    for (int k = 0; k < kAhead; k++) {
+                        if (which[k] >= 0)
+#pragma unroll
+                            for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
+                        bad |= which[k] == -2;
+                    }
+                }
+                i = j;
+            }
+        } else {
+            if (n == kLanes && __all_sync(team, segment == now && row >= 0)) {
+                // all of one segment
+#pragma unroll 1
+                for (int i = 0; i < kLanes; i += kAhead) {
+                    Pack<T, V> got[kAhead][U];
+#pragma unroll
+                    for (int k = 0; k < kAhead; k++) {
+                        const unsigned long long from = (unsigned long long)(unsigned)__shfl_sync(team, row, i + k, kLanes) * (unsigned)a.src_stride;
+#pragma unroll
+                        for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + from);
+                    }
+#pragma unroll
+                    for (int k = 0; k < kAhead; k++)
+#pragma unroll
+                        for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
+                }
+                continue;
+            }
+#pragma unroll 1
+            for (int i = 0; i < n; i += kAhead) {
                 Pack<T, V> got[kAhead][U];
 #pragma unroll
                 for (int k = 0; k < kAhead; k++) {
-                    const unsigned long long from = (unsigned long long)(unsigned)__shfl_sync(team, row, i + k, kLanes) * (unsigned)a.src_stride;
+                    // a position without a row reads the first one, and drops it
+                    const unsigned long long from = (unsigned long long)(unsigned)max(__shfl_sync(team, row, i + k, kLanes), 0) * (unsigned)a.src_stride;
+                    if (a.rows > 0)
 #pragma unroll
-                    for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + from);
+                        for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + from);
                 }
 #pragma unroll
-                for (int k = 0; k < kAhead; k++)
+                for (int k = 0; k < kAhead; k++) {
+                    const int next = __shfl_sync(team, segment, i + k, kLanes), which = __shfl_sync(team, row, i + k, kLanes);
+                    if (i + k >= n) continue;
+                    enter(next);
+                    if (which >= 0)
 #pragma unroll
-                    for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
-            }
-            continue;
-        }
-#pragma unroll 1
-        for (int i = 0; i < n; i += kAhead) {
-            Pack<T, V> got[kAhead][U];
-#pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                // a position without a row reads the first one, and drops it
-                const unsigned long long from = (unsigned long long)(unsigned)max(__shfl_sync(team, row, i + k, kLanes), 0) * (unsigned)a.src_stride;
-                if (a.rows > 0)
-#pragma unroll
-                    for (int u = 0; u < U; u++) got[k][u] = *(const Pack<T, V> *)(column[u] + from);
-            }
-#pragma unroll
-            for (int k = 0; k < kAhead; k++) {
-                const int next = __shfl_sync(team, segment, i + k, kLanes), which = __shfl_sync(team, row, i + k, kLanes);
-                if (i + k >= n) continue;
-                enter(next);
-                if (which >= 0)
-#pragma unroll
-                    for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
-                else bad |= which == -2;
+                        for (int u = 0; u < U; u++) accumulate<T, V>(acc[u], got[k][u]);
+                    else bad |= which == -2;
+                }
             }
         }
     }
@@ -332,10 +381,12 @@ GatherSpace gather_space(uint64_t at, int64_t positions, int64_t columns)
 template <class T, int V, int U, int kLanes>
 int launch_gather(const GatherArgs &a, cudaStream_t stream)
 {
+    constexpr int kLongRows = 8;         // rows of a segment, on the average
     constexpr int kWide = kLanes * V * U, kTeams = kGatherThreads / kLanes;
     const long long units = a.spans + (a.segments + kLanes - 1) / kLanes;
     const dim3 grid((unsigned)((units + kTeams - 1) / kTeams), (unsigned)((a.columns + kWide - 1) / kWide));
-    GTM_TRY(launch_early(gather_sum_kernel<T, V, U, kLanes>, grid, dim3(kGatherThreads), 0, stream, a));
+    const bool long_ones = a.positions >= a.segments * kLongRows;
+    GTM_TRY(launch_early(long_ones ? gather_sum_kernel<T, V, U, kLanes, true> : gather_sum_kernel<T, V, U, kLanes, false>, grid, dim3(kGatherThreads), 0, stream, a));
     if (a.spans > 1) GTM_TRY(launch_early(gather_join_kernel<T>, dim3((unsigned)((a.spans + 7) / 8), (unsigned)((a.columns + 127) / 128)), dim3(256), 0, stream, a));
     return GTM_OK;
 }
