@@ -16,6 +16,7 @@
 namespace gtm_readout {
 namespace {
 
+// What bounds a step in 32 bits is memory: 60 M fp32 parameters with bf16 gradients take 258 us, 6.0 TB/s of 26 bytes each.
 constexpr int kBlock = 256;                   // elements of a warp's turn, and of one 8-bit scale
 constexpr int kTensors = 512;                 // tensors of one launch: their table travels with the launch's arguments
 constexpr float kLeastScale = 1.1754943508222875e-38f, kLeastCode = 0.001953125f;
@@ -203,7 +204,9 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
 }
 
 // States of 8 bits.  The moments are computed operation by operation as in 32 bits: a last bit can decide between two codes, and with it what the states
-// are from then on.  The parameter is not among them: its quotient is the hardware's reciprocal (2^-23) in fused operations.
+// are from then on.  The parameter is not among them: its quotient is the hardware's reciprocal (2^-23) in fused operations.  What bounds it is
+// instructions, 85 an element, the root, the hash and the roundings being half of them: 592 us for 200 M bf16 parameters (3.4 TB/s).  Loading the next block
+// before the present one is worked on took 1,130 us: two registers for every one loaded left half as many warps.
 template <class P, class G>
 __global__ void __launch_bounds__(256, 4) adamw_narrow_kernel(const __grid_constant__ AdamArgs a)
 {
