@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kGatherThreads, U == 1 ? kGatherBlocks : 3) ga
     }
     // every lane's `base` is at or before its last position: any of them finds the next one's segment
     leave(last < a.positions && now >= 0 && segment_of(last) == now);
-    if (blockIdx.y == 0 && lane == 0) a.ends[unit] = ended;
+    if (blockIdx.y == 0 && lane == 0 && a.spans > 1) a.ends[unit] = ended;
 }
 
 // Segments of several spans: head and parts, added in the order of the list (7 us for 65,539 positions, bound by the way from one load to the next).  A warp has the segment that ends in its span (if one
@@ -373,8 +373,8 @@ struct GatherSpace {
 
 GatherSpace gather_space(uint64_t at, int64_t positions, int64_t columns)
 {
-    // of the shortest spans: a caller's workspace serves every element type
-    const uint64_t spans = (uint64_t)(positions + 31) / 32, sums = round_up(spans * partial_stride(columns) * 4, 256);
+    // of the shortest spans: a caller's workspace serves every element type.  What is one span needs none
+    const uint64_t spans = positions <= 128 ? 0 : (uint64_t)(positions + 31) / 32, sums = round_up(spans * partial_stride(columns) * 4, 256);
     return {at, at + sums, at + 2 * sums, at + 2 * sums + round_up(spans * 4, 256)};
 }
 
@@ -756,12 +756,13 @@ extern "C" int gtm_embed_gradient(int device, void *cuda_stream, int type, const
                                   float scale, void *table_gradient, int64_t rows, void *workspace, uint64_t workspace_bytes)
 {
     GTM_TRY(check_sizes("gtm_embed_gradient", type, rows, columns, number_of_ids, number_of_bags));
-    if (!table_gradient || (number_of_ids && (!ids || !gradient))) return fail(GTM_ERR_ARG, "gtm_embed_gradient: null array");
+    if (!table_gradient || (number_of_ids && (!offsets || number_of_bags) && (!ids || !gradient))) return fail(GTM_ERR_ARG, "gtm_embed_gradient: null array");
     if ((uintptr_t)gradient % type_bytes(type) || (uintptr_t)ids % (ids_64 ? 8 : 4) || (uintptr_t)offsets % (offsets_64 ? 8 : 4))
         return fail(GTM_ERR_ARG, "gtm_embed_gradient: an array does not start at a boundary of its elements");
     if (gradient_stride < 0 || gradient_stride >= kMostRows) return fail(GTM_ERR_ARG, "gtm_embed_gradient: row stride %lld of the gradient", (long long)gradient_stride);
     if ((uintptr_t)table_gradient % 16) return fail(GTM_ERR_ARG, "gtm_embed_gradient: the result does not start at a 16-byte boundary");
-    const GradientSpace space = gradient_space(number_of_ids, rows, columns);
+    const long long n = offsets && number_of_bags == 0 ? 0 : number_of_ids;          // no bag, no id
+    const GradientSpace space = gradient_space(n, rows, columns);
     if (workspace_bytes < space.total || !workspace || (uintptr_t)workspace % 16)
         return fail(GTM_ERR_ARG, "gtm_embed_gradient: workspace of %llu bytes, %llu needed (16-byte aligned)", (unsigned long long)workspace_bytes, (unsigned long long)space.total);
     DeviceGuard guard(device);
@@ -770,7 +771,6 @@ extern "C" int gtm_embed_gradient(int device, void *cuda_stream, int type, const
     char *w = (char *)workspace;
     uint2 *from = (uint2 *)(w + space.pairs[0]), *to = (uint2 *)(w + space.pairs[1]);
     unsigned *counts = (unsigned *)(w + space.counts);
-    const long long n = number_of_ids;
     if (n) {
         const unsigned tiles = (unsigned)space.tiles;
         const auto sort = [&](auto each) -> int {

@@ -1029,7 +1029,12 @@ Schedule together(const Product &first, const Product &second)
 
 int most_slices(const Schedule &s, const Product &p)
 {
-    if (p.tiles() > 1024) return std::min(kPairs, p.blocks / kLeastShare + 2);          // a bound
+    if (p.tiles() > 64) {
+        // a bound: by the smallest share that a pair has
+        long long least = (s.units - s.units_of_longer) / s.others;
+        if (least == 0 || (s.units_of_longer && s.units_of_longer / s.longer < least)) least = s.units_of_longer / s.longer;
+        return (int)std::min<long long>(kPairs, p.blocks / least + 2);
+    }
     int most = 1;
     for (int t = 0; t < p.tiles(); t++) most = std::max(most, s.slices(p.blocks, t));
     return most;
@@ -1385,7 +1390,7 @@ extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type
     Matrix wm;
     GTM_TRY(operand_of(&wm, type, weights, weights_stride, number_of_labels, columns, c.lay_out_w, nullptr, w + c.at_w, c.w_ld, stream));
     float *dx = (float *)(w + c.at_dx), *dw = (float *)(w + c.at_dw);
-    const int64_t size = (int64_t)type_bytes(type);
+    const int64_t size = (int64_t)type_bytes(type), x_bytes = examples * columns * 2 * c.parts;
     for (int64_t v = 0; v < number_of_labels; v += c.piece_labels) {
         const int64_t n = std::min(c.piece_labels, number_of_labels - v);
         const Matrix prob = {w + c.at_prob, examples, n, c.prob_ld, examples * c.prob_ld, c.parts, held};
@@ -1396,7 +1401,8 @@ extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type
             Launch l = {};
             Maps maps = {};
             Product &p = l.p[0] = product_of(examples, n, columns, c.products);
-            p.m_fast = 1, p.b_row = (int)v, p.type = type;
+            // x stays in L2 while the labels pass, or the piece's labels while the examples do
+            p.m_fast = x_bytes <= 64 << 20 || x_bytes <= n * columns * 2 * c.parts, p.b_row = (int)v, p.type = type;
             l.schedule = in_turn(p);
             l.scale = scale_of(p, columns, scale), l.labels = rows, l.first_label = (int)v, l.normalisers = normalisers, l.factors = factors, l.largest = largest;
             GTM_TRY(set_operands(maps, p, 0, x, piece, &prob));

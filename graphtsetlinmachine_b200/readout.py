@@ -37,37 +37,40 @@ def _cuda(name, t):
     return t
 
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and _cuda(name, t).device != device:
-            raise ValueError("%s lies on %s, the first argument on %s" % (name, t.device, device))
+def _device_of(name, t, device):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s is a torch tensor, not %s" % (name, type(t).__name__))
+    if t.device != device:
+        raise ValueError("%s lies on %s, the first argument on %s" % (name, t.device, device))
 
 
 def _matrix(name, t, dtype=None):
-    """Checks a matrix; returns its row stride in elements."""
-    _cuda(name, t)
+    """Checks a matrix; returns its rows, its columns and its row stride in elements."""
     if t.dim() != 2:
         raise ValueError("%s has %d dimensions instead of two" % (name, t.dim()))
     if t.dtype not in _TYPES or (dtype is not None and t.dtype != dtype):
         raise TypeError("%s is of %s: %s" % (name, t.dtype, dtype or "float32, bfloat16 and float16 are taken"))
-    if t.shape[1] == 0:
+    rows, columns = t.shape
+    if columns == 0:
         raise ValueError("%s has no columns" % name)
-    if t.stride(1) != 1 and t.shape[1] > 1:
-        raise ValueError("the elements of a row of %s lie %d apart: give it as %s.contiguous()" % (name, t.stride(1), name))
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    stride, step = t.stride()
+    if step != 1 and columns > 1:
+        raise ValueError("the elements of a row of %s lie %d apart: give it as %s.contiguous()" % (name, step, name))
+    return rows, columns, stride if rows > 1 else columns
 
 
-def _index(name, t, dim=1):
-    _cuda(name, t)
-    if t.dtype not in _INDEX:
+def _index(name, t, device, dim=1):
+    _device_of(name, t, device)
+    wide = _INDEX.get(t.dtype)
+    if wide is None:
         raise TypeError("%s is of %s: int32 and int64 are taken" % (name, t.dtype))
     if (dim is not None and t.dim() != dim) or not t.is_contiguous():
         raise ValueError("%s is not a contiguous tensor%s" % (name, "" if dim is None else " of %d dimension(s)" % dim))
-    return _INDEX[t.dtype]
+    return wide
 
 
-def _vector(name, t, size):
-    _cuda(name, t)
+def _vector(name, t, size, device):
+    _device_of(name, t, device)
     if t.dtype != torch.float32 or t.shape != (size,) or not t.is_contiguous():
         raise ValueError("%s is not a contiguous float32 tensor of %d elements" % (name, size))
 
@@ -80,15 +83,14 @@ def _workspace(size, device):
     return torch.empty(size, dtype=torch.uint8, device=device)
 
 
-def _bags(ids, offsets):
+def _bags(ids, offsets, device):
     """Checks ids and offsets: (wide ids, wide offsets, number of results, their leading shape)."""
-    wide = _index("ids", ids, None if offsets is None else 1)
     if offsets is None:
-        return wide, 0, ids.numel(), tuple(ids.shape)
-    wide_offsets = _index("offsets", offsets)
-    if offsets.numel() < 1:
+        return _index("ids", ids, device, None), 0, ids.numel(), tuple(ids.shape)
+    wide, wide_offsets, bags = _index("ids", ids, device), _index("offsets", offsets, device), offsets.shape[0] - 1
+    if bags < 0:
         raise ValueError("offsets has an element more than there are bags, so at least one")
-    return wide, wide_offsets, offsets.numel() - 1, (offsets.numel() - 1,)
+    return wide, wide_offsets, bags, (bags,)
 
 
 def embed(table, ids, offsets=None, scale=1.0):
@@ -97,23 +99,21 @@ def embed(table, ids, offsets=None, scale=1.0):
 
     A negative id is padding: a row of zeros, nothing in a bag.  An id beyond the table gives NaN.  ``offsets`` must not decrease;
     ids outside every bag are not used."""
-    stride = _matrix("table", table)
-    device = table.device
-    _same_device(device, ids=ids, offsets=offsets)
-    wide, wide_offsets, count, shape = _bags(ids, offsets)
-    rows, columns = table.shape
+    device = _cuda("table", table).device
+    rows, columns, stride = _matrix("table", table)
+    wide, wide_offsets, count, shape = _bags(ids, offsets, device)
+    number = ids.numel()
     if rows == 0:
         raise ValueError("table has no rows")
     lib = _lib.load()
     out = torch.empty(shape + (columns,), dtype=table.dtype, device=device)
     workspace, size = None, 0
-    if offsets is not None:
+    if offsets is not None and number > 128:
         need = C.c_uint64()
-        _lib.check(lib.gtm_embed_workspace(ids.numel(), columns, 1, C.byref(need)))
+        _lib.check(lib.gtm_embed_workspace(number, columns, 1, C.byref(need)))
         size = need.value
-        if size:
-            workspace = _workspace(size, device)
-    _lib.check(lib.gtm_embed(device.index, _stream(device), _TYPES[table.dtype], table.data_ptr(), rows, columns, stride, ids.data_ptr(), wide, ids.numel(),
+        workspace = _workspace(size, device)
+    _lib.check(lib.gtm_embed(device.index, _stream(device), _TYPES[table.dtype], table.data_ptr(), rows, columns, stride, ids.data_ptr(), wide, number,
                              None if offsets is None else offsets.data_ptr(), wide_offsets, count, scale, out.data_ptr(),
                              None if workspace is None else workspace.data_ptr(), size))
     return out
@@ -123,21 +123,18 @@ def embed_gradient(gradient, ids, rows, offsets=None, scale=1.0):
     """Gradient ``[rows, columns]`` of the table of ``embed(table, ids, offsets, scale)`` from the ``gradient`` of its result.
 
     Each row is summed in 32 bits in the order of ``ids``: results do not change from run to run."""
-    _cuda("gradient", gradient)
-    device = gradient.device
-    _same_device(device, ids=ids, offsets=offsets)
-    wide, wide_offsets, count, shape = _bags(ids, offsets)
+    device = _cuda("gradient", gradient).device
+    wide, wide_offsets, count, shape = _bags(ids, offsets, device)
     if gradient.dim() < 1 or tuple(gradient.shape[:-1]) != shape:
         raise ValueError("gradient has shape %s, the result of embed has %s rows" % (tuple(gradient.shape), shape))
     if gradient.dim() != 2:
         if not gradient.is_contiguous():
             raise ValueError("gradient is not contiguous: only one of two dimensions may have a row stride")
         gradient = gradient.view(count, gradient.shape[-1])
-    stride = _matrix("gradient", gradient)
+    _, columns, stride = _matrix("gradient", gradient)
     rows = int(rows)
     if rows < 1:
         raise ValueError("a table of %d rows" % rows)
-    columns = gradient.shape[1]
     lib = _lib.load()
     out = torch.empty((rows, columns), dtype=gradient.dtype, device=device)
     need = C.c_uint64()
@@ -150,24 +147,34 @@ def embed_gradient(gradient, ids, rows, offsets=None, scale=1.0):
 
 
 def _softmax_arguments(features, weights, scale, gradient):
-    """Checks features and weights: (library, device, the arguments that describe them, workspace or None, its size)."""
-    x_stride = _matrix("features", features)
-    w_stride = _matrix("weights", weights, features.dtype)
-    device = features.device
-    _same_device(device, weights=weights)
-    if features.shape[1] != weights.shape[1]:
-        raise ValueError("features have %d columns, weights %d" % (features.shape[1], weights.shape[1]))
-    if weights.shape[0] == 0:
+    """Checks features and weights: (library, device, the arguments that describe them, workspace or None, its address, its size)."""
+    device = _cuda("features", features).device
+    _device_of("weights", weights, device)
+    n, d, x_stride = _matrix("features", features)
+    v, columns, w_stride = _matrix("weights", weights, features.dtype)
+    if d != columns:
+        raise ValueError("features have %d columns, weights %d" % (d, columns))
+    if v == 0:
         raise ValueError("weights has no rows: there is no label")
     if not 0.0 < scale < float("inf"):
         raise ValueError("scale %r is not above zero and finite" % scale)
     lib = _lib.load()
-    kind, n, v, d = _TYPES[features.dtype], features.shape[0], weights.shape[0], features.shape[1]
-    x, w = features.data_ptr(), weights.data_ptr()
-    need = C.c_uint64()
-    _lib.check(lib.gtm_softmax_workspace(kind, x, n, x_stride, w, v, w_stride, d, gradient, C.byref(need)))
-    workspace = _workspace(max(need.value, 1), device)
-    return lib, device, (device.index, _stream(device), kind, x, n, x_stride, w, v, w_stride, d), workspace, need.value
+    kind, x, w = _TYPES[features.dtype], features.data_ptr(), weights.data_ptr()
+    workspace, address, size = None, None, 0
+    if gradient or v > 32 or v * d > 24576 or n > 65536:
+        need = C.c_uint64()
+        _lib.check(lib.gtm_softmax_workspace(kind, x, n, x_stride, w, v, w_stride, d, gradient, C.byref(need)))
+        size = need.value
+        workspace = _workspace(max(size, 1), device)
+        address = workspace.data_ptr()
+    return lib, device, (device.index, _stream(device), kind, x, n, x_stride, w, v, w_stride, d), workspace, address, size
+
+
+def _wanted(labels, n, device):
+    wide = _index("labels", labels, device)
+    if labels.shape[0] != n:
+        raise ValueError("%d labels for %d examples" % (labels.shape[0], n))
+    return wide
 
 
 def softmax_loss(features, weights, labels, scale=1.0, ignore_label=-1):
@@ -176,14 +183,12 @@ def softmax_loss(features, weights, labels, scale=1.0, ignore_label=-1):
     exponentials.  ``scale`` is above zero.
 
     An example whose label is ``ignore_label`` has loss zero; the loss of a label that there is not is NaN."""
-    lib, device, what, workspace, size = _softmax_arguments(features, weights, scale, 0)
-    _same_device(device, labels=labels)
-    wide, n = _index("labels", labels), features.shape[0]
-    if labels.numel() != n:
-        raise ValueError("%d labels for %d examples" % (labels.numel(), n))
+    lib, device, what, workspace, address, size = _softmax_arguments(features, weights, scale, 0)
+    n = what[4]
+    wide = _wanted(labels, n, device)
     losses = torch.empty(n, dtype=torch.float32, device=device)
     normalisers = torch.empty(n, dtype=torch.float32, device=device)
-    _lib.check(lib.gtm_softmax_loss(*what, labels.data_ptr(), wide, ignore_label, scale, losses.data_ptr(), normalisers.data_ptr(), workspace.data_ptr(), size))
+    _lib.check(lib.gtm_softmax_loss(*what, labels.data_ptr(), wide, ignore_label, scale, losses.data_ptr(), normalisers.data_ptr(), address, size))
     return losses, normalisers
 
 
@@ -192,29 +197,28 @@ def softmax_loss_gradient(features, weights, labels, normalisers, gradients, sca
     that call gave; ``gradients``: dL/dlosses, float32 of one element per example or of one element for all (1 / n for the mean).
 
     An ignored example's gradient is zero, and it adds nothing to the weights' gradient, whatever its features hold."""
-    lib, device, what, workspace, size = _softmax_arguments(features, weights, scale, 1)
-    _same_device(device, labels=labels, normalisers=normalisers, gradients=gradients)
-    wide, n = _index("labels", labels), features.shape[0]
-    if labels.numel() != n:
-        raise ValueError("%d labels for %d examples" % (labels.numel(), n))
-    _vector("normalisers", normalisers, n)
+    lib, device, what, workspace, address, size = _softmax_arguments(features, weights, scale, 1)
+    n = what[4]
+    wide = _wanted(labels, n, device)
+    _vector("normalisers", normalisers, n, device)
+    _device_of("gradients", gradients, device)
     if gradients.dtype != torch.float32 or gradients.dim() > 1 or gradients.numel() not in (1, n) or not gradients.is_contiguous():
         raise ValueError("gradients is not a contiguous float32 tensor of one element, or of one for each of %d examples" % n)
     features_gradient = torch.empty(features.shape, dtype=features.dtype, device=device)
     weights_gradient = torch.empty(weights.shape, dtype=weights.dtype, device=device)
     _lib.check(lib.gtm_softmax_loss_gradient(*what, labels.data_ptr(), wide, ignore_label, scale, normalisers.data_ptr(), gradients.data_ptr(),
                                              1 if gradients.numel() == n else 0, features_gradient.data_ptr(), weights_gradient.data_ptr(),
-                                             workspace.data_ptr(), size))
+                                             address, size))
     return features_gradient, weights_gradient
 
 
 def softmax_predict(features, weights, scale=1.0):
     """(labels int64, log probabilities float32): each example's most probable label under logits ``scale * features @ weights.T``,
     the lowest of equal ones.  -1 and NaN where an example's logits are not numbers."""
-    lib, device, what, workspace, size = _softmax_arguments(features, weights, scale, 0)
-    labels = torch.empty(features.shape[0], dtype=torch.int64, device=device)
-    log_probabilities = torch.empty(features.shape[0], dtype=torch.float32, device=device)
-    _lib.check(lib.gtm_softmax_predict(*what, scale, labels.data_ptr(), log_probabilities.data_ptr(), workspace.data_ptr(), size))
+    lib, device, what, workspace, address, size = _softmax_arguments(features, weights, scale, 0)
+    labels = torch.empty(what[4], dtype=torch.int64, device=device)
+    log_probabilities = torch.empty(what[4], dtype=torch.float32, device=device)
+    _lib.check(lib.gtm_softmax_predict(*what, scale, labels.data_ptr(), log_probabilities.data_ptr(), address, size))
     return labels, log_probabilities
 
 

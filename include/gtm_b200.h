@@ -248,7 +248,8 @@ typedef enum gtm_type { GTM_F32 = 0, GTM_BF16 = 1, GTM_F16 = 2 } gtm_type;
 
 /* Embedding lookup: out[b] = scale * sum of table[ids[i]] over offsets[b] <= i < offsets[b+1]; with offsets NULL one row per id
  * (number_of_bags is ignored).  offsets must not decrease; they are kept within 0..number_of_ids.  A negative id is padding and adds
- * nothing; the result of an id that the table does not have is NaN.  Bags may be empty: zeros. */
+ * nothing; the result of an id that the table does not have is NaN.  Bags may be empty: zeros.  Without bags, and with up to 128 ids in bags, no
+ * workspace is needed (NULL). */
 int gtm_embed_workspace(int64_t number_of_ids, int64_t columns, int bags, uint64_t *bytes_out);
 int gtm_embed(int device, void *cuda_stream, int type, const void *table, int64_t rows, int64_t columns, int64_t row_stride, const void *ids, int ids_64,
               int64_t number_of_ids, const void *offsets, int offsets_64, int64_t number_of_bags, float scale, void *out, void *workspace,
@@ -265,6 +266,7 @@ int gtm_embed_gradient(int device, void *cuda_stream, int type, const void *grad
  * loss of a label that there is not is NaN.
  * The gradient takes gradients[n * gradients_step] = dL/dlosses[n] (step 0: one value for all) and the normalisers of the forward
  * call.  Ignored examples have gradient zero, whatever their features hold.
+ * With up to 32 labels whose weights take up to 96 KB as floats, and up to 2^16 examples, the loss and the prediction need no workspace (NULL).
  * gtm_softmax_predict gives the most probable label, the lowest of equal ones, and its log probability; -1 and NaN where the logits are
  * not numbers. */
 int gtm_softmax_workspace(int type, const void *features, int64_t examples, int64_t features_stride, const void *weights, int64_t labels,

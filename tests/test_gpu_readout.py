@@ -117,6 +117,12 @@ def test_embed_gradient_sorts_any_table(rows):
     assert torch.equal(readout.embed_gradient(gradient, ids, rows).double(), want)
 
 
+def test_embed_gradient_without_bags_to_take_from():
+    got = readout.embed_gradient(torch.empty(0, 4, device="cuda"), torch.zeros(300, dtype=torch.int64, device="cuda"), 6, torch.zeros(1, dtype=torch.int64, device="cuda"))
+    assert torch.equal(got, torch.zeros(6, 4, device="cuda"))
+    assert readout.embed(got, torch.zeros(300, dtype=torch.int64, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")).shape == (0, 4)
+
+
 def test_embed_gradient_is_the_same_every_time():
     gen = generator(1)
     ids = torch.randint(50, (30000,), generator=gen, device="cuda")
