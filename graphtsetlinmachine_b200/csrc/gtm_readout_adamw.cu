@@ -18,7 +18,7 @@ namespace {
 
 // What bounds a step in 32 bits is memory: 60 M fp32 parameters with bf16 gradients take 258 us, 6.0 TB/s of 26 bytes each.
 constexpr int kBlock = 256;                   // elements of a warp's turn, and of one 8-bit scale
-constexpr int kTensors = 512;                 // tensors of one launch: their table travels with the launch's arguments
+constexpr int kTensors = 512, kFewTensors = 16;  // tensors of one launch, whose table travels with its arguments: a long one (20 KB) or a short one
 constexpr float kLeastScale = 1.1754943508222875e-38f, kLeastCode = 0.001953125f;
 
 struct AdamTensor {
@@ -28,7 +28,7 @@ struct AdamTensor {
     long long count, block;                   // first block of the flat arrays
 };
 
-struct AdamArgs {
+struct AdamHead {
     float b1, other1, b2, other2, decay, eps, gradient_scale;
     double lr, beta1, beta2;
     const long long *steps;                   // steps taken before this one
@@ -37,9 +37,13 @@ struct AdamArgs {
     unsigned seed;
     int tensors, copy_type;
     long long blocks;                         // of this launch
-    AdamTensor t[kTensors];
 };
-static_assert(sizeof(AdamArgs) <= 32764, "kernel arguments");
+
+template <int kMost>
+struct AdamArgs : AdamHead {
+    AdamTensor t[kMost];
+};
+static_assert(sizeof(AdamArgs<kTensors>) <= 32764, "kernel arguments");
 
 // Finaliser of MurmurHash3 (A. Appleby).
 __device__ __forceinline__ unsigned mix(unsigned x)
@@ -125,7 +129,7 @@ struct StepConstants {
     unsigned key;
 };
 
-__device__ __forceinline__ StepConstants step_constants(const AdamArgs &a)
+__device__ __forceinline__ StepConstants step_constants(const AdamHead &a)
 {
     __shared__ StepConstants c;
     if (threadIdx.x == 0) {
@@ -148,7 +152,7 @@ __device__ __forceinline__ bool is_whole(const AdamTensor &t, long long i)
 
 // The parameter as it is held, and its copy.
 template <class P, int N>
-__device__ __forceinline__ void store_param(const AdamArgs &a, const AdamTensor &t, long long i, bool whole, float (&p)[N])
+__device__ __forceinline__ void store_param(const AdamHead &a, const AdamTensor &t, long long i, bool whole, float (&p)[N])
 {
     store((P *)t.param, i, t.count, whole, p);
     if (!t.copy) return;
@@ -158,8 +162,8 @@ __device__ __forceinline__ void store_param(const AdamArgs &a, const AdamTensor 
     else store((__half *)t.copy, i, t.count, whole, p);
 }
 
-template <class P, class G>
-__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamArgs a)
+template <class P, class G, int kMost>
+__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamArgs<kMost> a)
 {
     next_may_start();
     wait_for_previous();
@@ -207,8 +211,8 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
 // are from then on.  The parameter is not among them: its quotient is the hardware's reciprocal (2^-23) in fused operations.  What bounds it is
 // instructions, 85 an element, the root, the hash and the roundings being half of them: 592 us for 200 M bf16 parameters (3.4 TB/s).  Loading the next block
 // before the present one is worked on took 1,130 us: two registers for every one loaded left half as many warps.
-template <class P, class G>
-__global__ void __launch_bounds__(256, 4) adamw_narrow_kernel(const __grid_constant__ AdamArgs a)
+template <class P, class G, int kMost>
+__global__ void __launch_bounds__(256, 4) adamw_narrow_kernel(const __grid_constant__ AdamArgs<kMost> a)
 {
     next_may_start();
     wait_for_previous();
@@ -296,23 +300,47 @@ __global__ void adamw_count_kernel(long long *steps)
     *steps += 1;
 }
 
-template <class P, class G>
-int launch(const AdamArgs &a, bool narrow, cudaStream_t stream)
+template <class P, class G, int kMost>
+int launch(const AdamArgs<kMost> &a, bool narrow, cudaStream_t stream)
 {
     int device = 0, sms = 0;
     GTM_CU(cudaGetDevice(&device));
     GTM_CU(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
     const long long want = (a.blocks + 7) / 8, most = (long long)sms * 8;
     const unsigned grid = (unsigned)(want < most ? want : most);
-    return launch_early(narrow ? adamw_narrow_kernel<P, G> : adamw_kernel<P, G>, dim3(grid), dim3(256), 0, stream, a);
+    return launch_early(narrow ? adamw_narrow_kernel<P, G, kMost> : adamw_kernel<P, G, kMost>, dim3(grid), dim3(256), 0, stream, a);
 }
 
-template <class P>
-int launch(const AdamArgs &a, int gradient_type, bool narrow, cudaStream_t stream)
+template <class P, int kMost>
+int launch(const AdamArgs<kMost> &a, int gradient_type, bool narrow, cudaStream_t stream)
 {
     return gradient_type == GTM_F32    ? launch<P, float>(a, narrow, stream)
            : gradient_type == GTM_BF16 ? launch<P, __nv_bfloat16>(a, narrow, stream)
                                        : launch<P, __half>(a, narrow, stream);
+}
+
+// All tensors of a step, kMost of them at a time.
+template <int kMost>
+int launch_all(const AdamHead &head, int64_t number_of_tensors, const int64_t *counts, int param_type, const void *const *params, int gradient_type, const void *const *gradients,
+               const void *const *copies, bool narrow, cudaStream_t stream)
+{
+    AdamArgs<kMost> a;
+    static_cast<AdamHead &>(a) = head;
+    long long block = 0;
+    for (int64_t i = 0; i < number_of_tensors;) {
+        a.tensors = 0, a.blocks = 0;
+        for (; i < number_of_tensors && a.tensors < kMost; i++) {
+            if (counts[i] == 0) continue;
+            a.t[a.tensors++] = {(void *)params[i], gradients[i], copies ? (void *)copies[i] : nullptr, counts[i], block};
+            const long long blocks = (counts[i] + kBlock - 1) / kBlock;
+            block += blocks, a.blocks += blocks;
+        }
+        if (a.tensors == 0) break;
+        GTM_TRY(param_type == GTM_F32    ? launch<float>(a, gradient_type, narrow, stream)
+                : param_type == GTM_BF16 ? launch<__nv_bfloat16>(a, gradient_type, narrow, stream)
+                                         : launch<__half>(a, gradient_type, narrow, stream));
+    }
+    return GTM_OK;
 }
 
 }  // namespace
@@ -347,24 +375,12 @@ extern "C" int gtm_adamw_step(int device, void *cuda_stream, int64_t number_of_t
     DeviceGuard guard(device);
     GTM_TRY(guard.status);
     cudaStream_t stream = (cudaStream_t)cuda_stream;
-    AdamArgs a;
+    AdamHead a = {};
     a.b1 = (float)beta1, a.other1 = (float)(1 - beta1), a.b2 = (float)beta2, a.other2 = (float)(1 - beta2);
     a.decay = (float)(1 - lr * weight_decay), a.eps = (float)eps, a.gradient_scale = (float)gradient_scale;
     a.lr = lr, a.beta1 = beta1, a.beta2 = beta2, a.steps = (const long long *)steps, a.seed = seed;
     a.first = first, a.second = second, a.first_scales = first_scales, a.second_scales = second_scales, a.copy_type = copy_type;
-    long long block = 0;
-    for (int64_t i = 0; i < number_of_tensors;) {
-        a.tensors = 0, a.blocks = 0;
-        for (; i < number_of_tensors && a.tensors < kTensors; i++) {
-            if (counts[i] == 0) continue;
-            a.t[a.tensors++] = {(void *)params[i], gradients[i], copies ? (void *)copies[i] : nullptr, counts[i], block};
-            const long long blocks = (counts[i] + kBlock - 1) / kBlock;
-            block += blocks, a.blocks += blocks;
-        }
-        if (a.tensors == 0) break;
-        GTM_TRY(param_type == GTM_F32    ? launch<float>(a, gradient_type, narrow, stream)
-                : param_type == GTM_BF16 ? launch<__nv_bfloat16>(a, gradient_type, narrow, stream)
-                                         : launch<__half>(a, gradient_type, narrow, stream));
-    }
+    GTM_TRY(number_of_tensors <= kFewTensors ? launch_all<kFewTensors>(a, number_of_tensors, counts, param_type, params, gradient_type, gradients, copies, narrow, stream)
+                                             : launch_all<kTensors>(a, number_of_tensors, counts, param_type, params, gradient_type, gradients, copies, narrow, stream));
     return launch_early(adamw_count_kernel, dim3(1), dim3(1), 0, stream, (long long *)steps);
 }

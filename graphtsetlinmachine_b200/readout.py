@@ -12,6 +12,7 @@ Matrices are float32, bfloat16 or float16 with any row stride and elements next 
 another order is refused, not copied.
 """
 
+import array
 import ctypes as C
 
 import numpy as np
@@ -254,20 +255,26 @@ def adamw_state(params, state_bits=32):
 
 
 def _pointers(name, tensors, shapes, device):
-    """Data pointers of a list of contiguous tensors of one type on one device, of the given shapes, and that type."""
-    for i, t in enumerate(tensors):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError("%s[%d] is a torch tensor, not %s" % (name, i, type(t).__name__))
-    kind = tensors[0].dtype
+    """Data pointers of a list of contiguous tensors of one type on one device, of the given shapes (an array of integers), and that type."""
+    count, index = len(tensors), device.index
+    try:
+        kind = tensors[0].dtype
+        # lists are compared as a whole; which tensor it is matters when they differ
+        same = ([t.dtype for t in tensors] == [kind] * count and [t.get_device() for t in tensors] == [index] * count
+                and all([t.is_contiguous() for t in tensors]) and [t.shape for t in tensors] == shapes)
+    except AttributeError:
+        raise TypeError("%s is a list of torch tensors" % name) from None
     if kind not in _TYPES:
         raise TypeError("%s[0] is of %s: float32, bfloat16 and float16 are taken" % (name, kind))
-    # lists are compared as a whole; which tensor it is matters when they differ
-    if ([t.dtype for t in tensors] != [kind] * len(tensors) or [t.device for t in tensors] != [device] * len(tensors)
-            or not all([t.is_contiguous() for t in tensors]) or [t.shape for t in tensors] != shapes):
+    if not same:
         for i, t in enumerate(tensors):
             if t.dtype != kind or t.device != device or not t.is_contiguous() or t.shape != shapes[i]:
                 raise ValueError("%s[%d] is not a contiguous %s tensor on %s of the parameter's shape" % (name, i, kind, device))
-    return (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors]), kind
+    return array.array("Q", [t.data_ptr() for t in tensors]), kind
+
+
+def _address(a):
+    return None if a is None else a.buffer_info()[0]
 
 
 def adamw_step(params, gradients, state, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, gradient_scale=1.0, copies=None, seed=0):
@@ -288,7 +295,7 @@ def adamw_step(params, gradients, state, lr, betas=(0.9, 0.999), eps=1e-8, weigh
     copy_ptrs, copy_kind = (None, torch.bfloat16) if copies is None else _pointers("copies", list(copies), shapes, device)
     if copy_kind == torch.float32:
         raise TypeError("copies are bfloat16 or float16")
-    counts = (C.c_int64 * len(params))(*sizes)
+    counts = array.array("q", sizes)
     total = _padded(sizes)
     first, second, steps = state["first"], state["second"], state["steps"]
     narrow = first.dtype == torch.float8_e4m3fn
@@ -302,7 +309,8 @@ def adamw_step(params, gradients, state, lr, betas=(0.9, 0.999), eps=1e-8, weigh
     if not 0 <= seed < 1 << 32:
         raise ValueError("seed %r is not within 0 to 2^32 - 1" % (seed,))
     _lib.check(_lib.load().gtm_adamw_step(
-        device.index, _stream(device), len(params), counts, _TYPES[param_kind], param_ptrs, _TYPES[gradient_kind], gradient_ptrs, _TYPES[copy_kind], copy_ptrs,
+        device.index, _stream(device), len(params), _address(counts), _TYPES[param_kind], _address(param_ptrs), _TYPES[gradient_kind], _address(gradient_ptrs),
+        _TYPES[copy_kind], _address(copy_ptrs),
         8 if narrow else 32, first.data_ptr(), second.data_ptr(), scales[0].data_ptr() if narrow else None, scales[1].data_ptr() if narrow else None,
         steps.data_ptr(), lr, betas[0], betas[1], eps, weight_decay, gradient_scale, seed))
     # whoever has saved one of them for a backward pass learns that it is another now
