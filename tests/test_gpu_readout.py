@@ -216,7 +216,7 @@ def check_gradient(x, w, labels, normalisers, gradients, scale, ignored=-1):
     return dx, dw
 
 
-SIZES = [(1, 1, 1), (1, 64, 10), (2, 7, 2), (60, 64, 10), (129, 65, 129), (256, 128, 256), (257, 200, 257), (300, 520, 1000), (33, 1024, 5001), (1000, 72, 300), (2100, 16, 40), (5000, 33, 7), (700, 300, 32), (3, 64, 33), (5, 1000, 513), (8, 40, 4000)]
+SIZES = [(1, 1, 1), (1, 64, 10), (2, 7, 2), (60, 64, 10), (129, 65, 129), (256, 128, 256), (257, 200, 257), (300, 520, 1000), (33, 1024, 5001), (1000, 72, 300), (2100, 16, 40), (5000, 33, 7), (700, 300, 32), (3, 64, 33), (5, 1000, 513), (8, 40, 4000), (64, 130, 700), (65, 130, 700), (17, 2000, 333), (40, 8, 20000)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -235,6 +235,13 @@ def test_softmax_in_pieces_of_the_labels(kind):
     x, w, labels = softmax_case(kind, n, 24, 9001)
     normalisers = check_loss(x, w, labels, 1.0)
     check_gradient(x, w, labels, normalisers, torch.full((n,), 1.0 / n, device="cuda"), 1.0)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_softmax_of_few_examples_in_pieces_of_the_labels(kind):
+    x, w, labels = softmax_case(kind, 20, 8, (1 << 20) + 5000)
+    normalisers = check_loss(x, w, labels, 1.0)
+    check_gradient(x, w, labels, normalisers, torch.full((20,), 0.05, device="cuda"), 1.0)
 
 
 @pytest.mark.parametrize("kind", TYPES)
