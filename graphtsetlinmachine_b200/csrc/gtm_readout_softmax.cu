@@ -8,7 +8,7 @@
 // the piece goes to the workspace in the operands' 16-bit type, and two products use it.  All products are one kernel on
 // tcgen05 over pairs of thread blocks: tiles of 256 x 256 (or 128), operands by TMA through a ring in shared memory, sums in tensor
 // memory, two tiles deep, so that a tile's epilogue runs under the next tile's products; results leave by TMA too.  dw and dx of a piece are one
-// launch: dw's tiles go round, and dx's work fills up what is left of the last round.  For up to four examples (eight in 32 bits) the forward
+// launch: dw's tiles go round, and dx's work fills up what is left of the last round.  For up to two examples (eight in 32 bits) the forward
 // pass is a kernel of plain dot products, whose time is that of reading w.
 //
 // 16-bit inputs are multiplied as they are, with sums in 32 bits.  32-bit inputs are split into three bf16 parts (24 bits of fraction),
@@ -493,11 +493,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
     if (warp == 2) tmem_free(tmem, 512);
 }
 
-// The forward pass for few examples, whose time is that of reading the weights (48 us for one example and 131,072 x 1,024 bf16, 5.6 TB/s; the product kernel
-// takes 87, most of its rows being outside of the matrix; at 16 examples that one takes 62 and this one would take 250): dot products in 32 bits, four rows of weights in a warp at
-// a time, of every lane 16 bytes (or, where rows start anywhere, an element).  A lane keeps the statistics of one of the four rows' products with one example;
-// a block leaves one part.
-constexpr int kFewRows = 4, kFewThreads = 256;
+// The forward pass for few examples, whose time is that of reading the weights.  A whole pass over 131,072 x 1,024 bf16 takes 52 us for one example
+// (5.2 TB/s), 60 for two and 90 for four; with the product kernel, most of its rows being outside of the matrix, it takes 67 for any of them.  Dot products
+// in 32 bits, four rows of weights in a warp at a time (two, and twice the blocks, where the sums of several examples take the registers: 82 us for two
+// examples with four), of every lane 16 bytes (or, where rows start anywhere, an element).  A lane keeps the statistics of one of the rows' products with
+// one example; a block leaves one part.
+constexpr int kFewThreads = 256;
+__host__ __device__ constexpr int few_rows(size_t element, int examples) { return element == 2 && examples > 1 ? 2 : 4; }
 
 struct FewArgs {
     const void *x, *w;
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs 
 {
     next_may_start();
     wait_for_previous();
-    constexpr int V = kWhole ? 16 / sizeof(T) : 1, kValues = kExamples * kFewRows, kStep = 32 * V;
+    constexpr int V = kWhole ? 16 / sizeof(T) : 1, kRows = few_rows(sizeof(T), kExamples), kValues = kExamples * kRows, kStep = 32 * V, kUnroll = sizeof(T) == 2 ? 4 : 2;
     extern __shared__ float4 shared_x4[];
     float *shared_x = (float *)shared_x4;       // [example][columns, rounded up to the step]
     __shared__ RowSums block_sums[kFewThreads / 32][kValues];
@@ -530,21 +532,21 @@ __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs 
     RowBest best = RowBest::none();
     const int my_row = lane / kExamples, my_example = lane % kExamples;     // lanes behind kValues keep nothing
     const int wanted = a.wanted && lane < kValues && my_example < a.examples ? a.wanted[my_example] : -1;
-    for (long long v0 = ((long long)blockIdx.x * (kFewThreads / 32) + warp) * kFewRows; v0 < a.labels; v0 += (long long)gridDim.x * (kFewThreads / 32) * kFewRows) {
-        float dot[kFewRows][kExamples];
-        const T *row[kFewRows];
+    for (long long v0 = ((long long)blockIdx.x * (kFewThreads / 32) + warp) * kRows; v0 < a.labels; v0 += (long long)gridDim.x * (kFewThreads / 32) * kRows) {
+        float dot[kRows][kExamples];
+        const T *row[kRows];
 #pragma unroll
-        for (int r = 0; r < kFewRows; r++) {
+        for (int r = 0; r < kRows; r++) {
             row[r] = (const T *)a.w + min(v0 + r, (long long)a.labels - 1) * a.w_stride;
 #pragma unroll
             for (int e = 0; e < kExamples; e++) dot[r][e] = 0.f;
         }
-#pragma unroll 2
+#pragma unroll kUnroll
         for (int c0 = 0; c0 < a.columns; c0 += kStep) {
             const int c = c0 + lane * V;
-            Pack<T, V> w[kFewRows];
+            Pack<T, V> w[kRows];
 #pragma unroll
-            for (int r = 0; r < kFewRows; r++)
+            for (int r = 0; r < kRows; r++)
                 if (c < a.columns) w[r] = *(const Pack<T, V> *)(row[r] + c);
                 else
 #pragma unroll
@@ -557,14 +559,14 @@ __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs 
                     for (int i = 0; i < V; i += 4) reinterpret_cast<float4 &>(x[i]) = *(const float4 *)(shared_x + e * padded + c + i);
                 else x[0] = shared_x[e * padded + c];
 #pragma unroll
-                for (int r = 0; r < kFewRows; r++)
+                for (int r = 0; r < kRows; r++)
 #pragma unroll
                     for (int i = 0; i < V; i++) dot[r][e] = fmaf(to_float(w[r].v[i]), x[i], dot[r][e]);
             }
         }
         float mine = 0.f;
 #pragma unroll
-        for (int r = 0; r < kFewRows; r++)
+        for (int r = 0; r < kRows; r++)
 #pragma unroll
             for (int e = 0; e < kExamples; e++) {
 #pragma unroll
@@ -585,7 +587,7 @@ __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs 
     RowSums all = RowSums::none();
     RowBest top = RowBest::none();
     for (int w = 0; w < kFewThreads / 32; w++)
-        for (int r = 0; r < kFewRows; r++) {
+        for (int r = 0; r < kRows; r++) {
             const RowSums s = block_sums[w][r * kExamples + threadIdx.x];
             const RowBest b = block_best[w][r * kExamples + threadIdx.x];
             if (kFindBest) {
@@ -1082,7 +1084,7 @@ int64_t piece_of(int64_t examples, int64_t labels, int parts)
     return best * 256;
 }
 
-constexpr int kFewBlocks = 148 * 4;
+constexpr int few_blocks(size_t element, int examples) { return 148 * (few_rows(element, examples) == 4 ? 4 : 8); }
 constexpr size_t kFewShared = 96 << 10;
 
 void lay_out_workspace(Call &c)
@@ -1090,9 +1092,9 @@ void lay_out_workspace(Call &c)
     c.products = c.type == GTM_F32 ? kPartProducts : 1;
     c.parts = c.type == GTM_F32 ? 3 : 1;
     const int64_t size = (int64_t)type_bytes(c.type);
-    // as many examples as are multiplied by the plain units about as fast as memory delivers the weights: 8 in 32 bits (and no parts to lay out), 4 in 16
+    // as many examples as are multiplied by the plain units about as fast as memory delivers the weights: 8 in 32 bits (and no parts to lay out), 2 in 16
     const int64_t padded = (int64_t)round_up(c.columns, 256);
-    c.few = !c.gradient && c.examples <= (c.type == GTM_F32 ? 8 : 4) && (c.examples <= 4 ? 4 : 8) * padded * 4 <= (int64_t)kFewShared;
+    c.few = !c.gradient && c.examples <= (c.type == GTM_F32 ? 8 : 2) && (c.examples <= 4 ? 4 : 8) * padded * 4 <= (int64_t)kFewShared;
     c.few_whole = aligned(c.w, c.w_stride * size, 16) && c.columns * size % 16 == 0;
     // the gradient's x is laid out anew in any case: examples that are ignored may hold anything
     c.lay_out_x = !c.few && (c.gradient || !direct(c.type, c.x, c.examples, c.x_stride, c.columns));
@@ -1107,7 +1109,7 @@ void lay_out_workspace(Call &c)
     c.at_rows = take(c.examples * 4);
     if (!c.gradient) {
         const int tile = tile_columns(c.examples, c.labels);
-        c.stat_parts = c.few ? kFewBlocks : (int)((c.labels + tile - 1) / tile) * 2;
+        c.stat_parts = c.few ? few_blocks(size, (int)c.examples) : (int)((c.labels + tile - 1) / tile) * 2;
         c.piece_rows = std::min<int64_t>(c.examples, clamp64(kStatBytes / (c.stat_parts * 8) / 256 * 256, 256, (int64_t)1 << 30));
         c.at_sums = take((uint64_t)c.stat_parts * c.piece_rows * 8);
         c.at_best = take((uint64_t)c.stat_parts * c.piece_rows * 4);
@@ -1217,8 +1219,10 @@ int launch_few(const FewArgs &a, bool whole, int blocks, cudaStream_t stream)
 {
     if (a.examples == 1) return whole ? launch_few<T, 1, true>(a, blocks, stream) : launch_few<T, 1, false>(a, blocks, stream);
     if (a.examples == 2) return whole ? launch_few<T, 2, true>(a, blocks, stream) : launch_few<T, 2, false>(a, blocks, stream);
-    if (a.examples <= 4) return whole ? launch_few<T, 4, true>(a, blocks, stream) : launch_few<T, 4, false>(a, blocks, stream);
-    if constexpr (sizeof(T) == 4) return whole ? launch_few<T, 8, true>(a, blocks, stream) : launch_few<T, 8, false>(a, blocks, stream);
+    if constexpr (sizeof(T) == 4) {
+        if (a.examples <= 4) return whole ? launch_few<T, 4, true>(a, blocks, stream) : launch_few<T, 4, false>(a, blocks, stream);
+        return whole ? launch_few<T, 8, true>(a, blocks, stream) : launch_few<T, 8, false>(a, blocks, stream);
+    }
     return fail(GTM_ERR_ARG, "more examples than are few");
 }
 
@@ -1252,7 +1256,9 @@ int forward(Call &c, const void *labels, int labels_64, int64_t ignored, float s
     };
     if (c.few) {
         const FewArgs a = {c.x, c.w, c.x_stride, c.w_stride, (int)c.examples, (int)c.labels, (int)c.columns, scale, rows, sums, labels ? nullptr : indices, label_logit};
-        const int blocks = (int)std::min<int64_t>(kFewBlocks, (c.labels + kFewRows * kFewThreads / 32 - 1) / (kFewRows * kFewThreads / 32));
+        const size_t size = type_bytes(c.type);
+        const int64_t turn = few_rows(size, (int)c.examples) * (kFewThreads / 32);
+        const int blocks = (int)std::min<int64_t>(few_blocks(size, (int)c.examples), (c.labels + turn - 1) / turn);
         GTM_TRY(c.type == GTM_F32    ? launch_few<float>(a, c.few_whole, blocks, stream)
                 : c.type == GTM_BF16 ? launch_few<__nv_bfloat16>(a, c.few_whole, blocks, stream)
                                      : launch_few<__half>(a, c.few_whole, blocks, stream));
