@@ -8,8 +8,9 @@
 // the piece goes to the workspace in the operands' 16-bit type, and two products use it.  All products are one kernel on
 // tcgen05 over pairs of thread blocks: tiles of 256 x 256 (or 128), operands by TMA through a ring in shared memory, sums in tensor
 // memory, two tiles deep, so that a tile's epilogue runs under the next tile's products; results leave by TMA too.  dw and dx of a piece are one
-// launch: dw's tiles go round, and dx's work fills up what is left of the last round.  For up to two examples (eight in 32 bits) the forward
-// pass is a kernel of plain dot products, whose time is that of reading w.
+// launch: dw's tiles go round, and dx's work fills up what is left of the last round.  For up to two examples (eight in 32 bits) the prediction
+// is a kernel of plain dot products, whose time is that of reading w.  The loss of so few stays with the product kernel: the gradient takes
+// P from the same logits then, and where P of the label is near one, a logit's error leaves it with the normaliser.
 //
 // 16-bit inputs are multiplied as they are, with sums in 32 bits.  32-bit inputs are split into three bf16 parts (24 bits of fraction),
 // and the six products of parts that reach 2^-24 are added, the smallest first.  The tensor cores cut sums off instead of rounding them, about 1e-8 of
@@ -493,7 +494,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
     if (warp == 2) tmem_free(tmem, 512);
 }
 
-// The forward pass for few examples, whose time is that of reading the weights.  A whole pass over 131,072 x 1,024 bf16 takes 52 us for one example
+// The prediction for few examples, whose time is that of reading the weights.  A whole pass over 131,072 x 1,024 bf16 takes 52 us for one example
 // (5.2 TB/s), 60 for two and 90 for four; with the product kernel, most of its rows being outside of the matrix, it takes 67 for any of them.  Dot products
 // in 32 bits, four rows of weights in a warp at a time (two, and twice the blocks, where the sums of several examples take the registers: 82 us for two
 // examples with four), of every lane 16 bytes (or, where rows start anywhere, an element).  A lane keeps the statistics of one of the rows' products with
@@ -506,13 +507,11 @@ struct FewArgs {
     long long x_stride, w_stride;
     int examples, labels, columns;
     float scale;
-    const int *wanted;                          // labels of the examples, null: none
     float2 *sums;
     int *best;
-    float *label_logit;
 };
 
-template <class T, int kExamples, bool kWhole, bool kFindBest>
+template <class T, int kExamples, bool kWhole>
 __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs a)
 {
     next_may_start();
@@ -520,7 +519,6 @@ __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs 
     constexpr int V = kWhole ? 16 / sizeof(T) : 1, kRows = few_rows(sizeof(T), kExamples), kValues = kExamples * kRows, kStep = 32 * V, kUnroll = sizeof(T) == 2 ? 4 : 2;
     extern __shared__ float4 shared_x4[];
     float *shared_x = (float *)shared_x4;       // [example][columns, rounded up to the step]
-    __shared__ RowSums block_sums[kFewThreads / 32][kValues];
     __shared__ RowBest block_best[kFewThreads / 32][kValues];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, padded = (a.columns + kStep - 1) / kStep * kStep;
     for (int i = threadIdx.x; i < kExamples * padded; i += kFewThreads) {
@@ -528,10 +526,8 @@ __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs 
         shared_x[i] = e < a.examples && c < a.columns ? to_float(((const T *)a.x)[e * a.x_stride + c]) : 0.f;
     }
     __syncthreads();
-    RowSums sums = RowSums::none();
     RowBest best = RowBest::none();
-    const int my_row = lane / kExamples, my_example = lane % kExamples;     // lanes behind kValues keep nothing
-    const int wanted = a.wanted && lane < kValues && my_example < a.examples ? a.wanted[my_example] : -1;
+    const int my_row = lane / kExamples;        // lanes behind kValues keep nothing
     for (long long v0 = ((long long)blockIdx.x * (kFewThreads / 32) + warp) * kRows; v0 < a.labels; v0 += (long long)gridDim.x * (kFewThreads / 32) * kRows) {
         float dot[kRows][kExamples];
         const T *row[kRows];
@@ -575,37 +571,26 @@ __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs 
             }
         if (lane < kValues && v0 + my_row < a.labels) {
             const float one[1] = {mine};
-            if (kFindBest) best.take(one, a.scale * kLog2e, (int)(v0 + my_row));
-            else sums.take(one, a.scale * kLog2e);
-            if (wanted == v0 + my_row) a.label_logit[my_example] = mine;
+            best.take(one, a.scale * kLog2e, (int)(v0 + my_row));
         }
     }
-    if (lane < kValues) block_sums[warp][lane] = sums, block_best[warp][lane] = best;
+    if (lane < kValues) block_best[warp][lane] = best;
     __syncthreads();
     if (threadIdx.x >= kExamples || threadIdx.x >= a.examples) return;
     const float slope = a.scale * kLog2e;
-    RowSums all = RowSums::none();
     RowBest top = RowBest::none();
     for (int w = 0; w < kFewThreads / 32; w++)
         for (int r = 0; r < kRows; r++) {
-            const RowSums s = block_sums[w][r * kExamples + threadIdx.x];
             const RowBest b = block_best[w][r * kExamples + threadIdx.x];
-            if (kFindBest) {
-                // labels of different warps are in no order: of equal products the lower label is the best
-                const bool lower = b.largest == top.largest && b.index < top.index;
-                const int index = b.index;
-                top.add(b.largest, b.rest, slope, index);
-                if (lower && b.largest > -INFINITY) top.index = index;
-            } else {
-                const float next = fmaxf(all.largest, s.largest);
-                if (next == -INFINITY) all.sum += s.sum;
-                else all.sum = (all.largest > -INFINITY ? all.sum * exp2_fast((all.largest - next) * slope) : all.sum) + (s.largest > -INFINITY ? s.sum * exp2_fast((s.largest - next) * slope) : s.sum);
-                all.largest = next;
-            }
+            // labels of different warps are in no order: of equal products the lower label is the best
+            const bool lower = b.largest == top.largest && b.index < top.index;
+            const int index = b.index;
+            top.add(b.largest, b.rest, slope, index);
+            if (lower && b.largest > -INFINITY) top.index = index;
         }
     const long long at = (long long)blockIdx.x * a.examples + threadIdx.x;
-    a.sums[at] = kFindBest ? make_float2(top.largest, top.rest) : make_float2(all.largest, all.sum);
-    if (kFindBest) a.best[at] = top.index;
+    a.sums[at] = make_float2(top.largest, top.rest);
+    a.best[at] = top.index;
 }
 
 // ------------------------------------------------------------------------------------------- around the products
@@ -1048,7 +1033,7 @@ struct Call {
     int64_t examples, labels, columns;
     const void *x, *w;
     int64_t x_stride, w_stride;
-    bool lay_out_x, lay_out_w, gradient;
+    bool lay_out_x, lay_out_w, gradient, predict;
     int64_t x_ld, w_ld;
     // forward
     bool few, few_whole;
@@ -1094,7 +1079,7 @@ void lay_out_workspace(Call &c)
     const int64_t size = (int64_t)type_bytes(c.type);
     // as many examples as are multiplied by the plain units about as fast as memory delivers the weights: 8 in 32 bits (and no parts to lay out), 2 in 16
     const int64_t padded = (int64_t)round_up(c.columns, 256);
-    c.few = !c.gradient && c.examples <= (c.type == GTM_F32 ? 8 : 2) && (c.examples <= 4 ? 4 : 8) * padded * 4 <= (int64_t)kFewShared;
+    c.few = c.predict && c.examples <= (c.type == GTM_F32 ? 8 : 2) && (c.examples <= 4 ? 4 : 8) * padded * 4 <= (int64_t)kFewShared;
     c.few_whole = aligned(c.w, c.w_stride * size, 16) && c.columns * size % 16 == 0;
     // the gradient's x is laid out anew in any case: examples that are ignored may hold anything
     c.lay_out_x = !c.few && (c.gradient || !direct(c.type, c.x, c.examples, c.x_stride, c.columns));
@@ -1207,11 +1192,8 @@ template <class T, int kExamples, bool kWhole>
 int launch_few(const FewArgs &a, int blocks, cudaStream_t stream)
 {
     const size_t shared = kExamples * round_up(a.columns, 256) * 4;
-    const auto run = [&](auto kernel) -> int {
-        GTM_CU(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewShared));
-        return launch_early(kernel, dim3(blocks), dim3(kFewThreads), shared, stream, a);
-    };
-    return a.best ? run(softmax_few_kernel<T, kExamples, kWhole, true>) : run(softmax_few_kernel<T, kExamples, kWhole, false>);
+    GTM_CU(cudaFuncSetAttribute(softmax_few_kernel<T, kExamples, kWhole>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFewShared));
+    return launch_early(softmax_few_kernel<T, kExamples, kWhole>, dim3(blocks), dim3(kFewThreads), shared, stream, a);
 }
 
 template <class T>
@@ -1255,7 +1237,7 @@ int forward(Call &c, const void *labels, int labels_64, int64_t ignored, float s
         });
     };
     if (c.few) {
-        const FewArgs a = {c.x, c.w, c.x_stride, c.w_stride, (int)c.examples, (int)c.labels, (int)c.columns, scale, rows, sums, labels ? nullptr : indices, label_logit};
+        const FewArgs a = {c.x, c.w, c.x_stride, c.w_stride, (int)c.examples, (int)c.labels, (int)c.columns, scale, sums, indices};
         const size_t size = type_bytes(c.type);
         const int64_t turn = few_rows(size, (int)c.examples) * (kFewThreads / 32);
         const int blocks = (int)std::min<int64_t>(few_blocks(size, (int)c.examples), (c.labels + turn - 1) / turn);
@@ -1291,18 +1273,21 @@ int forward(Call &c, const void *labels, int labels_64, int64_t ignored, float s
 
 using namespace gtm_readout;
 
-static Call call_of(int type, int64_t examples, int64_t labels, int64_t columns, const void *x, int64_t x_stride, const void *w, int64_t w_stride, bool gradient)
+enum { kLossCall, kGradientCall, kPredictCall };
+
+static Call call_of(int type, int64_t examples, int64_t labels, int64_t columns, const void *x, int64_t x_stride, const void *w, int64_t w_stride, int what)
 {
     Call c = {};
-    c.type = type, c.examples = examples, c.labels = labels, c.columns = columns, c.x = x, c.w = w, c.x_stride = x_stride, c.w_stride = w_stride, c.gradient = gradient;
+    c.type = type, c.examples = examples, c.labels = labels, c.columns = columns, c.x = x, c.w = w, c.x_stride = x_stride, c.w_stride = w_stride, c.gradient = what == kGradientCall, c.predict = what == kPredictCall;
     return c;
 }
 
 extern "C" int gtm_softmax_workspace(int type, const void *features, int64_t examples, int64_t features_stride, const void *weights, int64_t labels, int64_t weights_stride,
-                                     int64_t columns, int gradient, uint64_t *bytes_out)
+                                     int64_t columns, int what, uint64_t *bytes_out)
 {
     if (!bytes_out) return fail(GTM_ERR_ARG, "gtm_softmax_workspace: null output");
-    Call c = call_of(type, examples, labels, columns, features, features_stride, weights, weights_stride, gradient != 0);
+    if (what < kLossCall || what > kPredictCall) return fail(GTM_ERR_ARG, "gtm_softmax_workspace: call %d (0: loss, 1: gradient, 2: prediction)", what);
+    Call c = call_of(type, examples, labels, columns, features, features_stride, weights, weights_stride, what);
     GTM_TRY(check_call("gtm_softmax_workspace", c, 1.f));
     *bytes_out = 0;
     if (examples == 0) return GTM_OK;
@@ -1319,7 +1304,7 @@ extern "C" int gtm_softmax_loss(int device, void *cuda_stream, int type, const v
                                 int64_t weights_stride, int64_t columns, const void *labels, int labels_64, int64_t ignore_label, float scale, float *losses, float *normalisers,
                                 void *workspace, uint64_t workspace_bytes)
 {
-    Call c = call_of(type, examples, number_of_labels, columns, features, features_stride, weights, weights_stride, false);
+    Call c = call_of(type, examples, number_of_labels, columns, features, features_stride, weights, weights_stride, kLossCall);
     GTM_TRY(check_call("gtm_softmax_loss", c, scale));
     if (examples == 0) return GTM_OK;
     if (!features || !weights || !labels || !losses || !normalisers) return fail(GTM_ERR_ARG, "gtm_softmax_loss: null array");
@@ -1340,7 +1325,7 @@ extern "C" int gtm_softmax_loss(int device, void *cuda_stream, int type, const v
 extern "C" int gtm_softmax_predict(int device, void *cuda_stream, int type, const void *features, int64_t examples, int64_t features_stride, const void *weights, int64_t number_of_labels,
                                    int64_t weights_stride, int64_t columns, float scale, int64_t *labels_out, float *log_probabilities_out, void *workspace, uint64_t workspace_bytes)
 {
-    Call c = call_of(type, examples, number_of_labels, columns, features, features_stride, weights, weights_stride, false);
+    Call c = call_of(type, examples, number_of_labels, columns, features, features_stride, weights, weights_stride, kPredictCall);
     GTM_TRY(check_call("gtm_softmax_predict", c, scale));
     if (examples == 0) return GTM_OK;
     if (!features || !weights || !labels_out || !log_probabilities_out) return fail(GTM_ERR_ARG, "gtm_softmax_predict: null array");
@@ -1363,7 +1348,7 @@ extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type
                                          const float *normalisers, const float *gradients, int64_t gradients_step, void *features_gradient, void *weights_gradient, void *workspace,
                                          uint64_t workspace_bytes)
 {
-    Call c = call_of(type, examples, number_of_labels, columns, features, features_stride, weights, weights_stride, true);
+    Call c = call_of(type, examples, number_of_labels, columns, features, features_stride, weights, weights_stride, kGradientCall);
     GTM_TRY(check_call("gtm_softmax_loss_gradient", c, scale));
     if (!weights_gradient || (uintptr_t)weights_gradient % 16 || (uintptr_t)features_gradient % 16)
         return fail(GTM_ERR_ARG, "gtm_softmax_loss_gradient: a result is null or does not start at a 16-byte boundary");

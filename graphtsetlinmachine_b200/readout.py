@@ -147,8 +147,9 @@ def embed_gradient(gradient, ids, rows, offsets=None, scale=1.0):
     return out
 
 
-def _softmax_arguments(features, weights, scale, gradient):
-    """Checks features and weights: (library, device, the arguments that describe them, workspace or None, its address, its size)."""
+def _softmax_arguments(features, weights, scale, call):
+    """Checks features and weights: (library, device, the arguments that describe them, workspace or None, its address, its size).
+    Of a call: 0 for the loss, 1 for its gradient, 2 for the prediction."""
     device = _cuda("features", features).device
     _device_of("weights", weights, device)
     n, d, x_stride = _matrix("features", features)
@@ -162,9 +163,9 @@ def _softmax_arguments(features, weights, scale, gradient):
     lib = _lib.load()
     kind, x, w = _TYPES[features.dtype], features.data_ptr(), weights.data_ptr()
     workspace, address, size = None, None, 0
-    if gradient or v > 32 or v * d > 24576 or n > 65536:
+    if call == 1 or v > 32 or v * d > 24576 or n > 65536:
         need = C.c_uint64()
-        _lib.check(lib.gtm_softmax_workspace(kind, x, n, x_stride, w, v, w_stride, d, gradient, C.byref(need)))
+        _lib.check(lib.gtm_softmax_workspace(kind, x, n, x_stride, w, v, w_stride, d, call, C.byref(need)))
         size = need.value
         workspace = _workspace(max(size, 1), device)
         address = workspace.data_ptr()
@@ -216,7 +217,7 @@ def softmax_loss_gradient(features, weights, labels, normalisers, gradients, sca
 def softmax_predict(features, weights, scale=1.0):
     """(labels int64, log probabilities float32): each example's most probable label under logits ``scale * features @ weights.T``,
     the lowest of equal ones.  -1 and NaN where an example's logits are not numbers."""
-    lib, device, what, workspace, address, size = _softmax_arguments(features, weights, scale, 0)
+    lib, device, what, workspace, address, size = _softmax_arguments(features, weights, scale, 2)
     labels = torch.empty(what[4], dtype=torch.int64, device=device)
     log_probabilities = torch.empty(what[4], dtype=torch.float32, device=device)
     _lib.check(lib.gtm_softmax_predict(*what, scale, labels.data_ptr(), log_probabilities.data_ptr(), address, size))

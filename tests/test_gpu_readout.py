@@ -238,6 +238,42 @@ def test_softmax_in_pieces_of_the_labels(kind):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n, d, v", [(1, 1024, 279), (2, 1000, 279), (8, 1024, 1000), (9, 512, 300), (1, 160, 279), (1, 700, 20), (8, 700, 20)])
+def test_gradient_where_the_label_is_nearly_certain(kind, n, d, v):
+    """P - 1 of the label: its logit's error is in the normaliser too, so that what is left of it is times 1 - P.  The gradients of the weights are
+    P - 1 times the features."""
+    gen = generator(n + d + v)
+    w = normal(gen, v, d) / math.sqrt(d)
+    labels = torch.randperm(v, generator=gen, device="cuda")[:n]            # every label once: a row of dw is one example's
+    x = 14.0 * w[labels] / (w[labels] ** 2).sum(1, keepdim=True) + 0.1 * normal(gen, n, d)
+    x, w = x.to(kind), w.to(kind)
+    logits, off, normaliser = plain_softmax(x, w, 1.0)
+    at = torch.arange(n)
+    others = logits.clone()
+    others[at, labels] = -math.inf
+    q = -(torch.logsumexp(others, 1) - normaliser).exp()
+    _, normalisers = readout.softmax_loss(x, w, labels)
+    _, dw = readout.softmax_loss_gradient(x, w, labels, normalisers, torch.ones(n, device="cuda"))
+    xs = x.double()
+    rows = dw[labels].double()
+    others = torch.softmax(logits, 1)
+    others[at, labels] = 0.0
+    mixed = others[:, labels].t()                                           # what other examples add to a label's row
+    rows = rows - (mixed - torch.diag(torch.diag(mixed))) @ xs
+    got = (rows * xs).sum(1) / (xs * xs).sum(1)
+    # the normaliser's rounding and those of the sum and the logarithm in it, near one; the exponentials' 2^-21; the logits' errors, times 1 - P
+    bound = 2.0 ** -23 * normaliser.abs() + 2.0 ** -22 + q.abs() * (2 * off.amax(1) + 2.0 ** -20 + 2.0 ** -22 * normaliser.abs())
+    # q as an operand and the result are rounded, each by half a step; products of up to n terms; examples mixed in are off as their P are
+    bound = bound + q.abs() * (2 * max(half(kind), 2.0 ** -22) + (n + 16) * STEP)
+    length = xs.norm(dim=1)
+    amount = (mixed - torch.diag(torch.diag(mixed))) @ length / length      # of the others' P, at the most, in units of the example's features
+    bound = bound + amount * (2 * max(half(kind), 2.0 ** -22) + 2 * off.amax() + 2.0 ** -20 + 2.0 ** -22 * normaliser.abs().amax())
+    if kind == F16:
+        bound = bound + 2.0 ** -24 * math.sqrt(d) / length                  # results below fp16's normal ones
+    near(got, q, bound)
+
+
+@pytest.mark.parametrize("kind", TYPES)
 def test_softmax_of_few_examples_in_pieces_of_the_labels(kind):
     x, w, labels = softmax_case(kind, 20, 8, (1 << 20) + 5000)
     normalisers = check_loss(x, w, labels, 1.0)

@@ -102,3 +102,15 @@ def test_workspaces_grow_with_what_they_hold():
     assert forward < 8192 * 65536 * 2 // 8 and backward < 8192 * 65536 * 2 // 4
     assert size(lib.gtm_softmax_workspace, 1, POINTER, 0, 8, POINTER, 5, 8, 8, 0) == 0
     assert lib.gtm_softmax_workspace(1, POINTER, 3, 8, POINTER, 5, 8, 8, 0, None) == 1
+
+
+def test_softmax_workspaces_are_those_of_a_call():
+    lib, out = _lib.load(), C.c_uint64()
+    sizes = []
+    for what in (0, 1, 2):
+        assert lib.gtm_softmax_workspace(0, POINTER, 1, 1024, POINTER, 65536, 1024, 1024, what, C.byref(out)) == 0
+        sizes.append(out.value)
+    # in 32 bits a prediction for one example reads the weights as they are; loss and gradient have them in three parts of 16 bits
+    assert sizes[2] < 65536 * 1024 * 4 < 65536 * 1024 * 6 <= min(sizes[:2])
+    for what in (-1, 3):
+        assert lib.gtm_softmax_workspace(0, POINTER, 1, 1024, POINTER, 65536, 1024, 1024, what, C.byref(out)) == 1
