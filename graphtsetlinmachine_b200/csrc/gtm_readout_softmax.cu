@@ -16,7 +16,7 @@
 // and the six products of parts that reach 2^-24 are added, the smallest first.  The tensor cores cut sums off instead of rounding them, about 1e-8 of
 // the sum at every step of 16 elements and always towards zero; so where inputs have 32 bits, the large products of a logit are summed in two
 // halves, and sums for dw and dx go to memory after 512 elements, where they are added with rounding.  P is rounded to the operands' type, to as many bits as
-// dx and dw are; fp16 has too small a range for that, so P is scaled by 2^14 over the largest |gradient * scale| there.
+// dx and dw are; fp16 has too small a range for that, so P is scaled by 2^14 over the largest finite |gradient * scale| there (2^-38 of that is the smallest step of P).
 #include "gtm_readout.cuh"
 #include "gtm_readout_mma.cuh"
 #include "gtm_readout_softmax.h"
@@ -64,7 +64,7 @@ struct Product {
     unsigned what;                              // instruction descriptor
     int add;                                    // the result is added to what is there
     int type;                                   // of the result: GTM_F32 (slices of sums too) or a 16-bit type
-    const unsigned *out_scale;                  // bits of the largest |factor|: the result is 2^-14 times this, null: 1
+    const unsigned *out_scale;                  // bits of the largest finite |factor|: the result is 2^-14 times this, null: 1
 
     __host__ __device__ int tiles() const { return m_tiles * n_tiles; }
     __host__ __device__ int splits() const { return (blocks + per_split - 1) / per_split; }
@@ -118,7 +118,7 @@ struct Launch {
     int first_label;                            // label of column 0
     // kProb
     const float *normalisers, *factors;         // [rows]
-    const unsigned *largest;                    // bits of the largest |factor|, null: factors as they are
+    const unsigned *largest;                    // bits of the largest finite |factor|, null: factors as they are
 };
 
 // A pair's work, piece by piece.
@@ -394,8 +394,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
             if (kMode == kProb && real) {
                 normaliser = l.normalisers[row], factor = l.factors[row];
                 if (l.largest) {
-                    const float largest = __uint_as_float(*l.largest);
-                    factor = largest == 0.f ? 0.f : factor / largest * 16384.f;
+                    // a factor that is not finite has no part in the largest: it is its example's alone
+                    factor = factor == 0.f ? 0.f : isfinite(factor) ? factor / __uint_as_float(*l.largest) * 16384.f : __int_as_float(0x7fffffff);
                 }
             }
             if (kMode == kOut) slice = w.slice();
@@ -708,7 +708,7 @@ __global__ void __launch_bounds__(256) softmax_rows_kernel(const void *labels, i
     if (!factors) return;
     const float f = label == -1 ? 0.f : label == -2 ? __int_as_float(0x7fffffff) : gradients[r * gradients_step] * scale;
     factors[r] = f;
-    if (largest) atomicMax(largest, __float_as_uint(fabsf(f)));      // of magnitudes: the bits have their order, NaN above all
+    if (largest && isfinite(f)) atomicMax(largest, __float_as_uint(fabsf(f)));      // of finite magnitudes: the bits have their order
 }
 
 // Statistics of two sets of a row's products, joined.

@@ -198,7 +198,8 @@ def softmax_loss_gradient(features, weights, labels, normalisers, gradients, sca
     """Gradients (of features, of weights; each of the inputs' type) of ``softmax_loss`` with the same arguments.  ``normalisers``: what
     that call gave; ``gradients``: dL/dlosses, float32 of one element per example or of one element for all (1 / n for the mean).
 
-    An ignored example's gradient is zero, and it adds nothing to the weights' gradient, whatever its features hold."""
+    An ignored example's gradient is zero, and it adds nothing to the weights' gradient, whatever its features hold.  An example whose label
+    there is not, or whose element of ``gradients`` is not finite, spoils its own gradient and the weights', not that of other examples."""
     lib, device, what, workspace, address, size = _softmax_arguments(features, weights, scale, 1)
     n = what[4]
     wide = _wanted(labels, n, device)
