@@ -1291,7 +1291,7 @@ extern "C" int gtm_softmax_workspace(int type, const void *features, int64_t exa
     GTM_TRY(check_call("gtm_softmax_workspace", c, 1.f));
     *bytes_out = 0;
     if (examples == 0) return GTM_OK;
-    if (few_labels(examples, labels, columns, c.gradient)) {
+    if (few_labels(examples, labels, columns)) {
         *bytes_out = few_labels_workspace(examples, labels, columns, c.gradient);
         return GTM_OK;
     }
@@ -1308,7 +1308,7 @@ extern "C" int gtm_softmax_loss(int device, void *cuda_stream, int type, const v
     GTM_TRY(check_call("gtm_softmax_loss", c, scale));
     if (examples == 0) return GTM_OK;
     if (!features || !weights || !labels || !losses || !normalisers) return fail(GTM_ERR_ARG, "gtm_softmax_loss: null array");
-    const bool few_ones = few_labels(examples, number_of_labels, columns, false);
+    const bool few_ones = few_labels(examples, number_of_labels, columns);
     if (!few_ones) {
         lay_out_workspace(c);
         GTM_TRY(check_workspace("gtm_softmax_loss", workspace, workspace_bytes, c.total));
@@ -1329,7 +1329,7 @@ extern "C" int gtm_softmax_predict(int device, void *cuda_stream, int type, cons
     GTM_TRY(check_call("gtm_softmax_predict", c, scale));
     if (examples == 0) return GTM_OK;
     if (!features || !weights || !labels_out || !log_probabilities_out) return fail(GTM_ERR_ARG, "gtm_softmax_predict: null array");
-    const bool few_ones = few_labels(examples, number_of_labels, columns, false);
+    const bool few_ones = few_labels(examples, number_of_labels, columns);
     if (!few_ones) {
         lay_out_workspace(c);
         GTM_TRY(check_workspace("gtm_softmax_predict", workspace, workspace_bytes, c.total));
@@ -1361,7 +1361,7 @@ extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type
         return GTM_OK;
     }
     if (!features || !weights || !labels || !normalisers || !gradients || !features_gradient) return fail(GTM_ERR_ARG, "gtm_softmax_loss_gradient: null array");
-    if (few_labels(examples, number_of_labels, columns, true)) {
+    if (few_labels(examples, number_of_labels, columns)) {
         GTM_TRY(check_workspace("gtm_softmax_loss_gradient", workspace, workspace_bytes, few_labels_workspace(examples, number_of_labels, columns, true)));
         const FewLabels few = {type, examples, number_of_labels, columns, features, weights, features_stride, weights_stride, labels, labels_64, ignore_label, scale};
         return few_labels_gradient(few, normalisers, gradients, gradients_step, features_gradient, weights_gradient, workspace, stream);

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from graphtsetlinmachine_b200 import readout
-from test_gpu_readout import TYPES, _library, generator, softmax_case  # noqa: F401  (_library: no wait ran out)
+from test_gpu_readout import STEP, TYPES, _library, check_gradient, check_loss, generator, half, least, near, normal, softmax_case  # noqa: F401  (_library: no wait ran out)
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,38 @@ def test_an_example_without_a_gradient_leaves_the_others_alone(kind, n, d, v, ba
     others = torch.arange(n, device="cuda") != 3
     assert torch.equal(dx[others], want[others]) and (dx[labels == -7] == 0).all()
     assert not torch.isfinite(dx[3]).any() and not torch.isfinite(dw).any()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [65536, 65537, 70001])
+def test_few_labels_and_many_examples_take_the_same_logits(kind, n):
+    """Logits with a large part that all labels share: P of the label, nearly certain, less one is right only where the normaliser has the same error
+    as the logit.  The weights' first columns are c times the unit matrix, so that features' gradients show P - 1 by itself."""
+    v, d, c = 10, 2048, 4.0
+    gen = generator(n)
+    labels, at = torch.randint(v, (n,), generator=gen, device="cuda"), torch.arange(n, device="cuda")
+    w = torch.full((v, d), 1 / 16, device="cuda")
+    w[:, :v] = c * torch.eye(v, device="cuda")
+    x = normal(gen, n, d).abs()
+    x[:, :v] *= 0.1
+    x[at, labels] = 12 / c
+    x, w = x.to(kind), w.to(kind)
+    logits = x.double() @ w.double().t()
+    off = (d + 16) * STEP * logits.amax(1)
+    normaliser = torch.logsumexp(logits, 1)
+    logits[at, labels] = -math.inf
+    q = -(torch.logsumexp(logits, 1) - normaliser).exp()
+    _, normalisers = readout.softmax_loss(x, w, labels)
+    dx, _ = readout.softmax_loss_gradient(x, w, labels, normalisers, torch.ones(1, device="cuda"))
+    # the normaliser's rounding and those of the sum and the logarithm in it; the logits' errors and the exponential's, times 1 - P; P's rounding and dx'
+    bound = 2.0 ** -23 * normaliser + 2.0 ** -22 + q.abs() * (2 * off + 2.0 ** -20 + 2.0 ** -22 * normaliser + 2 * max(half(kind), 2.0 ** -22)) + least(kind)
+    near(dx[at, labels].double() / c, q, bound)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,d,v", [(70001, 33, 7), (200003, 8, 32), (66000, 300, 2)])
+def test_few_labels_and_many_examples(kind, n, d, v):
+    x, w, labels = softmax_case(kind, n, d, v)
+    labels[::9] = -1
+    normalisers = check_loss(x, w, labels, 1.25)
+    check_gradient(x, w, labels, normalisers, normal(generator(n), n).abs() + 0.1, 1.25)
