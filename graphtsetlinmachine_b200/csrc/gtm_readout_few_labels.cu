@@ -5,7 +5,9 @@
 // block's sums of dw over its examples (P in shared memory, a thread per column); the second adds the blocks' sums up, in their order.
 // What bounds it is the number of launches and, for many examples, reading x; the tensor cores' tiles would be mostly empty: 60 examples of 64
 // columns and ten labels in 32 bits take 4 us forward and 9 for the gradient, where products by tiles took 20 and 45.  Loss and gradient take the same
-// logits, those of these kernels, for as many examples: where P of the label is near one, a logit's error leaves it with the normaliser.
+// logits, those of these kernels, for as many examples: where P of the label is near one, a logit's error leaves it with the normaliser.  Up to 2^16 examples, whose P a block has
+// in 28 KB of shared memory; for more, tiles are faster (66,000 examples of 512 bf16, 32 labels: 48 and 1,110 us for loss and gradient, 163 and 1,920 with
+// these kernels and their examples in pieces; of 64 bf16, ten labels: 42 and 99 instead of 45 and 151).
 #include "gtm_readout.cuh"
 #include "gtm_readout_softmax.h"
 
@@ -16,11 +18,10 @@ namespace {
 
 constexpr int kWarps = 8, kTogether = 2;                // warps of a block, examples that a warp has at a time
 constexpr int kLargestShared = 96 << 10;                // bytes of weights
-constexpr int kPiece = 224;                             // examples whose P a block has in shared memory, 28 KB at the most
 
 struct Args {
     FewLabels p;
-    int per_block, piece;                               // examples of a block, and of them at a time
+    int per_block;                                      // examples
     float *losses, *normalisers_out;
     long long *labels_out;
     float *log_probabilities;
@@ -66,107 +67,100 @@ __global__ void __launch_bounds__(kWarps * 32) few_labels_kernel(const Args a)
     for (int v = warp; v < labels; v += kWarps)
         for (int c = lane; c < columns; c += 32) w[v * columns + c] = to_float(((const T *)p.w)[v * p.w_stride + c]);
     __syncthreads();
-    const long long block_first = (long long)blockIdx.x * a.per_block, block_last = min(block_first + a.per_block, (long long)p.examples);
-    for (long long first = block_first; first < block_last; first += a.piece) {
-        const long long last = min(first + a.piece, block_last);
-        for (long long e0 = first + warp * kTogether; e0 < last; e0 += kWarps * kTogether) {
-            float dot[kTogether][kLabels];
-            const T *row[kTogether];
+    const long long first = (long long)blockIdx.x * a.per_block, last = min(first + a.per_block, (long long)p.examples);
+    for (long long e0 = first + warp * kTogether; e0 < last; e0 += kWarps * kTogether) {
+        float dot[kTogether][kLabels];
+        const T *row[kTogether];
 #pragma unroll
-            for (int k = 0; k < kTogether; k++) {
-                row[k] = (const T *)p.x + min(e0 + k, last - 1) * p.x_stride;
+        for (int k = 0; k < kTogether; k++) {
+            row[k] = (const T *)p.x + min(e0 + k, last - 1) * p.x_stride;
 #pragma unroll
-                for (int v = 0; v < kLabels; v++) dot[k][v] = 0.f;
-            }
-#pragma unroll 2
-            for (int c = lane; c < columns; c += 32) {
-                float x[kTogether];
-#pragma unroll
-                for (int k = 0; k < kTogether; k++) x[k] = to_float(row[k][c]);
-#pragma unroll
-                for (int v = 0; v < kLabels; v++)
-                    if (v < labels) {
-                        const float weight = w[v * columns + c];
-#pragma unroll
-                        for (int k = 0; k < kTogether; k++) dot[k][v] = fmaf(x[k], weight, dot[k][v]);
-                    }
-            }
-#pragma unroll
-            for (int k = 0; k < kTogether; k++) {
-                const long long e = e0 + k;
-                float mine = 0.f;                            // the product of the lane's label
-#pragma unroll
-                for (int v = 0; v < kLabels; v++) {
-                    const float all = sum_of(dot[k][v]);
-                    if (lane == v) mine = all;
-                }
-                if (e >= last) continue;                     // the warp together
-                const bool real = lane < labels;
-                if (kMode == kGradient) {
-                    const int label = label_of(p, e);
-                    float q = 0.f;
-                    if (real && label != -1) {
-                        q = expf(fmaf(mine, p.scale, -a.normalisers[e]));
-                        if (label == lane) q -= 1.f;
-                        q = label == -2 ? __int_as_float(0x7fffffff) : q * (a.gradients[e * a.gradients_step] * p.scale);
-                    }
-                    if (lane < kLabels) prob[(e - first) * kLabels + lane] = q;
-                    __syncwarp();
-                    T *dx = (T *)a.dx + e * columns;
-                    for (int c = lane; c < columns; c += 32) {
-                        float sum = 0.f;
-#pragma unroll
-                        for (int v = 0; v < kLabels; v++)
-                            if (v < labels) sum = fmaf(prob[(e - first) * kLabels + v], w[v * columns + c], sum);
-                        dx[c] = from_float<T>(label == -1 ? 0.f : sum);
-                    }
-                    continue;
-                }
-                const float top = max_of(real ? mine : -INFINITY);
-                const float from = top == -INFINITY ? 0.f : top;
-                const float power = real ? expf((mine - from) * p.scale) : 0.f;
-                if (kMode == kLoss) {
-                    const int label = label_of(p, e);
-                    const float log_sum = logf(sum_of(power)), wanted = __shfl_sync(~0u, mine, label < 0 ? 0 : label);
-                    if (lane == 0) {
-                        a.normalisers_out[e] = fmaf(top, p.scale, log_sum);
-                        a.losses[e] = label == -1 ? 0.f : label == -2 ? __int_as_float(0x7fffffff) : fmaf(top - wanted, p.scale, log_sum);
-                    }
-                } else {
-                    // all but the first of the largest; a product that is no number makes the sum none
-                    const unsigned largest = __ballot_sync(~0u, real && mine == top);
-                    const int best = largest ? __ffs(largest) - 1 : -1;
-                    const float rest = sum_of(real && lane != best ? (mine == mine ? power : mine) : 0.f);
-                    if (lane == 0) {
-                        const float log_probability = best < 0 || top == -INFINITY ? __int_as_float(0x7fffffff) : -log1pf(rest);
-                        a.log_probabilities[e] = log_probability;
-                        a.labels_out[e] = log_probability == log_probability ? best : -1;
-                    }
-                }
-            }
+            for (int v = 0; v < kLabels; v++) dot[k][v] = 0.f;
         }
-        if (kMode != kGradient) return;                      // all of the block's examples were one piece
-        __syncthreads();
-        // the block's sums of dw: a thread has a column
-        for (int c = threadIdx.x; c < columns; c += kWarps * 32) {
-            float sum[kLabels];
+#pragma unroll 2
+        for (int c = lane; c < columns; c += 32) {
+            float x[kTogether];
 #pragma unroll
-            for (int v = 0; v < kLabels; v++) sum[v] = 0.f;
-#pragma unroll 4
-            for (long long e = first; e < last; e++) {
-                if (label_of(p, e) == -1) continue;          // its features may be anything
-                const float x = to_float(((const T *)p.x)[e * p.x_stride + c]);
-#pragma unroll
-                for (int v = 0; v < kLabels; v++) sum[v] = fmaf(prob[(e - first) * kLabels + v], x, sum[v]);
-            }
+            for (int k = 0; k < kTogether; k++) x[k] = to_float(row[k][c]);
 #pragma unroll
             for (int v = 0; v < kLabels; v++)
                 if (v < labels) {
-                    float *to = a.partial + ((long long)blockIdx.x * labels + v) * columns + c;
-                    *to = first == block_first ? sum[v] : *to + sum[v];
+                    const float weight = w[v * columns + c];
+#pragma unroll
+                    for (int k = 0; k < kTogether; k++) dot[k][v] = fmaf(x[k], weight, dot[k][v]);
                 }
         }
-        __syncthreads();                                     // P of the next piece takes the place
+#pragma unroll
+        for (int k = 0; k < kTogether; k++) {
+            const long long e = e0 + k;
+            float mine = 0.f;                            // the product of the lane's label
+#pragma unroll
+            for (int v = 0; v < kLabels; v++) {
+                const float all = sum_of(dot[k][v]);
+                if (lane == v) mine = all;
+            }
+            if (e >= last) continue;                     // the warp together
+            const bool real = lane < labels;
+            if (kMode == kGradient) {
+                const int label = label_of(p, e);
+                float q = 0.f;
+                if (real && label != -1) {
+                    q = expf(fmaf(mine, p.scale, -a.normalisers[e]));
+                    if (label == lane) q -= 1.f;
+                    q = label == -2 ? __int_as_float(0x7fffffff) : q * (a.gradients[e * a.gradients_step] * p.scale);
+                }
+                if (lane < kLabels) prob[(e - first) * kLabels + lane] = q;
+                __syncwarp();
+                T *dx = (T *)a.dx + e * columns;
+                for (int c = lane; c < columns; c += 32) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int v = 0; v < kLabels; v++)
+                        if (v < labels) sum = fmaf(prob[(e - first) * kLabels + v], w[v * columns + c], sum);
+                    dx[c] = from_float<T>(label == -1 ? 0.f : sum);
+                }
+                continue;
+            }
+            const float top = max_of(real ? mine : -INFINITY);
+            const float from = top == -INFINITY ? 0.f : top;
+            const float power = real ? expf((mine - from) * p.scale) : 0.f;
+            if (kMode == kLoss) {
+                const int label = label_of(p, e);
+                const float log_sum = logf(sum_of(power)), wanted = __shfl_sync(~0u, mine, label < 0 ? 0 : label);
+                if (lane == 0) {
+                    a.normalisers_out[e] = fmaf(top, p.scale, log_sum);
+                    a.losses[e] = label == -1 ? 0.f : label == -2 ? __int_as_float(0x7fffffff) : fmaf(top - wanted, p.scale, log_sum);
+                }
+            } else {
+                // all but the first of the largest; a product that is no number makes the sum none
+                const unsigned largest = __ballot_sync(~0u, real && mine == top);
+                const int best = largest ? __ffs(largest) - 1 : -1;
+                const float rest = sum_of(real && lane != best ? (mine == mine ? power : mine) : 0.f);
+                if (lane == 0) {
+                    const float log_probability = best < 0 || top == -INFINITY ? __int_as_float(0x7fffffff) : -log1pf(rest);
+                    a.log_probabilities[e] = log_probability;
+                    a.labels_out[e] = log_probability == log_probability ? best : -1;
+                }
+            }
+        }
+    }
+    if (kMode != kGradient) return;
+    __syncthreads();
+    // the block's sums of dw: a thread has a column
+    for (int c = threadIdx.x; c < columns; c += kWarps * 32) {
+        float sum[kLabels];
+#pragma unroll
+        for (int v = 0; v < kLabels; v++) sum[v] = 0.f;
+#pragma unroll 4
+        for (long long e = first; e < last; e++) {
+            if (label_of(p, e) == -1) continue;          // its features may be anything
+            const float x = to_float(((const T *)p.x)[e * p.x_stride + c]);
+#pragma unroll
+            for (int v = 0; v < kLabels; v++) sum[v] = fmaf(prob[(e - first) * kLabels + v], x, sum[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < kLabels; v++)
+            if (v < labels) a.partial[((long long)blockIdx.x * labels + v) * columns + c] = sum[v];
     }
 }
 
@@ -200,7 +194,7 @@ int per_block(int64_t examples)
 template <class T, int kLabels, int kMode>
 int run(const Args &a, unsigned blocks, cudaStream_t stream)
 {
-    const size_t shared = (size_t)a.p.labels * a.p.columns * 4 + (kMode == kGradient ? (size_t)a.piece * kLabels * 4 : 0);
+    const size_t shared = (size_t)a.p.labels * a.p.columns * 4 + (kMode == kGradient ? (size_t)a.per_block * kLabels * 4 : 0);
     if (shared > 48 << 10) GTM_CU(cudaFuncSetAttribute(few_labels_kernel<T, kLabels, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kLargestShared));
     return launch_early(few_labels_kernel<T, kLabels, kMode>, dim3(blocks), dim3(kWarps * 32), shared, stream, a);
 }
@@ -215,7 +209,6 @@ template <int kMode>
 int run(Args &a, cudaStream_t stream)
 {
     a.per_block = per_block(a.p.examples);
-    a.piece = kMode == kGradient ? std::min(a.per_block, kPiece) : a.per_block;
     const unsigned blocks = (unsigned)((a.p.examples + a.per_block - 1) / a.per_block);
     return a.p.type == GTM_F32    ? run<float, kMode>(a, blocks, stream)
            : a.p.type == GTM_BF16 ? run<__nv_bfloat16, kMode>(a, blocks, stream)

@@ -16,9 +16,9 @@ struct FewLabels {
     float scale;
 };
 
-constexpr int64_t kFewLabelsExamples = (int64_t)1 << 20;
+constexpr int64_t kFewLabelsExamples = (int64_t)1 << 16;
 
-// Whether these kernels take a problem: its loss, its gradient and its prediction alike.
+// Whether these kernels take a problem, its loss, its gradient and its prediction alike.
 bool few_labels(int64_t examples, int64_t labels, int64_t columns);
 uint64_t few_labels_workspace(int64_t examples, int64_t labels, int64_t columns, bool gradient);
 int few_labels_loss(const FewLabels &p, float *losses, float *normalisers, cudaStream_t stream);

@@ -163,7 +163,7 @@ def _softmax_arguments(features, weights, scale, call):
     lib = _lib.load()
     kind, x, w = _TYPES[features.dtype], features.data_ptr(), weights.data_ptr()
     workspace, address, size = None, None, 0
-    if call == 1 or v > 32 or v * d > 24576 or n > 1 << 20:
+    if call == 1 or v > 32 or v * d > 24576 or n > 65536:
         need = C.c_uint64()
         _lib.check(lib.gtm_softmax_workspace(kind, x, n, x_stride, w, v, w_stride, d, call, C.byref(need)))
         size = need.value

@@ -266,7 +266,7 @@ int gtm_embed_gradient(int device, void *cuda_stream, int type, const void *grad
  * loss of a label that there is not is NaN.
  * The gradient takes gradients[n * gradients_step] = dL/dlosses[n] (step 0: one value for all) and the normalisers of the forward
  * call.  Ignored examples have gradient zero, whatever their features hold.
- * With up to 32 labels whose weights take up to 96 KB as floats, and up to 2^20 examples, the loss and the prediction need no workspace (NULL).
+ * With up to 32 labels whose weights take up to 96 KB as floats, and up to 2^16 examples, the loss and the prediction need no workspace (NULL).
  * gtm_softmax_predict gives the most probable label, the lowest of equal ones, and its log probability; -1 and NaN where the logits are
  * not numbers.
  * what: 0 for the workspace of gtm_softmax_loss, 1 for the gradient's, 2 for gtm_softmax_predict's. */
