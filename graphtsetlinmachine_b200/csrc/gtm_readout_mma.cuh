@@ -37,15 +37,25 @@ __device__ __forceinline__ void barrier_expect(unsigned barrier, unsigned bytes)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(bytes) : "memory");
 }
 
+// Behind loads from tensor memory that have been waited for and `tmem_before_sync`, which order them; nothing else is told by it.  With .release the
+// arrival waited for the thread's stores too, 2,300 cycles.
 __device__ __forceinline__ void barrier_arrive_leader(unsigned barrier_in_leader)
 {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(barrier_in_leader) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(barrier_in_leader) : "memory");
 }
 
 __device__ __forceinline__ bool barrier_try(unsigned barrier, unsigned parity)
 {
     unsigned done;
     asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(barrier), "r"(parity) : "memory");
+    return done;
+}
+
+// Whether a phase of a barrier is over, without a wait.
+__device__ __forceinline__ bool barrier_test(unsigned barrier, unsigned parity)
+{
+    unsigned done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(done) : "r"(barrier), "r"(parity) : "memory");
     return done;
 }
 
@@ -56,12 +66,15 @@ __device__ __forceinline__ unsigned long long nanoseconds()
     return t;
 }
 
-// Waits for a phase of a barrier, ten seconds at most.
+// Waits for a phase of a barrier, ten seconds at most.  The clock is asked only once a usual wait is over.
 __device__ __forceinline__ bool barrier_wait(unsigned barrier, unsigned parity)
 {
-    if (barrier_try(barrier, parity)) return true;
+#pragma unroll 1
+    for (int i = 0; i < 4096; i++)
+        if (barrier_try(barrier, parity)) return true;
     const unsigned long long began = nanoseconds();
     while (nanoseconds() - began < 10000000000ull)
+#pragma unroll 1
         for (int i = 0; i < 64; i++)
             if (barrier_try(barrier, parity)) return true;
     return false;

@@ -13,9 +13,10 @@
 // P from the same logits then, and where P of the label is near one, a logit's error leaves it with the normaliser.
 //
 // 16-bit inputs are multiplied as they are, with sums in 32 bits.  32-bit inputs are split into three bf16 parts (24 bits of fraction),
-// and the six products of parts that reach 2^-24 are added, the smallest first.  The tensor cores cut sums off instead of rounding them, about 1e-8 of
-// the sum at every step of 16 elements and always towards zero; so where inputs have 32 bits, the large products of a logit are summed in two
-// halves, and sums for dw and dx go to memory after 512 elements, where they are added with rounding.  P is rounded to the operands' type, to as many bits as
+// and the six products of parts that reach 2^-24 are added, the smallest first.  The tensor cores cut sums off instead of rounding them, about 3e-8 of
+// the sum at every step of 16 elements (1e-7 where all terms have one sign) and always towards zero.  So logits are summed in chunks of up to 256 elements (128 of inputs
+// of 32 bits), which the epilogue adds up in registers, with rounding; and sums for dw and dx of 32-bit inputs go to memory after 512
+// elements, where they are added with rounding.  P is rounded to the operands' type, to as many bits as
 // dx and dw are; fp16 has too small a range for that, so P is scaled by 2^14 over the largest finite |gradient * scale| there (2^-38 of that is the smallest step of P).
 #include "gtm_readout.cuh"
 #include "gtm_readout_mma.cuh"
@@ -33,6 +34,9 @@ constexpr int kHalfBytes = 128 * kDepth * 2;               // an operand's share
 constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kThreads = 384, kEpilogue = 8;               // warps 0: copies, 1: products, 2: tensor memory; 4..11: epilogue
 constexpr int kBoxBytes = 32 * 128;                        // 32 rows of 128 bytes: what a warp of the epilogue stores at once, from two buffers in turn
+// Registers of a thread: as many as launched with (kLaunchedRegisters, the most for so many threads) are split anew between the first four warps and the epilogue, which holds 128 logits.
+constexpr int kLaunchedRegisters = 168, kFewRegisters = 104, kManyRegisters = 200;
+static_assert(128 * kFewRegisters + (kThreads - 128) * kManyRegisters <= kThreads * kLaunchedRegisters, "a block waits for registers that it does not have");
 constexpr int kPairs = 74;                                 // pairs of SMs
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int64_t kPieceBytes = 128 << 20;                 // of P in the workspace at a time
@@ -122,6 +126,7 @@ struct Launch {
 };
 
 // A pair's work, piece by piece.
+template <bool kCut>
 struct Work {
     const Launch &l;
     int pair, item, at;                          // the next item of the first product, and where in it
@@ -136,9 +141,10 @@ struct Work {
         unit = begin = l.schedule.units ? l.schedule.begin(pair) : 0;
         end = l.schedule.units ? l.schedule.begin(pair + 1) : 0;
     }
-    // The end of a piece that begins at block `from`.
+    // The end of a piece that begins at block `from`: of sums in memory a chunk (of several products of parts), of logits the tile.
     __device__ __forceinline__ static int cut(const Product &p, int from, long long end)
     {
+        if (!kCut) return p.blocks;
         const int chunk = p.chunk * p.products;
         return (int)min(end, p.products == 1 ? (long long)p.blocks : min((long long)p.blocks, (from / chunk + 1ll) * chunk));
     }
@@ -315,154 +321,108 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
     wait_for_previous();
 
     bool fine = true;
-    if (warp == 0 && lane == 0) {
-        // copies: the ring's stages of this block, counted on the leader's barriers
-        int stage = 0, phase = 0;
-        for (Work w(l); fine && w.next();) {
-            const Product &p = l.p[w.which];
-            const CUtensorMap *map_a = &maps.a[w.which], *map_b = &maps.b[w.which];
-            const int half_columns = p.tile_columns / 2;
-            const int m0 = w.m * 256 + (int)rank * 128, n0 = w.n * p.tile_columns + (int)rank * half_columns + p.b_row;
-            // the product of parts, and the block of the sum's index, of a chunk at a time
-            const int chunk = w.first / (p.chunk * p.products), chunk_first = chunk * p.chunk, chunk_blocks = min(p.chunk, p.depth_blocks - chunk_first);
-            int product = (w.first - chunk_first * p.products) / chunk_blocks, block = w.first - chunk_first * p.products - product * chunk_blocks;
-            for (int i = w.first; i < w.last; i++) {
-                if (!(fine = barrier_wait(empty + 8 * stage, phase ^ 1))) break;
-                const unsigned to = ring + stage * kStageBytes, bar = in_leader(full + 8 * stage);
-                if (rank == 0) barrier_expect(full + 8 * stage, 2 * (kHalfBytes + half_columns * kDepth * 2));
-                int part_a, part_b;
-                parts_of(p.products, product, part_a, part_b);
-                const int k = (chunk_first + block) * kDepth;
-                if (p.a_rows)
-                    for (int g = 0; g < 2; g++) load_box(map_a, to + g * 8192, bar, m0 + g * 64, p.a_first + k, part_a);
-                else load_box(map_a, to, bar, k, m0, part_a);
-                load_box(map_b, to + kHalfBytes, bar, k, n0, part_b);
-                if (++block == chunk_blocks) block = 0, product++;
+    if (warp < 4) {
+        if constexpr (kMode != kOut) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+        if (warp == 0 && lane == 0) {
+            // copies: the ring's stages of this block, counted on the leader's barriers
+            int stage = 0, phase = 0;
+            for (Work<kMode == kOut> w(l); fine && w.next();) {
+                const Product &p = l.p[w.which];
+                const CUtensorMap *map_a = &maps.a[w.which], *map_b = &maps.b[w.which];
+                const int half_columns = p.tile_columns / 2;
+                const int m0 = w.m * 256 + (int)rank * 128, n0 = w.n * p.tile_columns + (int)rank * half_columns + p.b_row;
+                // the product of parts, and the block of the sum's index, of a chunk at a time
+                int chunk_first = w.first == 0 ? 0 : w.first / (p.chunk * p.products) * p.chunk, chunk_blocks = min(p.chunk, p.depth_blocks - chunk_first);
+                int product = w.first == 0 ? 0 : (w.first - chunk_first * p.products) / chunk_blocks, block = w.first - chunk_first * p.products - product * chunk_blocks;
+                for (int i = w.first; i < w.last; i++) {
+                    if (!(fine = barrier_wait(empty + 8 * stage, phase ^ 1))) break;
+                    const unsigned to = ring + stage * kStageBytes, bar = in_leader(full + 8 * stage);
+                    if (rank == 0) barrier_expect(full + 8 * stage, 2 * (kHalfBytes + half_columns * kDepth * 2));
+                    int part_a, part_b;
+                    parts_of(p.products, product, part_a, part_b);
+                    const int k = (chunk_first + block) * kDepth;
+                    if (p.a_rows)
+                        for (int g = 0; g < 2; g++) load_box(map_a, to + g * 8192, bar, m0 + g * 64, p.a_first + k, part_a);
+                    else load_box(map_a, to, bar, k, m0, part_a);
+                    load_box(map_b, to + kHalfBytes, bar, k, n0, part_b);
+                    if (++block == chunk_blocks) {
+                        block = 0;
+                        if (++product == p.products) product = 0, chunk_first += chunk_blocks, chunk_blocks = min(p.chunk, p.depth_blocks - chunk_first);
+                    }
+                    if (++stage == kStages) stage = 0, phase ^= 1;
+                }
+            }
+            // the products' last arrivals come to this block's barriers before it ends
+            for (int i = 0; i < kStages && fine; i++) {
+                fine = barrier_wait(empty + 8 * stage, phase ^ 1);
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
-        }
-        // the products' last arrivals come to this block's barriers before it ends
-        for (int i = 0; i < kStages && fine; i++) {
-            fine = barrier_wait(empty + 8 * stage, phase ^ 1);
-            if (++stage == kStages) stage = 0, phase ^= 1;
-        }
-        // copies that nobody will wait for any more end before the block does: 20 ms are thousands of times what one takes
-        if (!fine)
-            for (const unsigned long long began = nanoseconds(); nanoseconds() - began < 20000000ull;) __nanosleep(1000);
-    } else if (warp == 1 && lane == 0 && rank == 0) {
-        int stage = 0, phase = 0, buffer = 0, buffer_phase = 0;
-        for (Work w(l); fine && w.next();) {
-            const Product &p = l.p[w.which];
-            // rows next to each other: 64 of them and 8 of the sum's index are 1024 bytes, 64 more rows one box further; a step of 16 is 2048 bytes.
-            // the sum's index next to each other: 8 rows are 1024 bytes; a step of 16 is 32 bytes
-            const unsigned a_leading = p.a_rows ? 8192 : 16, a_step = p.a_rows ? 2048 : 32, what = p.what;
-            if (!(fine = barrier_wait(sums_empty + 8 * buffer, buffer_phase ^ 1))) break;
-            tmem_after_sync();
-            unsigned to = tmem + buffer * 256;
-            const bool halves = kMode != kOut && p.products > 1;
-            int fresh = w.first;                  // the block that begins a sum
-            for (int i = w.first; i < w.last; i++) {
-                if (!(fine = barrier_wait(full + 8 * stage, phase))) break;
-                tmem_after_sync();
-                const unsigned a = ring + stage * kStageBytes, b = a + kHalfBytes;
-                if (halves && i == p.blocks - p.depth_blocks / 2) to += 256, fresh = i;      // the other half of the large products
+            // copies that nobody will wait for any more end before the block does: 20 ms are thousands of times what one takes
+            if (!fine)
+                for (const unsigned long long began = nanoseconds(); nanoseconds() - began < 20000000ull;) __nanosleep(1000);
+        } else if (warp == 1 && lane == 0 && rank == 0) {
+            // barriers of the next stage and of the next sum are asked before products are issued, and answer while they are
+            int stage = 0, phase = 0, buffer = 0, buffer_phase = 0;
+            bool loaded = false, drained = true;
+            for (Work<kMode == kOut> w(l); fine && w.next();) {
+                const Product &p = l.p[w.which];
+                // rows next to each other: 64 of them and 8 of the sum's index are 1024 bytes, 64 more rows one box further; a step of 16 is 2048 bytes.
+                // the sum's index next to each other: 8 rows are 1024 bytes; a step of 16 is 32 bytes
+                const unsigned a_leading = p.a_rows ? 8192 : 16, a_step = p.a_rows ? 2048 : 32, what = p.what;
+                const int chunk = kMode == kOut ? w.last - w.first : p.chunk * p.products;
+                for (int first = w.first; fine && first < w.last; first += chunk) {
+                    const unsigned to = tmem + buffer * 256, sums = sums_full + 8 * buffer;
+                    if (!drained && !(fine = barrier_wait(sums_empty + 8 * buffer, buffer_phase ^ 1))) break;
+                    if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+                    const int blocks = min(chunk, w.last - first);
+                    for (int i = 0; i < blocks; i++) {
+                        if (!loaded && !(fine = barrier_wait(full + 8 * stage, phase))) break;
+                        tmem_after_sync();
+                        const unsigned a = ring + stage * kStageBytes, b = a + kHalfBytes, done = empty + 8 * stage;
+                        if (++stage == kStages) stage = 0, phase ^= 1;
+                        loaded = barrier_test(full + 8 * stage, phase);
+                        drained = barrier_test(sums_empty + 8 * buffer, buffer_phase ^ 1);
 #pragma unroll
-                for (int k = 0; k < kDepth / 16; k++)
-                    multiply(to, operand(a + k * a_step, a_leading, 1024), operand(b + k * 32, 16, 1024), what, i > fresh || k > 0);
-                commit_to_pair(empty + 8 * stage);
-                if (++stage == kStages) stage = 0, phase ^= 1;
+                        for (int k = 0; k < kDepth / 16; k++)
+                            multiply(to, operand(a + k * a_step, a_leading, 1024), operand(b + k * 32, 16, 1024), what, i > 0 || k > 0);
+                        commit_to_pair(done);
+                    }
+                    if (fine) commit_to_pair(sums);
+                }
             }
-            if (!fine) break;
-            commit_to_pair(sums_full + 8 * buffer);
-            if (halves || ++buffer == 2) buffer = 0, buffer_phase ^= 1;
         }
-    } else if (warp >= 4) {
+    } else {
+        if constexpr (kMode != kOut) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
         const int quarter = (warp - 4) & 3, half = (warp - 4) / 4;
         int buffer = 0, buffer_phase = 0;
         BoxStore store = {ring + kStages * kStageBytes + (warp - 4) * 2 * kBoxBytes};
-        for (Work w(l); w.next();) {
+        for (Work<kMode == kOut> w(l); w.next();) {
             const Product &p = l.p[w.which];
             const int half_columns = p.tile_columns / 2;
             const long long row0 = (long long)w.m * 256 + rank * 128 + quarter * 32, row = row0 + lane;
             const bool real = row < p.rows;
             const long long column0 = (long long)w.n * p.tile_columns + half * half_columns;
-            RowSums sums = RowSums::none();
-            RowBest best = RowBest::none();
-            float normaliser = 0.f, factor = 0.f;
-            int label = -1, slice = 0;
-            if ((kMode == kSums || kMode == kProb) && real && l.labels) label = l.labels[row] - l.first_label;
-            if (kMode == kProb && real) {
-                normaliser = l.normalisers[row], factor = l.factors[row];
-                if (l.largest) {
-                    // a factor that is not finite has no part in the largest: it is its example's alone
-                    factor = factor == 0.f ? 0.f : isfinite(factor) ? factor / __uint_as_float(*l.largest) * 16384.f : __int_as_float(0x7fffffff);
-                }
-            }
-            if (kMode == kOut) slice = w.slice();
-            const float out_scale = kMode == kOut && p.out_scale ? __uint_as_float(*p.out_scale) * (1.f / 16384.f) : 1.f;
-            fine = barrier_wait(sums_full + 8 * buffer, buffer_phase);
-            if (!__all_sync(~0u, fine)) break;
-            tmem_after_sync();
-            const bool halves = kMode != kOut && p.products > 1;
-            const unsigned from = tmem + buffer * 256 + half * half_columns + ((unsigned)(quarter * 32) << 16);
+            const unsigned tile = tmem + half * half_columns + ((unsigned)(quarter * 32) << 16);
+            const auto leave = [&] {
+                // the tile's last columns are in registers: the next but one may overwrite it
+                tmem_before_sync();
+                __syncwarp();
+                if (lane == 0) barrier_arrive_leader(in_leader(sums_empty + 8 * buffer));
+                if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+            };
+            if constexpr (kMode == kOut) {
+                const int slice = w.slice();
+                const float out_scale = p.out_scale ? __uint_as_float(*p.out_scale) * (1.f / 16384.f) : 1.f;
+                fine = barrier_wait(sums_full + 8 * buffer, buffer_phase);
+                if (!__all_sync(~0u, fine)) break;
+                tmem_after_sync();
 #pragma unroll 1
-            for (int c = 0; c < half_columns; c += 64) {
-                const long long column = column0 + c, left = p.columns - column;
-                if (left <= 0) break;                                       // the warp together
-                float v[64];
-                tmem_load64(from + c, v);
-                if (halves && p.depth_blocks > 1)
-#pragma unroll
-                    for (int h = 0; h < 64; h += 32) {
-                        float other[32];
-                        tmem_load32(from + 256 + c + h, other);
-#pragma unroll
-                        for (int j = 0; j < 32; j++) v[h + j] += other[j];
-                    }
-                if (c + 64 >= half_columns || left <= 64) {
-                    // the tile's last columns are in registers: the next but one may overwrite it
-                    tmem_before_sync();
-                    __syncwarp();
-                    if (lane == 0) barrier_arrive_leader(in_leader(sums_empty + 8 * buffer));
-                }
-                if (kMode == kSums || kMode == kBest) {
-                    if (left < 64)
-#pragma unroll
-                        for (int j = 0; j < 64; j++)
-                            if (j >= left) v[j] = -INFINITY;
-                    if (kMode == kSums) {
-                        sums.take(v, l.scale * kLog2e);
-                        const long long at = label - column;
-                        if (__any_sync(~0u, at >= 0 && at < 64 && label >= 0)) {
-                            float mine = 0.f;
-#pragma unroll
-                            for (int j = 0; j < 64; j++)
-                                if (at == j) mine = v[j];
-                            if (label >= 0 && at >= 0 && at < 64 && real) l.label_logit[row] = mine;
-                        }
-                    } else {
-                        best.take(v, l.scale * kLog2e, (int)column);
-                    }
-                } else if (kMode == kProb) {
-#pragma unroll
-                    for (int j = 0; j < 64; j++) v[j] = exp2_fast(fmaf(v[j], l.scale, -normaliser) * kLog2e);
-                    const long long at = label - column;
-                    if (__any_sync(~0u, at >= 0 && at < 64))
-#pragma unroll
-                        for (int j = 0; j < 64; j++)
-                            if (at == j) v[j] -= 1.f;
-#pragma unroll
-                    for (int j = 0; j < 64; j++) v[j] = factor == 0.f ? 0.f : v[j] * factor;
-                    if (row0 >= p.rows) continue;                           // the warp together
-                    send_16(store, v, p.type == GTM_F16, &maps.out[0], (int)column, (int)row0, 0);
-                    if (p.products > 1)
-#pragma unroll 1
-                        for (int part = 1; part < 3; part++) {
-#pragma unroll
-                            for (int j = 0; j < 64; j++) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
-                            send_16(store, v, false, &maps.out[0], (int)column, (int)row0, part);
-                        }
-                } else {
+                for (int c = 0; c < half_columns; c += 64) {
+                    const long long column = column0 + c, left = p.columns - column;
+                    if (left <= 0) break;                                   // the warp together
+                    float v[64];
+                    tmem_load64(tile + buffer * 256 + c, v);
+                    if (c + 64 >= half_columns || left <= 64) leave();
 #pragma unroll
                     for (int j = 0; j < 64; j++) v[j] *= out_scale;
                     if (row0 >= p.rows) continue;
@@ -471,18 +431,91 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
                     if (p.type == GTM_F32) send_32(store, v, &maps.out[w.which], (int)column, (int)row0, slice, p.add || !w.fresh, left);
                     else send_16(store, v, p.type == GTM_F16, &maps.out[w.which], (int)column, (int)row0, slice);
                 }
+                if (column0 >= p.columns) leave();                          // no column of this half
+            } else {
+                float normaliser = 0.f, factor = 0.f;
+                int label = -1;
+                if ((kMode == kSums || kMode == kProb) && real && l.labels) label = l.labels[row] - l.first_label;
+                if (kMode == kProb && real) {
+                    normaliser = l.normalisers[row], factor = l.factors[row];
+                    if (l.largest) {
+                        // a factor that is not finite has no part in the largest: it is its example's alone
+                        factor = factor == 0.f ? 0.f : isfinite(factor) ? factor / __uint_as_float(*l.largest) * 16384.f : __int_as_float(0x7fffffff);
+                    }
+                }
+                float sum[128];                   // a tile's logits of the lane's row, added up chunk by chunk
+                for (int done = 0; done < p.depth_blocks; done += p.chunk) {
+                    fine = barrier_wait(sums_full + 8 * buffer, buffer_phase);
+                    if (!__all_sync(~0u, fine)) break;
+                    tmem_after_sync();
+                    const unsigned from = tile + buffer * 256;
+#pragma unroll
+                    for (int c = 0; c < 128; c += 32) {
+                        if (c >= half_columns || column0 + c >= p.columns) break;
+                        if (done == 0) {
+                            tmem_load32(from + c, reinterpret_cast<float (&)[32]>(sum[c]));
+                        } else {
+                            float more[32];
+                            tmem_load32(from + c, more);
+#pragma unroll
+                            for (int j = 0; j < 32; j++) sum[c + j] += more[j];
+                        }
+                    }
+                    leave();
+                }
+                if (!__all_sync(~0u, fine)) break;
+                RowSums sums = RowSums::none();
+                RowBest best = RowBest::none();
+#pragma unroll
+                for (int c = 0; c < 128; c += 64) {
+                    const long long column = column0 + c, left = p.columns - column;
+                    if (c >= half_columns || left <= 0) break;              // the warp together
+                    float (&v)[64] = reinterpret_cast<float (&)[64]>(sum[c]);
+                    if (kMode == kSums || kMode == kBest) {
+                        if (left < 64)
+#pragma unroll
+                            for (int j = 0; j < 64; j++)
+                                if (j >= left) v[j] = -INFINITY;
+                        if (kMode == kSums) {
+                            sums.take(v, l.scale * kLog2e);
+                            const long long at = label - column;
+                            if (__any_sync(~0u, at >= 0 && at < 64 && label >= 0)) {
+                                float mine = 0.f;
+#pragma unroll
+                                for (int j = 0; j < 64; j++)
+                                    if (at == j) mine = v[j];
+                                if (label >= 0 && at >= 0 && at < 64 && real) l.label_logit[row] = mine;
+                            }
+                        } else {
+                            best.take(v, l.scale * kLog2e, (int)column);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 64; j++) v[j] = exp2_fast(fmaf(v[j], l.scale, -normaliser) * kLog2e);
+                        const long long at = label - column;
+                        if (__any_sync(~0u, at >= 0 && at < 64))
+#pragma unroll
+                            for (int j = 0; j < 64; j++)
+                                if (at == j) v[j] -= 1.f;
+#pragma unroll
+                        for (int j = 0; j < 64; j++) v[j] = factor == 0.f ? 0.f : v[j] * factor;
+                        if (row0 >= p.rows) continue;                       // the warp together
+                        send_16(store, v, p.type == GTM_F16, &maps.out[0], (int)column, (int)row0, 0);
+                        if (p.products > 1)
+#pragma unroll 1
+                            for (int part = 1; part < 3; part++) {
+#pragma unroll
+                                for (int j = 0; j < 64; j++) v[j] -= __bfloat162float(__float2bfloat16_rn(v[j]));
+                                send_16(store, v, false, &maps.out[0], (int)column, (int)row0, part);
+                            }
+                    }
+                }
+                if ((kMode == kSums || kMode == kBest) && real) {
+                    const long long at = (w.n * 2ll + half) * p.rows + row;
+                    l.sums[at] = kMode == kSums ? make_float2(sums.largest, sums.sum) : make_float2(best.largest, best.rest);
+                    if (kMode == kBest) l.best[at] = best.index;
+                }
             }
-            if (column0 >= p.columns) {                                     // no column of this half
-                tmem_before_sync();
-                __syncwarp();
-                if (lane == 0) barrier_arrive_leader(in_leader(sums_empty + 8 * buffer));
-            }
-            if ((kMode == kSums || kMode == kBest) && real) {
-                const long long at = (w.n * 2ll + half) * p.rows + row;
-                l.sums[at] = kMode == kSums ? make_float2(sums.largest, sums.sum) : make_float2(best.largest, best.rest);
-                if (kMode == kBest) l.best[at] = best.index;
-            }
-            if (halves || ++buffer == 2) buffer = 0, buffer_phase ^= 1;
         }
         if (kStores) BoxStore::finish();
     }
@@ -960,6 +993,12 @@ int launch_product(const Maps &maps, Launch &l, cudaStream_t stream)
     if (!error) {
         GTM_CU(cudaGetSymbolAddress(&error, softmax_error));
         GTM_CU(cudaFuncSetAttribute(softmax_product_kernel<kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared_of(kMode)));
+        if (kMode != kOut) {
+            // built otherwise, its epilogue would wait for registers for good
+            cudaFuncAttributes built;
+            GTM_CU(cudaFuncGetAttributes(&built, softmax_product_kernel<kMode>));
+            if (built.numRegs < kLaunchedRegisters) return fail(GTM_ERR_CUDA, "the product kernel is built for %d registers a thread instead of %d", built.numRegs, kLaunchedRegisters);
+        }
         if (device < 64) errors[device].store(error);
     }
     l.error = (int *)error;
@@ -986,13 +1025,14 @@ Product product_of(int64_t rows, int64_t columns, int64_t depth, int products, i
     return p;
 }
 
-// The scale of logits from the tensor cores: sums that are cut off are too small, for terms of both signs by 1.5e-8 at every step of 16
-// elements (measured from 64 to 8,192 elements; 4e-8 to 7e-8 for thousands of terms of one sign, nothing for whole numbers), which the scale makes up for.
-// Losses of 8,192 examples and 1,024 columns are 3e-7 off with it, 1e-6 without.
-float scale_of(const Product &p, int64_t columns, float scale)
+// Blocks of the index whose products follow each other in tensor memory, for logits.  What the tensor cores cut off a sum grows with the square of its steps, so there
+// are up to four blocks (256 elements, 16 steps), two for 32-bit inputs, and two sums from three blocks on; losses of 16-bit inputs are then as far from 64 bits as
+// those of plain 32-bit products, from 64 to 2,048 columns.  Statistics of 8,192 x 1,024 bf16 and 65,536 labels take 833 us so, 787 in sums of
+// eight blocks, 900 of three: the epilogue reads tensor memory while products write to it.
+int logits_chunk(const Product &p)
 {
-    const double steps = columns / (p.products == 1 ? 16.0 : 32.0);
-    return (float)(scale * (1.0 + 1.5e-8 * steps));
+    const int most = p.products == 1 ? 4 : 2, chunks = std::max((p.depth_blocks + most - 1) / most, p.depth_blocks > 2 ? 2 : 1);
+    return (p.depth_blocks + chunks - 1) / chunks;
 }
 
 // One product alone, its tiles in turn.
@@ -1257,13 +1297,13 @@ int forward(Call &c, const void *labels, int labels_64, int64_t ignored, float s
         Launch l = {};
         Maps maps = {};
         Product &p = l.p[0] = product_of(n, c.labels, c.columns, c.products, tile_columns(c.examples, c.labels));      // as the workspace has it
-        p.m_fast = 1;
+        p.m_fast = 1, p.chunk = logits_chunk(p);
         l.schedule = in_turn(p);
-        l.scale = scale_of(p, c.columns, scale), l.sums = sums, l.best = indices, l.label_logit = label_logit, l.labels = labels ? rows + r : nullptr;
+        l.scale = scale, l.sums = sums, l.best = indices, l.label_logit = label_logit, l.labels = labels ? rows + r : nullptr;
         GTM_TRY(set_operands(maps, p, 0, piece, weights, nullptr));
         if (labels) GTM_TRY(launch_product<kSums>(maps, l, stream));
         else GTM_TRY(launch_product<kBest>(maps, l, stream));
-        GTM_TRY(join(r, n, p.n_tiles * 2, l.scale));
+        GTM_TRY(join(r, n, p.n_tiles * 2, scale));
     }
     return GTM_OK;
 }
@@ -1393,9 +1433,9 @@ extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type
             Maps maps = {};
             Product &p = l.p[0] = product_of(examples, n, columns, c.products);
             // x stays in L2 while the labels pass, or the piece's labels while the examples do
-            p.m_fast = x_bytes <= 64 << 20 || x_bytes <= n * columns * 2 * c.parts, p.b_row = (int)v, p.type = type;
+            p.m_fast = x_bytes <= 64 << 20 || x_bytes <= n * columns * 2 * c.parts, p.b_row = (int)v, p.type = type, p.chunk = logits_chunk(p);
             l.schedule = in_turn(p);
-            l.scale = scale_of(p, columns, scale), l.labels = rows, l.first_label = (int)v, l.normalisers = normalisers, l.factors = factors, l.largest = largest;
+            l.scale = scale, l.labels = rows, l.first_label = (int)v, l.normalisers = normalisers, l.factors = factors, l.largest = largest;
             GTM_TRY(set_operands(maps, p, 0, x, piece, &prob));
             GTM_TRY(launch_product<kProb>(maps, l, stream));
         }

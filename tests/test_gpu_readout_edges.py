@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from graphtsetlinmachine_b200 import readout
-from test_gpu_readout import STEP, TYPES, _library, check_gradient, check_loss, generator, half, least, near, normal, softmax_case  # noqa: F401  (_library: no wait ran out)
+from test_gpu_readout import F32, STEP, TYPES, _library, check_gradient, check_loss, generator, half, least, near, normal, softmax_case  # noqa: F401  (_library: no wait ran out)
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +69,36 @@ def test_few_labels_and_many_examples(kind, n, d, v):
     labels[::9] = -1
     normalisers = check_loss(x, w, labels, 1.25)
     check_gradient(x, w, labels, normalisers, normal(generator(n), n).abs() + 0.1, 1.25)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,d,v", [(3, 4096, 300), (16, 4096, 300), (16, 32768, 300), (300, 2048, 1000), (9, 700, 40)])
+def test_softmax_of_whole_numbers_of_one_sign(kind, n, d, v):
+    """Logits without a rounding: what is left is the exponentials' and the sums', however many columns there are and whichever kernel multiplies."""
+    gen = generator(n + d)
+    x, w = torch.randint(0, 3, (n, d), generator=gen, device="cuda"), torch.randint(0, 3, (v, d), generator=gen, device="cuda")
+    scale = 2.0 ** -6
+    logits = (x.double() @ w.double().t()) * scale
+    normaliser, top = torch.logsumexp(logits, 1), logits.amax(1)
+    x, w = x.to(kind), w.to(kind)
+    _, log_probability = readout.softmax_predict(x, w, scale=scale)
+    losses, normalisers = readout.softmax_loss(x, w, logits.argmax(1), scale=scale)
+    # an exponential's argument is rounded twice: 2^-22 of the distance to the largest logit, on the average under the softmax
+    mean = (torch.softmax(logits, 1) * (top[:, None] - logits)).sum(1)
+    bound = 2.0 ** -20 * (1 + (top - normaliser).abs()) + 2.0 ** -22 * mean
+    near(log_probability, top - normaliser, bound)
+    near(losses, normaliser - top, bound)
+    near(normalisers, normaliser, bound + 2.0 ** -22 * normaliser)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,d,v", [(16, 1024, 300), (16, 32768, 300), (16, 131072, 300), (5, 20000, 40)])
+def test_softmax_of_long_sums_of_one_sign(kind, n, d, v):
+    """What tensor cores cut off a sum of one sign adds up: steps of 16 lose less than 2^-22 of it each, 16 in a chunk of 256 elements (of 32-bit inputs: fewer large
+    ones in a chunk of 128); chunks are added with rounding, 2^-24 each.  The scale leaves one label, so that the normaliser is its logit."""
+    gen = generator(n + d)
+    x, w = normal(gen, n, d).abs().to(kind), (normal(gen, v, d).abs() / 1024).to(kind)
+    logits = x.double() @ w.double().t() * 1024.0
+    _, normalisers = readout.softmax_loss(x, w, logits.argmax(1), scale=1024.0)
+    want = torch.logsumexp(logits, 1)
+    near(normalisers, want, (16 * 2.0 ** -22 + (d / (128 if kind == F32 else 256) + 4) * 2.0 ** -24) * want)
