@@ -91,6 +91,7 @@ PROTOTYPES = {
     "gtm_softmax_predict": [C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_float, C.c_void_p,
                             C.c_void_p, C.c_void_p, C.c_uint64],
     "gtm_softmax_failed": [C.c_int, C.POINTER(C.c_int)],
+    "gtm_debug_softmax_lose": [C.c_int],
     "gtm_adamw_step": [C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p,
                        C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, C.c_uint32],
     "gtm_dataset_create_scored": [C.c_void_p, C.POINTER(GraphsView), C.c_int, C.c_void_p, C.POINTER(C.c_void_p)],

@@ -66,14 +66,14 @@ __device__ __forceinline__ unsigned long long nanoseconds()
     return t;
 }
 
-// Waits for a phase of a barrier, ten seconds at most.  The clock is asked only once a usual wait is over.
-__device__ __forceinline__ bool barrier_wait(unsigned barrier, unsigned parity)
+// Waits for a phase of a barrier, `limit` nanoseconds at most.  The clock is asked only once a usual wait is over.
+__device__ __forceinline__ bool barrier_wait(unsigned barrier, unsigned parity, unsigned long long limit)
 {
 #pragma unroll 1
-    for (int i = 0; i < 4096; i++)
+    for (int i = 0; i < 64; i++)
         if (barrier_try(barrier, parity)) return true;
     const unsigned long long began = nanoseconds();
-    while (nanoseconds() - began < 10000000000ull)
+    while (nanoseconds() - began < limit)
 #pragma unroll 1
         for (int i = 0; i < 64; i++)
             if (barrier_try(barrier, parity)) return true;

@@ -111,7 +111,9 @@ struct Maps {
 struct Launch {
     Product p[2];
     Schedule schedule;
-    int *error;
+    unsigned *error;                            // counts waits that ran out
+    unsigned long long limit;                   // of a wait, nanoseconds
+    int lost;                                   // copies are left out, so that waits run out
     // kSums, kBest
     float2 *sums;                               // [part][rows]: largest product and sum of exponentials (kBest: all but the largest's)
     int *best;                                  // [part][rows]
@@ -326,7 +328,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
         if (warp == 0 && lane == 0) {
             // copies: the ring's stages of this block, counted on the leader's barriers
             int stage = 0, phase = 0;
-            for (Work<kMode == kOut> w(l); fine && w.next();) {
+            for (Work<kMode == kOut> w(l); fine && !l.lost && w.next();) {
                 const Product &p = l.p[w.which];
                 const CUtensorMap *map_a = &maps.a[w.which], *map_b = &maps.b[w.which];
                 const int half_columns = p.tile_columns / 2;
@@ -335,7 +337,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
                 int chunk_first = w.first == 0 ? 0 : w.first / (p.chunk * p.products) * p.chunk, chunk_blocks = min(p.chunk, p.depth_blocks - chunk_first);
                 int product = w.first == 0 ? 0 : (w.first - chunk_first * p.products) / chunk_blocks, block = w.first - chunk_first * p.products - product * chunk_blocks;
                 for (int i = w.first; i < w.last; i++) {
-                    if (!(fine = barrier_wait(empty + 8 * stage, phase ^ 1))) break;
+                    if (!(fine = barrier_wait(empty + 8 * stage, phase ^ 1, l.limit))) break;
                     const unsigned to = ring + stage * kStageBytes, bar = in_leader(full + 8 * stage);
                     if (rank == 0) barrier_expect(full + 8 * stage, 2 * (kHalfBytes + half_columns * kDepth * 2));
                     int part_a, part_b;
@@ -354,7 +356,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
             }
             // the products' last arrivals come to this block's barriers before it ends
             for (int i = 0; i < kStages && fine; i++) {
-                fine = barrier_wait(empty + 8 * stage, phase ^ 1);
+                fine = barrier_wait(empty + 8 * stage, phase ^ 1, l.limit);
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
             // copies that nobody will wait for any more end before the block does: 20 ms are thousands of times what one takes
@@ -372,11 +374,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
                 const int chunk = kMode == kOut ? w.last - w.first : p.chunk * p.products;
                 for (int first = w.first; fine && first < w.last; first += chunk) {
                     const unsigned to = tmem + buffer * 256, sums = sums_full + 8 * buffer;
-                    if (!drained && !(fine = barrier_wait(sums_empty + 8 * buffer, buffer_phase ^ 1))) break;
+                    if (!drained && !(fine = barrier_wait(sums_empty + 8 * buffer, buffer_phase ^ 1, l.limit))) break;
                     if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
                     const int blocks = min(chunk, w.last - first);
                     for (int i = 0; i < blocks; i++) {
-                        if (!loaded && !(fine = barrier_wait(full + 8 * stage, phase))) break;
+                        if (!loaded && !(fine = barrier_wait(full + 8 * stage, phase, l.limit))) break;
                         tmem_after_sync();
                         const unsigned a = ring + stage * kStageBytes, b = a + kHalfBytes, done = empty + 8 * stage;
                         if (++stage == kStages) stage = 0, phase ^= 1;
@@ -403,6 +405,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
             const bool real = row < p.rows;
             const long long column0 = (long long)w.n * p.tile_columns + half * half_columns;
             const unsigned tile = tmem + half * half_columns + ((unsigned)(quarter * 32) << 16);
+            // Whichever wait of the pair runs out, this one does too.  What was not multiplied is NaN then, in this tile and in those that are to come
+            const auto arrived = [&] {
+                if (fine) fine = __all_sync(~0u, barrier_wait(sums_full + 8 * buffer, buffer_phase, l.limit));
+                if (fine) tmem_after_sync();
+                return fine;
+            };
             const auto leave = [&] {
                 // the tile's last columns are in registers: the next but one may overwrite it
                 tmem_before_sync();
@@ -413,16 +421,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
             if constexpr (kMode == kOut) {
                 const int slice = w.slice();
                 const float out_scale = p.out_scale ? __uint_as_float(*p.out_scale) * (1.f / 16384.f) : 1.f;
-                fine = barrier_wait(sums_full + 8 * buffer, buffer_phase);
-                if (!__all_sync(~0u, fine)) break;
-                tmem_after_sync();
+                arrived();
 #pragma unroll 1
                 for (int c = 0; c < half_columns; c += 64) {
                     const long long column = column0 + c, left = p.columns - column;
                     if (left <= 0) break;                                   // the warp together
                     float v[64];
-                    tmem_load64(tile + buffer * 256 + c, v);
-                    if (c + 64 >= half_columns || left <= 64) leave();
+                    if (fine) {
+                        tmem_load64(tile + buffer * 256 + c, v);
+                        if (c + 64 >= half_columns || left <= 64) leave();
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 64; j++) v[j] = __int_as_float(0x7fffffff);
+                    }
 #pragma unroll
                     for (int j = 0; j < 64; j++) v[j] *= out_scale;
                     if (row0 >= p.rows) continue;
@@ -431,7 +442,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
                     if (p.type == GTM_F32) send_32(store, v, &maps.out[w.which], (int)column, (int)row0, slice, p.add || !w.fresh, left);
                     else send_16(store, v, p.type == GTM_F16, &maps.out[w.which], (int)column, (int)row0, slice);
                 }
-                if (column0 >= p.columns) leave();                          // no column of this half
+                if (fine && column0 >= p.columns) leave();                  // no column of this half
             } else {
                 float normaliser = 0.f, factor = 0.f;
                 int label = -1;
@@ -445,9 +456,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
                 }
                 float sum[128];                   // a tile's logits of the lane's row, added up chunk by chunk
                 for (int done = 0; done < p.depth_blocks; done += p.chunk) {
-                    fine = barrier_wait(sums_full + 8 * buffer, buffer_phase);
-                    if (!__all_sync(~0u, fine)) break;
-                    tmem_after_sync();
+                    if (!arrived()) break;
                     const unsigned from = tile + buffer * 256;
 #pragma unroll
                     for (int c = 0; c < 128; c += 32) {
@@ -463,7 +472,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
                     }
                     leave();
                 }
-                if (!__all_sync(~0u, fine)) break;
+                if (!fine)
+#pragma unroll
+                    for (int j = 0; j < 128; j++) sum[j] = __int_as_float(0x7fffffff);
                 RowSums sums = RowSums::none();
                 RowBest best = RowBest::none();
 #pragma unroll
@@ -519,7 +530,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
         }
         if (kStores) BoxStore::finish();
     }
-    if (!fine) atomicExch(l.error, 1);
+    if (!fine && lane == 0) atomicAdd(l.error, 1u);
     __syncwarp();
     tmem_before_sync();
     cluster_sync();
@@ -971,7 +982,10 @@ int make_map(CUtensorMap *map, const Matrix &a, unsigned box_columns, unsigned b
     return GTM_OK;
 }
 
-__device__ int softmax_error;                    // set by a wait that ran out
+__device__ unsigned softmax_error;               // counts waits that ran out
+
+constexpr unsigned long long kWait = 10000000000ull, kShortWait = 50000000ull;      // nanoseconds
+thread_local int lost_launches;                  // of the calling thread that are to come: their waits run out
 
 int set_operands(Maps &maps, Product &p, int which, const Matrix &a, const Matrix &b, const Matrix *out)
 {
@@ -1001,7 +1015,9 @@ int launch_product(const Maps &maps, Launch &l, cudaStream_t stream)
         }
         if (device < 64) errors[device].store(error);
     }
-    l.error = (int *)error;
+    l.error = (unsigned *)error;
+    l.limit = kWait, l.lost = 0;
+    if (lost_launches > 0) lost_launches--, l.limit = kShortWait, l.lost = 1;
     const unsigned pairs = (unsigned)(l.schedule.units ? l.schedule.pairs : std::min(l.schedule.items, l.schedule.pairs));
     return launch_early(softmax_product_kernel<kMode>, dim3(2 * pairs), dim3(kThreads), shared_of(kMode), stream, maps, l);
 }
@@ -1463,12 +1479,22 @@ extern "C" int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type
 
 extern "C" int gtm_softmax_failed(int device, int *failed_out)
 {
+    static thread_local unsigned known[64];      // counts that the thread was told of: no question hides a failure from another thread
     if (!failed_out) return fail(GTM_ERR_ARG, "gtm_softmax_failed: null output");
+    if (device < 0 || device >= 64) return fail(GTM_ERR_ARG, "gtm_softmax_failed: device %d (0 to 63)", device);
     DeviceGuard guard(device);
     GTM_TRY(guard.status);
-    const int zero = 0;
+    unsigned count = 0;
     GTM_CU(cudaDeviceSynchronize());
-    GTM_CU(cudaMemcpyFromSymbol(failed_out, softmax_error, sizeof(int)));
-    GTM_CU(cudaMemcpyToSymbol(softmax_error, &zero, sizeof(int)));
+    GTM_CU(cudaMemcpyFromSymbol(&count, softmax_error, sizeof count));
+    *failed_out = count != known[device];
+    known[device] = count;
+    return GTM_OK;
+}
+
+extern "C" int gtm_debug_softmax_lose(int launches)
+{
+    if (launches < 0) return fail(GTM_ERR_ARG, "gtm_debug_softmax_lose: %d launches", launches);
+    lost_launches = launches;
     return GTM_OK;
 }

@@ -226,8 +226,8 @@ def softmax_predict(features, weights, scale=1.0):
 
 
 def softmax_failed(device=0):
-    """Whether a wait inside a softmax kernel (ten seconds at most) ran out on the device since the last question: results since then are
-    not to be used.  Waits for the device."""
+    """Whether a wait inside a softmax kernel (ten seconds at most) ran out on the device since the calling thread asked last.  What could not be
+    computed then is NaN (a label -1) in the call's results.  Waits for the device."""
     failed = C.c_int()
     _lib.check(_lib.load().gtm_softmax_failed(int(device), C.byref(failed)))
     return bool(failed.value)
@@ -382,6 +382,7 @@ class ClauseReadout:
         ends = offsets.cpu().numpy()
         labels = torch.from_numpy(Y.astype(np.int64)).to(self.device)
         history = []
+        softmax_failed(self.device.index)                            # of others before
         for _ in range(epochs):
             total = torch.zeros((), device=self.device)
             for first in range(0, len(Y), batch_size):
@@ -389,7 +390,13 @@ class ClauseReadout:
                 bags = (offsets[first:last + 1] - offsets[first]).contiguous()
                 total += self._step(ids[int(ends[first]):int(ends[last])], bags, labels[first:last]).sum()
             history.append(total / len(Y))
-        return [float(v) for v in history]
+        history = [float(v) for v in history]
+        self._complete()
+        return history
+
+    def _complete(self):
+        if softmax_failed(self.device.index):
+            raise RuntimeError("a wait inside a softmax kernel ran out: what it was to compute is missing")
 
     def gradients(self, ids, offsets, labels):
         """(losses, gradients of the two weight matrices for their mean) of a batch of bags."""
@@ -411,8 +418,10 @@ class ClauseReadout:
         if self.number_of_outputs is None:
             raise RuntimeError("the readout is not fitted")
         features = embed(self.copies[0], *self.active_clauses(graphs), scale=self._scale())
-        labels, log_probabilities = softmax_predict(features, self.copies[1])
-        return labels.cpu().numpy(), log_probabilities.cpu().numpy()
+        labels, log_probabilities = (t.cpu().numpy() for t in softmax_predict(features, self.copies[1]))
+        if np.isnan(log_probabilities).any():
+            self._complete()
+        return labels, log_probabilities
 
     def predict(self, graphs):
         return self.score(graphs)[0]

@@ -282,8 +282,9 @@ int gtm_softmax_loss_gradient(int device, void *cuda_stream, int type, const voi
 int gtm_softmax_predict(int device, void *cuda_stream, int type, const void *features, int64_t examples, int64_t features_stride, const void *weights,
                         int64_t number_of_labels, int64_t weights_stride, int64_t columns, float scale, int64_t *labels_out, float *log_probabilities_out,
                         void *workspace, uint64_t workspace_bytes);
-/* Waits for the device and tells whether a wait inside a softmax kernel ran out since the last call (*failed_out = 0 or 1, then cleared).  Such
- * waits are bounded at ten seconds; results of a call in which one ran out are not to be used. */
+/* Waits for the device and tells whether a wait inside a softmax kernel ran out on it since the calling thread asked last, or since the library was
+ * loaded (*failed_out = 0 or 1).  Such waits are bounded at ten seconds.  What a call could not compute because one ran out is NaN (a predicted
+ * label -1) in its results. */
 int gtm_softmax_failed(int device, int *failed_out);
 
 /* One AdamW step over a list of tensors, in place: with t = *steps + 1 (*steps, int64 in device memory, is then counted up), g = gradient *
@@ -313,6 +314,9 @@ int gtm_debug_evaluate(gtm_model *model, gtm_dataset *dataset, int number_of_nod
                        uint32_t *cno_out, uint32_t *messages_out, int32_t *n_inc_out, int32_t *class_sum_out);
 int gtm_debug_last_feedback(gtm_model *model, int32_t *clause_node_out, int32_t *class_clause_update_out);
 int gtm_debug_last_fit_kernel(gtm_model *model, int32_t *info_out);
+/*  gtm_debug_softmax_lose: the next `launches` product kernels that the calling thread's softmax calls launch multiply nothing: their copies are left out, so
+ *   that their waits, 50 ms each then, run out. */
+int gtm_debug_softmax_lose(int launches);
 
 /* Profiling tap (no counterpart in the reference): SM clock cycles that the first warp of CTA 0 of the last gtm_fit launch
  * spent in its phases.  Chain kernel: uint64[8] = {clause evaluation of message layers, waiting at grid barriers, waiting for

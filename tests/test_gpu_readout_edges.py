@@ -4,12 +4,16 @@ terms of one sign - and in calls that the usual sizes do not make.
 Tolerances count roundings, as in test_gpu_readout."""
 
 import math
+import threading
 
+import numpy as np
 import pytest
 import torch
 
-from graphtsetlinmachine_b200 import readout
+from graphtsetlinmachine_b200 import _lib, readout
+from graphtsetlinmachine_b200.tm import MultiClassGraphTsetlinMachine
 from test_gpu_readout import F32, STEP, TYPES, _library, check_gradient, check_loss, generator, half, least, near, normal, softmax_case  # noqa: F401  (_library: no wait ran out)
+from util import random_graphs
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +106,72 @@ def test_softmax_of_long_sums_of_one_sign(kind, n, d, v):
     _, normalisers = readout.softmax_loss(x, w, logits.argmax(1), scale=1024.0)
     want = torch.logsumexp(logits, 1)
     near(normalisers, want, (16 * 2.0 ** -22 + (d / (128 if kind == F32 else 256) + 4) * 2.0 ** -24) * want)
+
+
+# ------------------------------------------------------------------------------------------- waits that run out
+def lose(launches):
+    """The next product kernels wait 50 ms for copies that do not come."""
+    _lib.check(_lib.load().gtm_debug_softmax_lose(launches))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,d,v", [(300, 200, 700), (70, 40, 33)])
+def test_a_wait_that_runs_out_leaves_no_numbers(kind, n, d, v):
+    x, w, labels = softmax_case(kind, n, d, v)
+    labels[::5] = -1
+    one = torch.ones(1, device="cuda")
+    fine = [*readout.softmax_loss(x, w, labels), *readout.softmax_predict(x, w)]
+    fine += readout.softmax_loss_gradient(x, w, labels, fine[1], one)
+    assert not readout.softmax_failed()
+    lose(1)
+    losses, normalisers = readout.softmax_loss(x, w, labels)
+    assert torch.isnan(losses[labels != -1]).all() and torch.isnan(normalisers).all() and readout.softmax_failed() and not readout.softmax_failed()
+    lose(1)
+    label, log_probability = readout.softmax_predict(x, w)
+    assert (label == -1).all() and torch.isnan(log_probability).all() and readout.softmax_failed()
+    for launches, rows in ((1, labels != -1), (2, labels == labels)):               # P, or what is made of it too
+        lose(launches)
+        dx, dw = readout.softmax_loss_gradient(x, w, labels, fine[1], one)
+        assert torch.isnan(dx[rows]).all() and torch.isnan(dw).all() and readout.softmax_failed()
+    # and nothing is left of it
+    again = [*readout.softmax_loss(x, w, labels), *readout.softmax_predict(x, w)]
+    again += readout.softmax_loss_gradient(x, w, labels, again[1], one)
+    assert all(torch.equal(a, b) for a, b in zip(again, fine)) and not readout.softmax_failed()
+
+
+def test_a_question_hides_no_failure_from_another_thread():
+    x, w, labels = softmax_case(F32, 20, 16, 40)
+    assert not readout.softmax_failed()
+    told = []
+    thread = threading.Thread(target=lambda: told.append(readout.softmax_failed()))      # what came before is not its matter
+    thread.start()
+    thread.join()
+    lose(1)
+    readout.softmax_loss(x, w, labels)
+    thread = threading.Thread(target=lambda: told.append(readout.softmax_failed()))
+    thread.start()
+    thread.join()
+    assert told[1] and readout.softmax_failed() and not readout.softmax_failed()
+
+
+def test_a_classifier_tells_of_a_wait_that_ran_out():
+    rng = np.random.default_rng(7)
+    graphs, labels = random_graphs(60, rng, max_nodes=5), rng.permutation(60) % 40
+    np.random.seed(4)
+    tm = MultiClassGraphTsetlinMachine(40, 100, 2.0, depth=1, seed=1)
+    tm.fit(graphs, labels % 3, epochs=1)
+    head = readout.ClauseReadout(tm, embedding_size=24)
+    head.fit(graphs, labels, epochs=1)
+    before = head.score(graphs)
+    lose(1)
+    with pytest.raises(RuntimeError, match="ran out"):
+        head.score(graphs)
+    after = head.score(graphs)
+    assert all(np.array_equal(a, b) for a, b in zip(before, after))
+    for launches in (1, 2, 3):
+        lose(launches)
+        with pytest.raises(RuntimeError, match="ran out"):
+            head.fit(graphs, labels, epochs=1)
+    lose(1)
+    readout.softmax_loss(*softmax_case(F32, 20, 16, 40))                     # not the classifier's matter
+    assert all(math.isfinite(v) for v in head.fit(graphs, labels, epochs=1))
