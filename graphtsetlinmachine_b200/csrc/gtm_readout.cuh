@@ -53,10 +53,11 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// Element `i` of an array of int32 or int64.
+// Element `i` of an array of int32 or int64.  Not by the read-only path: the kernels begin while the one before them still writes, and what that path
+// loads must not change as long as a kernel lives.
 __device__ __forceinline__ long long index_at(const void *p, int wide, long long i)
 {
-    return wide ? __ldg((const long long *)p + i) : (long long)__ldg((const int *)p + i);
+    return wide ? ((const long long *)p)[i] : (long long)((const int *)p)[i];
 }
 
 // The kernel behind this one may be set up while this one ends, and waits for its end before it reads what others have written.
