@@ -13,6 +13,10 @@
 // repeated.  A u above zero never gets the code of zero, or the next step would divide m by eps alone.
 #include "gtm_readout.cuh"
 
+#include <algorithm>
+#include <memory>
+#include <new>
+
 namespace gtm_readout {
 namespace {
 
@@ -343,6 +347,25 @@ int launch_all(const AdamHead &head, int64_t number_of_tensors, const int64_t *c
     return GTM_OK;
 }
 
+// Memory that a step touches.
+struct Range {
+    uintptr_t first, end;
+    bool written;
+};
+
+// Whether something written meets anything else: the order of two writes, or of a read and a write, would be open.  Gradients may share memory.
+bool overlap(Range *ranges, size_t count)
+{
+    std::sort(ranges, ranges + count, [](const Range &a, const Range &b) { return a.first < b.first; });
+    uintptr_t written = 0, any = 0;               // ends so far
+    for (size_t i = 0; i < count; i++) {
+        if (ranges[i].first < (ranges[i].written ? any : written)) return true;
+        any = std::max(any, ranges[i].end);
+        if (ranges[i].written) written = std::max(written, ranges[i].end);
+    }
+    return false;
+}
+
 }  // namespace
 }  // namespace gtm_readout
 
@@ -372,6 +395,21 @@ extern "C" int gtm_adamw_step(int device, void *cuda_stream, int64_t number_of_t
     }
     if (all && (!first || !second || (uintptr_t)first % 16 || (uintptr_t)second % 16)) return fail(GTM_ERR_ARG, "gtm_adamw_step: null or misaligned states");
     if (all && narrow && (!first_scales || !second_scales)) return fail(GTM_ERR_ARG, "gtm_adamw_step: 8-bit states need scales");
+    std::unique_ptr<Range[]> ranges(new (std::nothrow) Range[(size_t)number_of_tensors * 3 + 5]);
+    if (!ranges) return fail(GTM_ERR_OOM, "gtm_adamw_step: no memory for a list of %lld tensors", (long long)number_of_tensors);
+    size_t count = 0;
+    const auto take = [&](const void *p, uint64_t bytes, bool written) {
+        if (bytes) ranges[count++] = {(uintptr_t)p, (uintptr_t)p + bytes, written};
+    };
+    uint64_t blocks = 0;
+    for (int64_t i = 0; i < number_of_tensors; i++) {
+        take(params[i], counts[i] * type_bytes(param_type), true), take(gradients[i], counts[i] * type_bytes(gradient_type), false);
+        if (copies) take(copies[i], counts[i] * 2, true);
+        blocks += (counts[i] + kBlock - 1) / kBlock;
+    }
+    take(steps, 8, true), take(first, blocks * kBlock * (narrow ? 1 : 4), true), take(second, blocks * kBlock * (narrow ? 1 : 4), true);
+    if (narrow) take(first_scales, blocks * 4, true), take(second_scales, blocks * 4, true);
+    if (overlap(ranges.get(), count)) return fail(GTM_ERR_ARG, "gtm_adamw_step: a tensor, a state or a copy overlaps another");
     DeviceGuard guard(device);
     GTM_TRY(guard.status);
     cudaStream_t stream = (cudaStream_t)cuda_stream;

@@ -282,7 +282,7 @@ def _address(a):
 def adamw_step(params, gradients, state, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, gradient_scale=1.0, copies=None, seed=0):
     """One AdamW step over a list of tensors, in place, in one launch for up to 512 of them.  ``state`` (see ``adamw_state``) decides
     between states of 32 and of 8 bits, and counts the steps on the device.  All parameters have one type, all gradients have one; ``copies`` (optional,
-    bfloat16 or float16) receive the parameters once more.  States of 8 bits are rounded by a hash of ``seed`` (0 to 2^32 - 1), the step and the
+    bfloat16 or float16) receive the parameters once more; nothing that is written may share memory with anything else.  States of 8 bits are rounded by a hash of ``seed`` (0 to 2^32 - 1), the step and the
     element: the same call gives the same result.  The numbers, ``lr`` among them, are those of the call: a captured step keeps them."""
     params, gradients = list(params), list(gradients)
     if not params:

@@ -292,7 +292,7 @@ int gtm_softmax_failed(int device, int *failed_out);
  * (sqrt(v) / sqrt(1 - beta2^t) + eps).  The states of all tensors lie in two flat arrays in which every tensor starts at a multiple of 256
  * elements (16-byte aligned).  state_bits 32: m and v, float.  state_bits 8: e4m3 codes of m and of sqrt(v) in units of one float scale per 256
  * elements, rounded to one of their two neighbours by a hash of (seed, t, element).  copies (may be NULL) receive the parameters
- * once more, as GTM_BF16 or GTM_F16.  No tensor, state or copy may overlap another. */
+ * once more, as GTM_BF16 or GTM_F16.  No tensor, state or copy may overlap another (refused); gradients may share memory. */
 int gtm_adamw_step(int device, void *cuda_stream, int64_t number_of_tensors, const int64_t *counts, int param_type, const void *const *params,
                    int gradient_type, const void *const *gradients, int copy_type, const void *const *copies, int state_bits, void *first, void *second,
                    float *first_scales, float *second_scales, int64_t *steps, double lr, double beta1, double beta2, double eps, double weight_decay,

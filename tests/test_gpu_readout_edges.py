@@ -175,3 +175,18 @@ def test_a_classifier_tells_of_a_wait_that_ran_out():
     lose(1)
     readout.softmax_loss(*softmax_case(F32, 20, 16, 40))                     # not the classifier's matter
     assert all(math.isfinite(v) for v in head.fit(graphs, labels, epochs=1))
+
+
+# ------------------------------------------------------------------------------------------------------- adamw
+def test_adamw_of_the_same_tensor_twice_is_refused():
+    p = torch.ones(600, device="cuda")
+    for params in ([p, p], [p[:400], p[300:500]]):
+        with pytest.raises(_lib.GtmError, match="overlap"):
+            readout.adamw_step(params, [torch.ones_like(q) for q in params], readout.adamw_state(params), 0.1)
+    with pytest.raises(_lib.GtmError, match="overlap"):
+        readout.adamw_step([p], [p], readout.adamw_state([p]), 0.1)
+    assert (p == 1).all()
+    # one gradient for two parameters, and neighbours in one memory, are fine
+    params, g = [p[:300], p[300:]], torch.ones(300, device="cuda")
+    readout.adamw_step(params, [g, g], readout.adamw_state(params), 0.1)
+    assert torch.equal(params[0], params[1]) and (p < 1).all()
