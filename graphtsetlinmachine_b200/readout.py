@@ -28,6 +28,7 @@ _INDEX = {torch.int32: 0, torch.int64: 1}
 # the current stream's handle, without the object around it where torch has that
 _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 BLOCK = 256      # elements; every tensor starts at a multiple of it in the flat states of `adamw_step`
+OUTPUTS = 1 << 28      # clause outputs, of four bytes each, that `ClauseReadout` has on the host at a time
 
 
 def _cuda(name, t):
@@ -342,12 +343,18 @@ class ClauseReadout:
         self.number_of_outputs = None
         self.device = torch.device("cuda", tm.device)
 
+    def _pieces(self, graphs):
+        """The graphs, or as many of them at a time as have ``OUTPUTS`` clause outputs."""
+        number, most = graphs.number_of_graphs, max(1, OUTPUTS // self.tm.number_of_clauses)
+        if number == 0:
+            raise ValueError("there are no graphs")
+        for first in range(0, number, most):
+            yield graphs if most >= number else graphs[first:min(first + most, number)]
+
     def active_clauses(self, graphs):
         """(ids int32, offsets int64) of the clauses that are active for each graph, on the device: bags for ``embed``."""
-        most = max(1, (1 << 28) // self.tm.number_of_clauses)       # graphs at a time: a clause output has four bytes
         clauses, counts = [], []
-        for first in range(0, graphs.number_of_graphs, most):
-            piece = graphs if most >= graphs.number_of_graphs else graphs[first:min(first + most, graphs.number_of_graphs)]
+        for piece in self._pieces(graphs):
             outputs, _ = self.tm.transform(piece)
             clauses.append(np.nonzero(outputs)[1].astype(np.int32))
             counts.append(np.count_nonzero(outputs, axis=1))
@@ -374,11 +381,12 @@ class ClauseReadout:
             raise ValueError("Y holds one label, zero or more, for each of %d graphs" % graphs.number_of_graphs)
         if batch_size < 1:
             raise ValueError("batch_size %r" % (batch_size,))
-        if self.number_of_outputs is None or not incremental:
-            self._init(int(np.max(Y) + 1))
-        elif int(np.max(Y)) >= self.number_of_outputs:
+        again = self.number_of_outputs is None or not incremental
+        if not again and Y.size and int(np.max(Y)) >= self.number_of_outputs:
             raise ValueError("label %d of a readout of %d labels" % (int(np.max(Y)), self.number_of_outputs))
         ids, offsets = self.active_clauses(graphs)
+        if again:
+            self._init(int(np.max(Y) + 1))
         ends = offsets.cpu().numpy()
         labels = torch.from_numpy(Y.astype(np.int64)).to(self.device)
         history = []
@@ -417,8 +425,11 @@ class ClauseReadout:
         """(labels int64, log probabilities float32) of the most probable label of every graph, numpy arrays."""
         if self.number_of_outputs is None:
             raise RuntimeError("the readout is not fitted")
-        features = embed(self.copies[0], *self.active_clauses(graphs), scale=self._scale())
-        labels, log_probabilities = (t.cpu().numpy() for t in softmax_predict(features, self.copies[1]))
+        scored = []
+        for piece in self._pieces(graphs):
+            features = embed(self.copies[0], *self.active_clauses(piece), scale=self._scale())
+            scored.append([t.cpu().numpy() for t in softmax_predict(features, self.copies[1])])
+        labels, log_probabilities = (np.concatenate(parts) for parts in zip(*scored))
         if np.isnan(log_probabilities).any():
             self._complete()
         return labels, log_probabilities

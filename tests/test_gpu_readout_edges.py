@@ -177,6 +177,29 @@ def test_a_classifier_tells_of_a_wait_that_ran_out():
     assert all(math.isfinite(v) for v in head.fit(graphs, labels, epochs=1))
 
 
+def test_a_classifier_of_more_graphs_than_are_scored_at_a_time(monkeypatch):
+    rng = np.random.default_rng(5)
+    graphs, labels = random_graphs(60, rng, max_nodes=5), rng.integers(0, 3, size=60)
+    np.random.seed(4)
+    tm = MultiClassGraphTsetlinMachine(40, 100, 2.0, depth=1, seed=1)
+    tm.fit(graphs, labels, epochs=1)
+    head = readout.ClauseReadout(tm, embedding_size=24)
+    head.fit(graphs, labels, epochs=1)
+    whole, bags = head.score(graphs), head.active_clauses(graphs)
+    monkeypatch.setattr(readout, "OUTPUTS", 40 * 17 + 3)                          # 17 graphs, the last piece 9
+    pieces = head.score(graphs)
+    assert all(torch.equal(a, b) for a, b in zip(head.active_clauses(graphs), bags))
+    # sums of up to 40 rows in another order, rounded to bfloat16: logits below 8 in magnitude are off by 2^-8 of that
+    assert pieces[0].shape == (60,) and np.abs(pieces[1] - whole[1]).max() <= 2 ** -4
+    # a fit that fails leaves what was learned
+    monkeypatch.setattr(tm, "transform", lambda graphs: 1 / 0)
+    with pytest.raises(ZeroDivisionError):
+        head.fit(graphs, labels + 1, epochs=1)
+    monkeypatch.undo()
+    again = head.score(graphs)
+    assert all(np.array_equal(a, b) for a, b in zip(again, whole))
+
+
 # ------------------------------------------------------------------------------------------------------- adamw
 def test_adamw_of_the_same_tensor_twice_is_refused():
     p = torch.ones(600, device="cuda")

@@ -4,10 +4,11 @@ import ctypes as C
 import glob
 import os
 import re
+from types import SimpleNamespace
 
 import pytest
 
-from graphtsetlinmachine_b200 import _lib
+from graphtsetlinmachine_b200 import _lib, readout
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -42,3 +43,16 @@ def test_steps_over_memory_that_is_written_twice_are_refused(bits, change):
     assert lib.gtm_adamw_step(0, None, 2, (C.c_int64 * 2)(300, 700), 0, _pointers(*a["params"]), 0, _pointers(*a["gradients"]), 1, _pointers(*a["copies"]), bits, a["first"],
                               a["second"], 0xa0000, 0xb0000, a["steps"], 0.1, 0.9, 0.99, 1e-8, 0.0, 1.0, 0) == 1
     assert b"overlap" in lib.gtm_last_error()
+
+
+def test_a_classifier_of_no_graphs_is_refused():
+    none, head = SimpleNamespace(number_of_graphs=0), readout.ClauseReadout(SimpleNamespace(device=0, number_of_clauses=10))
+    for incremental in (False, True):
+        with pytest.raises(ValueError, match="no graphs"):
+            head.fit(none, [], incremental=incremental)
+    with pytest.raises(ValueError, match="no graphs"):
+        head.active_clauses(none)
+    head.number_of_outputs = 3                                   # as after a fit
+    for call in (lambda: head.fit(none, [], incremental=True), lambda: head.score(none), lambda: head.predict(none)):
+        with pytest.raises(ValueError, match="no graphs"):
+            call()
