@@ -12,7 +12,7 @@ import torch
 
 from graphtsetlinmachine_b200 import _lib, readout
 from graphtsetlinmachine_b200.tm import MultiClassGraphTsetlinMachine
-from test_gpu_readout import F32, STEP, TYPES, _library, check_gradient, check_loss, generator, half, least, near, normal, softmax_case  # noqa: F401  (_library: no wait ran out)
+from test_gpu_readout import F32, STEP, TYPES, _library, batch_of, check_gradient, check_loss, flat, generator, half, least, near, normal, plain_softmax, softmax_case, step_of  # noqa: F401  (_library: no wait ran out)
 from util import random_graphs
 
 pytestmark = pytest.mark.gpu
@@ -213,3 +213,120 @@ def test_adamw_of_the_same_tensor_twice_is_refused():
     params, g = [p[:300], p[300:]], torch.ones(300, device="cuda")
     readout.adamw_step(params, [g, g], readout.adamw_state(params), 0.1)
     assert torch.equal(params[0], params[1]) and (p < 1).all()
+
+
+# ------------------------------------------------------------------------- pieces, slices, streams, threads
+@pytest.mark.parametrize("kind", TYPES)
+def test_softmax_in_pieces_of_the_examples(kind):
+    """More parts of statistics than the workspace holds at a time: the second piece of examples begins behind row 35,000."""
+    n, d, v = 40000, 8, 30000
+    x, w, labels = softmax_case(kind, n, d, v)
+    labels[::7] = -1
+    losses, normalisers = readout.softmax_loss(x, w, labels)
+    label, log_probability = readout.softmax_predict(x, w)
+    rows = torch.cat([torch.arange(0, n, 97, device="cuda"), torch.arange(35200, 35500, device="cuda"), torch.tensor([n - 1], device="cuda")])
+    logits, off, normaliser = plain_softmax(x[rows], w, 1.0)
+    bound = off.amax(1) + 2.0 ** -20 + 2.0 ** -22 * normaliser.abs()
+    near(normalisers[rows], normaliser, bound)
+    at = labels[rows]
+    near(losses[rows], torch.where(at >= 0, normaliser - logits[torch.arange(len(rows)), at.clamp_min(0)], 0.0), 2 * bound)
+    top = logits.amax(1)
+    near(log_probability[rows], top - normaliser, 2 * bound)
+    # the label is one of those that cannot be told from the best
+    assert (logits[torch.arange(len(rows)), label[rows]] >= top - 2 * off.amax(1)).all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,d,v", [(9000, 300, 520), (4300, 1100, 260), (300, 5000, 40)])
+def test_softmax_gradient_of_many_tiles(kind, n, d, v):
+    """More than 64 tiles of the features' gradient, whose slices are counted by a bound."""
+    x, w, labels = softmax_case(kind, n, d, v)
+    normalisers = check_loss(x, w, labels, 1.0)
+    check_gradient(x, w, labels, normalisers, torch.full((n,), 1.0 / n, device="cuda"), 1.0)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,d,v", [(50, 40, 70), (40, 30, 9)])
+def test_softmax_gradient_against_differences_along_itself(kind, n, d, v):
+    """Central differences of the formula in 64 bits in the gradient's own direction, where they are its square: what the roundings may be off is
+    a small part of that, so that no gradient would not pass."""
+    x, w, labels = softmax_case(kind, n, d, v)
+    _, normalisers = readout.softmax_loss(x, w, labels)
+    got = readout.softmax_loss_gradient(x, w, labels, normalisers, torch.ones(1, device="cuda"))
+    base, at = [x.double(), w.double()], torch.arange(n)
+    logits, off, normaliser = plain_softmax(x, w, 1.0)
+    p = torch.softmax(logits, 1)
+    q = p.clone()
+    q[at, labels] -= 1.0
+    # of q: the logits' and normalisers' errors, the exponential's 2^-21, the rounding to the operands' type
+    wrong = p * (2 * off.amax(1, keepdim=True) + 2.0 ** -20 + 2.0 ** -22 * normaliser.abs()[:, None]) + max(half(kind), 2.0 ** -22) * q.abs() + 2.0 ** -23
+    bounds = [(wrong + (v + 16) * STEP * q.abs()) @ base[1].abs(), (wrong + (n + 16) * STEP * q.abs()).t() @ base[0].abs()]
+
+    def loss(x, w):
+        logits = x @ w.t()
+        return (torch.logsumexp(logits, 1) - logits[at, labels]).sum()
+
+    for i in (0, 1):
+        way = got[i].double()
+        way = way / way.norm()
+        ends, h = [], 1e-5
+        for sign in (1, -1):
+            moved = list(base)
+            moved[i] = base[i] + sign * h * way
+            ends.append(loss(*moved))
+        want = (ends[0] - ends[1]) / (2 * h)
+        # differences: the third derivative's part h^2, and the losses' 2^-52 over h
+        slack = ((bounds[i] + half(kind) * (got[i].double().abs() + bounds[i])) * way.abs()).sum() + 1e-6 * (1 + want.abs())
+        assert slack <= 0.25 * want and abs((got[i].double() * way).sum() - want) <= slack
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_on_two_streams_at_once(bits):
+    """Two batches in turn on one stream, and at the same time on two: each is what it is alone."""
+    alone = []
+    for seed in (2, 9):
+        batch = batch_of(seed, bits)
+        for _ in range(4):
+            out = step_of(batch)
+        alone.append(flat(out, batch))
+    batches, streams, outs = [batch_of(2, bits), batch_of(9, bits)], [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                outs[k] = step_of(batches[k])
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        assert all(torch.equal(a, b) for a, b in zip(flat(outs[k], batches[k]), alone[k]))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_of_two_threads_at_once(bits):
+    alone, batches, got, failed = [], [batch_of(s, bits) for s in (2, 9)], [None, None], []
+    for seed in (2, 9):
+        batch = batch_of(seed, bits)
+        for _ in range(8):
+            out = step_of(batch)
+        alone.append(flat(out, batch))
+    torch.cuda.synchronize()
+    begin = threading.Barrier(2)
+
+    def steps(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                begin.wait(timeout=60)
+                for _ in range(8):
+                    out = step_of(batches[k])
+                got[k] = flat(out, batches[k])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                    # noqa: BLE001  told by the test
+            failed.append(e)
+
+    threads = [threading.Thread(target=steps, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for k in (0, 1):
+        assert all(torch.equal(a, b) for a, b in zip(got[k], alone[k]))
