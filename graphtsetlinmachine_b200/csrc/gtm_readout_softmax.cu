@@ -638,6 +638,17 @@ __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs 
 }
 
 // ------------------------------------------------------------------------------------------- around the products
+// The next part of a 32-bit value, of which the rest is left: rounded, and towards zero where rounding would leave the range (the lowest value, with which
+// labels are masked, has to stay finite: an infinite part times a part that is zero is no number).
+__device__ __forceinline__ __nv_bfloat16 part_of(float &rest)
+{
+    __nv_bfloat16 part = __float2bfloat16_rn(rest);
+    if (isinf(__bfloat162float(part)) && !isinf(rest)) part = __float2bfloat16_rz(rest);
+    const float held = __bfloat162float(part);
+    rest = isfinite(held) ? rest - held : 0.f;
+    return part;
+}
+
 // Rows of a matrix with 16-byte boundaries, in parts where they are 32-bit ones; rows of examples that are ignored are zero.  A thread has eight
 // elements in a row; kWhole: rows start at 16-byte boundaries and have all eight.
 template <class T, bool kWhole>
@@ -668,11 +679,7 @@ __global__ void __launch_bounds__(256) softmax_lay_out_kernel(const T *from, lon
             for (int p = 0; p < 3; p++) {
                 Pack<__nv_bfloat16, 8> b;
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    b.v[k] = __float2bfloat16_rn(v.v[k]);
-                    const float held = __bfloat162float(b.v[k]);
-                    v.v[k] = fabsf(held) <= 3.4e38f ? v.v[k] - held : 0.f;
-                }
+                for (int k = 0; k < 8; k++) b.v[k] = part_of(v.v[k]);
                 *(Pack<__nv_bfloat16, 8> *)(q + p * part) = b;
             }
         } else {
@@ -712,11 +719,7 @@ __global__ void __launch_bounds__(256) softmax_lay_out_both_kernel(const T *from
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 if constexpr (kParts == 1) b.v[k] = v.v[k];
-                else {
-                    b.v[k] = __float2bfloat16_rn(v.v[k]);
-                    const float held = __bfloat162float(b.v[k]);
-                    v.v[k] = fabsf(held) <= 3.4e38f ? v.v[k] - held : 0.f;
-                }
+                else b.v[k] = part_of(v.v[k]);
             }
             if (r < rows && c < columns) *(Pack<Out, 8> *)((Out *)to + p * part + r * to_stride + c) = b;
             *(Pack<Out, 8> *)&tile[p][r0 + h][c8] = b;

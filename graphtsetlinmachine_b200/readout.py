@@ -9,7 +9,8 @@ other path.  Gradients are functions of their own (``embed_gradient``, ``softmax
 current stream of the tensors' device, whichever device is current, and no call synchronises.  Results, and workspaces, come from
 torch's allocator on that stream, so that calls can be captured into a CUDA graph (after one call outside it has loaded the kernels).
 Matrices are float32, bfloat16 or float16 with any row stride and elements next to each other within a row; a tensor in
-another order is refused, not copied.
+another order is refused, not copied.  The softmax operators multiply float32 matrices in parts on the tensor cores: an infinite
+element gives NaN logits there (mask with the lowest value instead).
 """
 
 import array

@@ -269,6 +269,7 @@ int gtm_embed_gradient(int device, void *cuda_stream, int type, const void *grad
  * With up to 32 labels whose weights take up to 96 KB as floats, and up to 2^16 examples, the loss and the prediction need no workspace (NULL).
  * gtm_softmax_predict gives the most probable label, the lowest of equal ones, and its log probability; -1 and NaN where the logits are
  * not numbers.
+ * GTM_F32 matrices are multiplied in parts (more than 32 labels): an infinite element gives NaN logits there; the lowest value masks a label.
  * what: 0 for the workspace of gtm_softmax_loss, 1 for the gradient's, 2 for gtm_softmax_predict's. */
 int gtm_softmax_workspace(int type, const void *features, int64_t examples, int64_t features_stride, const void *weights, int64_t labels,
                           int64_t weights_stride, int64_t columns, int what, uint64_t *bytes_out);

@@ -330,3 +330,31 @@ def test_steps_of_two_threads_at_once(bits):
     assert not failed
     for k in (0, 1):
         assert all(torch.equal(a, b) for a, b in zip(got[k], alone[k]))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,d,v", [(40, 24, 70), (9, 24, 300), (3, 24, 300), (30, 24, 10)])
+def test_labels_masked_by_the_lowest_value(kind, n, d, v):
+    """A column of ones, and the type's lowest value in it for labels that are not to be: logits of about that, probability zero, no NaN."""
+    x, w, labels = softmax_case(kind, n, d, v)
+    masked = torch.arange(v, device="cuda") % 3 == 1
+    labels = torch.where(masked[labels], labels - 1, labels)
+    x[:, 5], w[:, 5] = 1.0, 0.0
+    kept = (~masked).nonzero()[:, 0]
+    position = torch.zeros(v, dtype=torch.int64, device="cuda")
+    position[kept] = torch.arange(len(kept), device="cuda")
+    w[masked, 5] = torch.finfo(kind).min
+    # as if there were only the other labels
+    logits, off, normaliser = plain_softmax(x, w[kept], 1.0)
+    bound = off.amax(1) + 2.0 ** -20 + 2.0 ** -22 * normaliser.abs()
+    losses, normalisers = readout.softmax_loss(x, w, labels)
+    near(normalisers, normaliser, bound)
+    near(losses, normaliser - logits[torch.arange(n), position[labels]], 2 * bound)
+    label, log_probability = readout.softmax_predict(x, w)
+    near(log_probability, logits.amax(1) - normaliser, 2 * bound)
+    assert not masked[label].any()
+    dx, dw = readout.softmax_loss_gradient(x, w, labels, normalisers, torch.ones(1, device="cuda"))
+    want, _ = readout.softmax_loss_gradient(x, w[kept].contiguous(), position[labels], normalisers, torch.ones(1, device="cuda"))
+    assert torch.isfinite(dx).all() and (dw[masked] == 0).all() and torch.isfinite(dw).all()
+    size = torch.softmax(logits, 1) @ w[kept].double().abs() + w[labels].double().abs()
+    near(dx, want, 4 * max(half(kind), (v + 16) * STEP) * size + least(kind))
