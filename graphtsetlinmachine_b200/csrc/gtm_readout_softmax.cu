@@ -41,6 +41,7 @@ constexpr int kPairs = 74;                                 // pairs of SMs
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int64_t kPieceBytes = 128 << 20;                 // of P in the workspace at a time
 constexpr int64_t kStatBytes = 64 << 20;                   // of partial sums of exponentials at a time
+constexpr int kLongestSum = 512;                           // blocks of a sum in tensor memory, for gradients of 16 bits: 2,048 steps cut off up to 2e-4 of it
 
 enum Epilogue { kSums = 0, kBest = 1, kProb = 2, kOut = 3 };
 __host__ __device__ constexpr int stages_of(int mode) { return mode == kSums || mode == kBest ? 6 : 5; }
@@ -1162,6 +1163,9 @@ void lay_out_workspace(Call &c)
         c.at_factors = take(c.examples * 4);
         c.at_largest = take(4);
         c.piece_labels = piece_of(c.examples, c.labels, c.parts);
+        // a piece's sums of dx are cut as well, by pairs of SMs that share a tile
+        const int64_t dx_tiles = ((c.columns + 255) / 256) * ((c.examples + 255) / 256);
+        if (c.products == 1) c.piece_labels = std::min(c.piece_labels, kLongestSum * kDepth * std::max<int64_t>(1, kPairs / dx_tiles));
         c.prob_ld = (int64_t)round_up(c.piece_labels, 64);
         c.sums_ld = (int64_t)round_up(c.columns, 4);
         c.turned_ld = (int64_t)round_up(c.examples, 8);
@@ -1170,8 +1174,8 @@ void lay_out_workspace(Call &c)
         c.dx = product_of(c.columns, c.examples, c.piece_labels, c.products, c.examples <= 128 ? 128 : 256);      // turned: its operand B is P
         c.dw = product_of(c.piece_labels, c.columns, c.examples, c.products);
         if (c.products > 1) c.dx.chunk = c.dw.chunk = 8;
-        // dw's tiles are cut where they are less than half of the pairs of SMs, into eight blocks or more
-        const int splits = std::max(1, std::min(kPairs / c.dw.tiles(), c.dw.blocks / 8));
+        // dw's tiles are cut where they are less than half of the pairs of SMs, into eight blocks or more, and where sums would be too long
+        const int splits = std::max(std::max(1, std::min(kPairs / c.dw.tiles(), c.dw.blocks / 8)), c.products == 1 ? (c.dw.blocks + kLongestSum - 1) / kLongestSum : 1);
         c.dw.per_split = (c.dw.blocks + splits - 1) / splits;
         c.schedule = together(c.dw, c.dx);
         c.dx_slices = most_slices(c.schedule, c.dx);

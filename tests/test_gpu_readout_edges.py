@@ -12,7 +12,7 @@ import torch
 
 from graphtsetlinmachine_b200 import _lib, readout
 from graphtsetlinmachine_b200.tm import MultiClassGraphTsetlinMachine
-from test_gpu_readout import F32, STEP, TYPES, _library, batch_of, check_gradient, check_loss, flat, generator, half, least, near, normal, plain_softmax, softmax_case, step_of  # noqa: F401  (_library: no wait ran out)
+from test_gpu_readout import F16, F32, STEP, TYPES, _library, batch_of, check_gradient, check_loss, flat, generator, half, least, near, normal, plain_softmax, softmax_case, step_of  # noqa: F401  (_library: no wait ran out)
 from util import random_graphs
 
 pytestmark = pytest.mark.gpu
@@ -358,3 +358,26 @@ def test_labels_masked_by_the_lowest_value(kind, n, d, v):
     assert torch.isfinite(dx).all() and (dw[masked] == 0).all() and torch.isfinite(dw).all()
     size = torch.softmax(logits, 1) @ w[kept].double().abs() + w[labels].double().abs()
     near(dx, want, 4 * max(half(kind), (v + 16) * STEP) * size + least(kind))
+
+
+def test_gradients_of_very_long_sums():
+    """Sums of hundreds of thousands of terms of one sign, where neither product is cut into splits for want of tiles.  What tensor cores cut off is on the
+    average of all results below 2^-23 for each of at most 2,048 steps of 16 terms; results' roundings have no sign."""
+    bound = 2048 * 2.0 ** -23
+    n, d, v = 1 << 18, 38 * 256, 33                              # dw: 38 tiles of 262,144 terms
+    gen = generator(1)
+    x, w = torch.rand(n, d, generator=gen, device="cuda", dtype=F16), torch.zeros(v, d, device="cuda", dtype=F16)
+    labels = torch.arange(n, device="cuda") % 32
+    _, normalisers = readout.softmax_loss(x, w, labels)
+    _, dw = readout.softmax_loss_gradient(x, w, labels, normalisers, torch.full((1,), 1 / 64, device="cuda"))
+    want = torch.stack([x[i::16].double().sum(0) for i in range(16)]).sum(0) / 64 / v      # of the label that no example has
+    assert abs((dw[32].double() / want - 1).mean().item()) <= bound
+    del x, dw
+    n, d, v = 64, 19 * 256, 1 << 20                              # dx: 19 tiles of 1,048,576 terms
+    x, w = torch.zeros(n, d, device="cuda", dtype=F16), torch.rand(v, d, generator=gen, device="cuda", dtype=F16)
+    w[0] = 0.0
+    labels = torch.zeros(n, dtype=torch.int64, device="cuda")
+    _, normalisers = readout.softmax_loss(x, w, labels)
+    dx, _ = readout.softmax_loss_gradient(x, w, labels, normalisers, torch.ones(1, device="cuda"))
+    want = torch.stack([w[i::64].double().sum(0) for i in range(64)]).sum(0) / v
+    assert abs((dx.double() / want - 1).mean().item()) <= bound
