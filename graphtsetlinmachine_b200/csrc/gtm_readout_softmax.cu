@@ -179,6 +179,9 @@ struct Work {
     __device__ __forceinline__ int slice() const { return which == 0 ? split : pair - l.schedule.pair_of((long long)split * l.p[1].blocks); }
 };
 
+// Of exponents of two.  A scale may be so large that this would be infinite, and infinity times the distance zero no number.
+__device__ __forceinline__ float slope_of(float scale) { return fminf(scale * kLog2e, 3.402823466e38f); }
+
 // Softmax statistics of a row, over some of its products at a time.
 struct RowSums {
     float largest, sum;
@@ -489,7 +492,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
                             for (int j = 0; j < 64; j++)
                                 if (j >= left) v[j] = -INFINITY;
                         if (kMode == kSums) {
-                            sums.take(v, l.scale * kLog2e);
+                            sums.take(v, slope_of(l.scale));
                             const long long at = label - column;
                             if (__any_sync(~0u, at >= 0 && at < 64 && label >= 0)) {
                                 float mine = 0.f;
@@ -499,7 +502,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
                                 if (label >= 0 && at >= 0 && at < 64 && real) l.label_logit[row] = mine;
                             }
                         } else {
-                            best.take(v, l.scale * kLog2e, (int)column);
+                            best.take(v, slope_of(l.scale), (int)column);
                         }
                     } else {
 #pragma unroll
@@ -616,13 +619,13 @@ __global__ void __launch_bounds__(kFewThreads) softmax_few_kernel(const FewArgs 
             }
         if (lane < kValues && v0 + my_row < a.labels) {
             const float one[1] = {mine};
-            best.take(one, a.scale * kLog2e, (int)(v0 + my_row));
+            best.take(one, slope_of(a.scale), (int)(v0 + my_row));
         }
     }
     if (lane < kValues) block_best[warp][lane] = best;
     __syncthreads();
     if (threadIdx.x >= kExamples || threadIdx.x >= a.examples) return;
-    const float slope = a.scale * kLog2e;
+    const float slope = slope_of(a.scale);
     RowBest top = RowBest::none();
     for (int w = 0; w < kFewThreads / 32; w++)
         for (int r = 0; r < kRows; r++) {

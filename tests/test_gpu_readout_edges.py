@@ -381,3 +381,18 @@ def test_gradients_of_very_long_sums():
     dx, _ = readout.softmax_loss_gradient(x, w, labels, normalisers, torch.ones(1, device="cuda"))
     want = torch.stack([w[i::64].double().sum(0) for i in range(64)]).sum(0) / v
     assert abs((dx.double() / want - 1).mean().item()) <= bound
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,v", [(20, 300), (2, 300), (20, 10)])
+def test_softmax_of_the_largest_scale(kind, n, v):
+    """Any scale above zero and finite: logits that are equal stay so, however far it would take others."""
+    x, w = torch.zeros(n, 16, device="cuda", dtype=kind), torch.ones(v, 16, device="cuda", dtype=kind)
+    for scale in (1e-38, 1.0, 3.4e38):
+        losses, normalisers = readout.softmax_loss(x, w, torch.zeros(n, dtype=torch.int64, device="cuda"), scale=scale)
+        label, log_probability = readout.softmax_predict(x, w, scale=scale)
+        want = torch.full((n,), math.log(v), device="cuda", dtype=torch.float64)
+        near(losses, want, 2.0 ** -20 * want)
+        near(normalisers, want, 2.0 ** -20 * want)
+        near(log_probability, -want, 2.0 ** -20 * want)
+        assert (label == 0).all()
