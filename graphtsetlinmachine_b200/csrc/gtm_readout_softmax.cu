@@ -14,7 +14,7 @@
 //
 // 16-bit inputs are multiplied as they are, with sums in 32 bits.  32-bit inputs are split into three bf16 parts (24 bits of fraction),
 // and the six products of parts that reach 2^-24 are added, the smallest first.  The tensor cores cut sums off instead of rounding them, about 3e-8 of
-// the sum at every step of 16 elements (1e-7 where all terms have one sign) and always towards zero.  So logits are summed in chunks of up to 256 elements (128 of inputs
+// the sum at every step of 16 elements (1e-7 where all terms have one sign) and always towards zero.  So logits are summed in chunks of up to 320 elements (128 of inputs
 // of 32 bits), which the epilogue adds up in registers, with rounding; and sums for dw and dx of 32-bit inputs go to memory after 512
 // elements, where they are added with rounding.  P is rounded to the operands' type, to as many bits as
 // dx and dw are; fp16 has too small a range for that, so P is scaled by 2^14 over the largest finite |gradient * scale| there (2^-38 of that is the smallest step of P).
@@ -1049,12 +1049,12 @@ Product product_of(int64_t rows, int64_t columns, int64_t depth, int products, i
 }
 
 // Blocks of the index whose products follow each other in tensor memory, for logits.  What the tensor cores cut off a sum grows with the square of its steps, so there
-// are up to four blocks (256 elements, 16 steps), two for 32-bit inputs, and two sums from three blocks on; losses of 16-bit inputs are then as far from 64 bits as
-// those of plain 32-bit products, from 64 to 2,048 columns.  Statistics of 8,192 x 1,024 bf16 and 65,536 labels take 833 us so, 787 in sums of
-// eight blocks, 900 of three: the epilogue reads tensor memory while products write to it.
+// are up to five blocks (320 elements, 20 steps), two for 32-bit inputs, and two sums from three blocks on; losses of 16-bit inputs are then 0.5 to 1.2 times as far from
+// 64 bits as those of plain 32-bit products, from 130 to 2,048 columns.  Statistics of 8,192 x 1,024 bf16 and 65,536 labels take 833 us so (four sums), 814 in three, 787 in two
+// (errors 1.4 times larger), 900 in six: the epilogue reads tensor memory while products write to it.
 int logits_chunk(const Product &p)
 {
-    const int most = p.products == 1 ? 4 : 2, chunks = std::max((p.depth_blocks + most - 1) / most, p.depth_blocks > 2 ? 2 : 1);
+    const int most = p.products == 1 ? 5 : 2, chunks = std::max((p.depth_blocks + most - 1) / most, p.depth_blocks > 2 ? 2 : 1);
     return (p.depth_blocks + chunks - 1) / chunks;
 }
 

@@ -98,8 +98,8 @@ def test_softmax_of_whole_numbers_of_one_sign(kind, n, d, v):
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("n,d,v", [(16, 1024, 300), (16, 32768, 300), (16, 131072, 300), (5, 20000, 40)])
 def test_softmax_of_long_sums_of_one_sign(kind, n, d, v):
-    """What tensor cores cut off a sum of one sign adds up: steps of 16 lose less than 2^-22 of it each, 16 in a chunk of 256 elements (of 32-bit inputs: fewer large
-    ones in a chunk of 128); chunks are added with rounding, 2^-24 each.  The scale leaves one label, so that the normaliser is its logit."""
+    """What tensor cores cut off a sum of one sign adds up: steps of 16 lose less than 2^-22 of the sum so far each, and 20 of a chunk (320 elements; fewer large
+    ones of 32-bit inputs) meet half of its sum on the average, so that 16 times 2^-22 is beyond them; chunks are added with rounding, 2^-24 each.  The scale leaves one label, so that the normaliser is its logit."""
     gen = generator(n + d)
     x, w = normal(gen, n, d).abs().to(kind), (normal(gen, v, d).abs() / 1024).to(kind)
     logits = x.double() @ w.double().t() * 1024.0
