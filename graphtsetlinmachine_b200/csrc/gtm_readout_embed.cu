@@ -94,7 +94,8 @@ __device__ __forceinline__ void accumulate(float2 (&acc)[(V + 1) / 2], const Pac
 }
 
 // Four rows ahead at 28 warps an SM, eight at 20: 72 us and 80 for 819,200 rows of 256 bf16 in bags of 200.  kLong: 64 us (6.6 TB/s, from L2)
-// and 45 for the gradient of 65,539 rows of 512 fp16 in segments of two; otherwise 72 and 33.
+// and 45 for the gradient of 65,539 rows of 512 fp16 in segments of two; otherwise 72 and 33.  At 28 warps a thread has 72 registers, which the bf16 variants of 16-byte loads do
+// not get by with (kLong: up to 400 bytes spilled; fp16 24, fp32 4): fp16 takes 49 us (8.5 TB/s) for what bf16 takes 64.
 constexpr int kGatherThreads = 128, kGatherBlocks = 7;
 
 // A lane has U runs of V columns next to each other, kLanes * V apart.  kLong: segments of several rows, taken one after the other; otherwise rows

@@ -17,7 +17,9 @@
 // the sum at every step of 16 elements (1e-7 where all terms have one sign) and always towards zero.  So logits are summed in chunks of up to 320 elements (128 of inputs
 // of 32 bits), which the epilogue adds up in registers, with rounding; and sums for dw and dx of 32-bit inputs go to memory after 512
 // elements, where they are added with rounding.  P is rounded to the operands' type, to as many bits as
-// dx and dw are; fp16 has too small a range for that, so P is scaled by 2^14 over the largest finite |gradient * scale| there (2^-38 of that is the smallest step of P).
+// dx and dw are (their errors are 1.25 times as large for it on the median of 78 problems, twice for a single example, whose P are all of a sum; P in two parts would
+// double both products); fp16 has too small a range for that, so P is scaled by 2^14 over the largest finite |gradient * scale| there (2^-38 of that is the smallest
+// step of P: an example that weighs 2^-20 of another has fewer bits).
 #include "gtm_readout.cuh"
 #include "gtm_readout_mma.cuh"
 #include "gtm_readout_softmax.h"
@@ -298,8 +300,8 @@ __device__ __forceinline__ void send_32(BoxStore &to, const float (&v)[64], cons
 
 // The product kernel.  A pair of blocks has a tile of 256 x 256: each loads its 128 rows of A and half of B, 32 KB for 64 elements of the sum's index, which
 // the tensor cores take 512 cycles for and shared memory, at 128 bytes a cycle written and read once, as long: both are at their limit, as is, in longer runs, the
-// GPU's power.  A block of 64 takes 0.42 to 0.46 us.  Measured alone (8,192 x 1,024 features, 65,536 labels): statistics 0.74 to 0.94 ms (1.2 to 1.5 PFLOP/s by
-// the clock that the power leaves), P 0.92 to 1.1 ms, both gradients 1.6 to 1.85 ms (1.2 to 1.35).  A sixth stage of the ring, or a seventh, changed nothing.
+// GPU's power.  A block of 64 takes 0.42 to 0.46 us.  Of 8,192 x 1,024 features and 65,536 labels: statistics 0.83 to 1.02 ms (1.1 to 1.3 PFLOP/s by
+// the clock that the power leaves), P 1.24 to 1.35 ms, both gradients 1.85 to 1.99 ms (1.1 to 1.2).  A commit takes 120 cycles of the tensor cores.  A sixth stage of the ring, or a seventh, changed nothing.
 template <int kMode>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax_product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Launch l)
 {
@@ -542,8 +544,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) softmax
     if (warp == 2) tmem_free(tmem, 512);
 }
 
-// The prediction for few examples, whose time is that of reading the weights.  A whole pass over 131,072 x 1,024 bf16 takes 52 us for one example
-// (5.2 TB/s), 60 for two and 90 for four; with the product kernel, most of its rows being outside of the matrix, it takes 67 for any of them.  Dot products
+// The prediction for few examples, whose time is that of reading the weights.  A whole pass over 131,072 x 1,024 bf16 takes 51 us for one example
+// (5.3 TB/s), 58 for two and 90 for four; with the product kernel, most of its rows being outside of the matrix, it takes 74 to 80 for any of them.  Dot products
 // in 32 bits, four rows of weights in a warp at a time (two, and twice the blocks, where the sums of several examples take the registers: 82 us for two
 // examples with four), of every lane 16 bytes (or, where rows start anywhere, an element).  A lane keeps the statistics of one of the rows' products with
 // one example; a block leaves one part.
